@@ -383,6 +383,57 @@ int lbm_vq_remap_codes_i64(int64_t* idx, int64_t N, const int64_t* code_map, int
 /* training/model.py:142-144: perplexity = exp(-sum(p * log(p + 1e-10))), p = hist / sum(hist). out: [1]. */
 int lbm_perplexity_u64(const unsigned long long* hist, float* out, int32_t K, lbm_stream_t stream);
 
+/* ---- scores of the codes, and what is made of them ------------------------------------------------------
+ * The reference decides codes by argmin only (training/model.py:90-95, 152-158); these entry points give the scores themselves, their
+ * gradients, a usage-balance loss over them and a draw from them.  No counterpart in the reference.
+ *
+ * lbm_code_logits_f32: logits[n*ldl + k] = (2 x_n . e_k - |e_k|^2) / temperature -- minus the squared distance over the temperature
+ *   without the row constant |x_n|^2 / temperature.  x, ldx, layout (LBM_VQ_ROWS or LBM_VQ_CHANNEL_MAJOR), S as for lbm_vq_argmin_f32;
+ *   any D >= 1, K >= 1, any 4-byte alignment; e_sqnorm_or_null [K]: taken instead of |e_k|^2 (folded codebooks).
+ *   temperature positive and finite.
+ * lbm_code_logits_grad_f32: gradients of a loss with dL/dlogits = g [N, K] (row stride ldg): dx [N, D] = (2 / temperature) g E and
+ *   de [K, D] = (2 / temperature) (g^T x - diag(column sums of g) E); norm_grad = 0 leaves the second term out (e_sqnorm was given as a
+ *   constant).  Either output may be NULL.  workspace (only for de): lbm_code_logits_grad_workspace_bytes bytes, 16-byte aligned.
+ *   Partial sums are joined in a fixed order: the same input gives the same bits. */
+#define LBM_F32 0
+#define LBM_F16 1
+#define LBM_BF16 2
+int lbm_code_logits_f32(const float* x, int64_t ldx, int32_t layout, int64_t S, const float* codebook, const float* e_sqnorm_or_null,
+                        float* logits, int64_t ldl, int64_t N, int32_t D, int32_t K, double temperature, lbm_stream_t stream);
+size_t lbm_code_logits_grad_workspace_bytes(int64_t N, int32_t D, int32_t K);
+int lbm_code_logits_grad_f32(const float* g, int64_t ldg, const float* x, int64_t ldx, const float* codebook, float* dx_or_null,
+                             float* de_or_null, int32_t norm_grad, void* workspace, int64_t N, int32_t D, int32_t K, double temperature,
+                             lbm_stream_t stream);
+
+/* lbm_code_balance: scores [N, K] of type dtype (LBM_F32 / LBM_F16 / LBM_BF16), row stride lds in scores; K <= 8192.
+ *   codes_or_null: [N, slots] int64 codes picked per row (outside [0, K): not counted); NULL: the best score's code, lowest index first.
+ *   keep_or_null: [N] bytes, 0 = the row does not count (its scores are not read).  A row whose scores are all -inf does not count either.
+ *   Over the M rows that count: mean[k] = mean of softmax(scores)[k], counts[k] = picks of k,
+ *   loss[0] = K * sum_k counts[k] / sum(counts) * mean[k]; all 0 where M = 0.  NaN in a row that counts spreads as softmax spreads it.
+ *   row_stat [N][2] f32 (8-byte aligned) and totals [2] f64 are what lbm_code_balance_grad reads;
+ *   workspace: lbm_code_balance_workspace_bytes bytes, 16-byte aligned (0 = unsupported sizes).  Same input, same bits.
+ * lbm_code_balance_grad: dscores [N, K] (dense, the scores' type) from dL/dloss (g_loss [1]) and dL/dmean (g_mean [K]); NULL = zero.
+ *   counts are constants.  Rows that do not count get zeros. */
+size_t lbm_code_balance_workspace_bytes(int64_t N, int32_t K);
+int lbm_code_balance(const void* scores, int32_t dtype, int64_t lds, const int64_t* codes_or_null, int32_t slots,
+                     const uint8_t* keep_or_null, float* loss, int64_t* counts, float* mean, float* row_stat, double* totals,
+                     void* workspace, int64_t N, int32_t K, lbm_stream_t stream);
+int lbm_code_balance_grad(const void* scores, int32_t dtype, int64_t lds, const float* row_stat, const int64_t* counts,
+                          const double* totals, const float* g_loss_or_null, const float* g_mean_or_null, void* dscores, int64_t N,
+                          int32_t K, lbm_stream_t stream);
+
+/* lbm_code_sample: codes[n] = one code drawn from row n of scores [N, K] (types as above, K <= 8192) with the uniform number u[n] of [0, 1).
+ *   w_k = exp((s_k - max s) / temperature) in 64 bits; top_k > 0 keeps the k best (equal scores: lowest index first); top_p < 1 then keeps, in
+ *   descending order, each code before which less than top_p of the kept weight lies; min_p then keeps w_k >= min_p; the answer is the first
+ *   index whose running sum exceeds u times the total.  temperature 0: the best code, lowest index first.  Each setting is one value, or one
+ *   per row where the *_row pointer is given (a temperature there that is not > 0 means 0, top_k <= 0 and top_p >= 1 mean all).
+ *   allowed_or_null: bytes, 0 = the code may not be drawn; row n at allowed + n * allowed_ld (allowed_ld 0: one mask for all rows).
+ *   Scores of +inf share all the weight; NaN counts as -inf; a row with nothing to draw from answers -1.  hist_or_null [K]: codes are counted into it (ADDED; -1 is not). */
+int lbm_code_sample(const void* scores, int32_t dtype, int64_t lds, const float* u, const float* temperature_row_or_null,
+                    double temperature, const int32_t* top_k_row_or_null, int32_t top_k, const float* top_p_row_or_null, double top_p,
+                    const float* min_p_row_or_null, double min_p, const uint8_t* allowed_or_null, int64_t allowed_ld, int64_t* codes,
+                    unsigned long long* hist_or_null, int64_t N, int32_t K, lbm_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

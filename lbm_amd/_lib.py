@@ -20,8 +20,9 @@ STD_NONE, STD_EPOCH_CHANNEL = 0, 1
 WIN_BOXCAR, WIN_HANN, WIN_HAMMING = 0, 1, 2
 AVG_MEAN, AVG_MEDIAN, AVG_NONE = 0, 1, 2
 VQ_ROWS, VQ_CHANNEL_MAJOR, VQ_NO_XNORM = 0, 1, 2
+SCORE_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}     # LBM_F32 / LBM_F16 / LBM_BF16
 
-_p, _i64, _i32, _f32 = C.c_void_p, C.c_int64, C.c_int32, C.c_float
+_p, _i64, _i32, _f32, _f64 = C.c_void_p, C.c_int64, C.c_int32, C.c_float, C.c_double
 
 # name -> (restype, argtypes); mirrors include/lbm_abi.h one to one
 SIGNATURES = {
@@ -73,6 +74,13 @@ SIGNATURES = {
     "lbm_vq_ema_sums_f32": (C.c_int, [_p, _i64, _p, _p, _p, _p, _i64, _i32, _i32, _p]),
     "lbm_vq_ema_apply_f32": (C.c_int, [_p, _p, _p, _p, _p, _i32, _i32, _f32, _f32, _f32, _p]),
     "lbm_perplexity_u64": (C.c_int, [_p, _p, _i32, _p]),
+    "lbm_code_logits_f32": (C.c_int, [_p, _i64, _i32, _i64, _p, _p, _p, _i64, _i64, _i32, _i32, _f64, _p]),
+    "lbm_code_logits_grad_workspace_bytes": (C.c_size_t, [_i64, _i32, _i32]),
+    "lbm_code_logits_grad_f32": (C.c_int, [_p, _i64, _p, _i64, _p, _p, _p, _i32, _p, _i64, _i32, _i32, _f64, _p]),
+    "lbm_code_balance_workspace_bytes": (C.c_size_t, [_i64, _i32]),
+    "lbm_code_balance": (C.c_int, [_p, _i32, _i64, _p, _i32, _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _p]),
+    "lbm_code_balance_grad": (C.c_int, [_p, _i32, _i64, _p, _p, _p, _p, _p, _p, _i64, _i32, _p]),
+    "lbm_code_sample": (C.c_int, [_p, _i32, _i64, _p, _p, _f64, _p, _i32, _p, _f64, _p, _f64, _p, _i64, _p, _p, _i64, _i32, _p]),
 }
 
 _lib = None

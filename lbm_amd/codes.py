@@ -1,0 +1,267 @@
+"""Scores of the codebook's codes and what is made of them: the scores as a matrix with gradients, a usage-balance loss, and codes drawn
+from the scores.
+
+The reference decides every code by argmin (training/model.py:90-95, 152-158) and only measures collapse (perplexity, :142-144); its
+shipped codebook has 100 codes of 512 that are never used.  ``code_logits`` + ``code_balance_loss`` give training a term that works
+against it (``VectorQuantizerEMA(balance_weight=...)``); ``code_logits`` + ``sample_codes`` tokenize by a draw instead of the argmin
+(``VQVAE.encode(sampling=...)``), and ``sample_codes`` alone draws the next code from any model's scores over codes.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+
+# --------------------------------------------------------------------------------------------------------------- scores
+class _CodeLogits(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, codebook, e_sqnorm, temperature):
+        N, D = x.shape
+        K = codebook.shape[0]
+        out = torch.empty((N, K), dtype=torch.float32, device=x.device)
+        _lib.check(_lib.load().lbm_code_logits_f32(_lib.ptr(x), x.stride(0) if N > 1 else D, _lib.VQ_ROWS, 0, _lib.ptr(codebook),
+                                                   _lib.ptr(e_sqnorm), _lib.ptr(out), K, N, D, K, temperature, _lib.stream_ptr()),
+                   "lbm_code_logits_f32")
+        ctx.save_for_backward(x, codebook)
+        ctx.temperature, ctx.norm_grad = temperature, e_sqnorm is None
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, codebook = ctx.saved_tensors
+        need_x, need_e = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        N, D = x.shape
+        K = codebook.shape[0]
+        if g.stride(1) != 1 or (N > 1 and g.stride(0) < K):
+            g = g.contiguous()
+        lib = _lib.load()
+        dx = torch.empty((N, D), dtype=torch.float32, device=x.device) if need_x else None
+        de = torch.empty((K, D), dtype=torch.float32, device=x.device) if need_e else None
+        ws = torch.empty((lib.lbm_code_logits_grad_workspace_bytes(N, D, K),), dtype=torch.uint8, device=x.device) if need_e else None
+        _lib.check(lib.lbm_code_logits_grad_f32(_lib.ptr(g), g.stride(0) if N > 1 else K, _lib.ptr(x), x.stride(0) if N > 1 else D,
+                                                _lib.ptr(codebook), _lib.ptr(dx), _lib.ptr(de), int(ctx.norm_grad), _lib.ptr(ws), N, D, K,
+                                                ctx.temperature, _lib.stream_ptr()), "lbm_code_logits_grad_f32")
+        return dx, de, None, None
+
+
+def _f32_param(t, what):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        return _lib.dev_f32(t)
+    if not t.is_floating_point():
+        raise ValueError(f"{what} must be a floating-point tensor")
+    return t.to(torch.float32)
+
+
+@_lib.on_tensor_device
+def code_logits(x: torch.Tensor, codebook: torch.Tensor, temperature: float = 1.0, *, e_sqnorm: torch.Tensor = None,
+                channel_major: bool = False) -> torch.Tensor:
+    """Scores of all codes: ``out[n, k] = (2 x_n.e_k - |e_k|^2) / temperature``, float32 [N, K].
+
+    That is minus the squared distance over ``temperature`` up to a constant of the row, so softmax, argmax and every ranking of a row are
+    those of the distances.  ``x``: [N, D] rows (any row stride), or with ``channel_major`` the encoder output z[B, D, S] (N = B*S rows, row
+    n = (n // S, n % S), no permute copy).  Differentiable in ``x`` and ``codebook``; with ``channel_major`` and a gradient to take, the
+    rows are copied first.  ``e_sqnorm`` ([K], as ``fold_projection`` returns it) takes the place of |e_k|^2 as a constant.
+
+    The backward pass reads ``x`` and ``codebook`` as they are then: hand it a copy of a codebook that an EMA step rewrites in between
+    (``vq_ema_apply`` writes through raw pointers, which autograd's version check does not see)."""
+    temperature = float(temperature)
+    if not (temperature > 0.0 and math.isfinite(temperature)):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    x, cb = _f32_param(x, "x"), _f32_param(codebook, "codebook").contiguous()
+    if cb.dim() != 2 or cb.numel() == 0:
+        raise ValueError("codebook must be a non-empty [K, D] tensor")
+    K, D = cb.shape
+    if x.dim() != (3 if channel_major else 2):
+        raise ValueError("x must be [B, D, S] with channel_major" if channel_major else "x must be [N, D]")
+    if x.shape[1] != D:
+        raise ValueError(f"input dim {x.shape[1]} != codebook dim {D}")
+    ee = None
+    if e_sqnorm is not None:
+        ee = _lib.dev_f32(e_sqnorm.detach() if isinstance(e_sqnorm, torch.Tensor) else e_sqnorm)
+        if ee.numel() != K:
+            raise ValueError(f"e_sqnorm has {ee.numel()} entries, the codebook {K}")
+    if channel_major:
+        if torch.is_grad_enabled() and (x.requires_grad or cb.requires_grad):
+            x = x.permute(0, 2, 1).reshape(-1, D)
+        else:
+            from .quantizer import _pitched_rows
+            x, cb = _pitched_rows(x.detach()), cb.detach()
+            B, _, S = x.shape
+            out = torch.empty((B * S, K), dtype=torch.float32, device=x.device)
+            if out.numel():
+                _lib.check(_lib.load().lbm_code_logits_f32(_lib.ptr(x), x.stride(1) if B * D > 1 else S, _lib.VQ_CHANNEL_MAJOR, S,
+                                                           _lib.ptr(cb), _lib.ptr(ee), _lib.ptr(out), K, B * S, D, K, temperature,
+                                                           _lib.stream_ptr()), "lbm_code_logits_f32")
+            return out
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < D):
+        x = x.contiguous()
+    return _CodeLogits.apply(x, cb, ee, temperature)
+
+
+# -------------------------------------------------------------------------------------------------------------- balance
+def _score_rows(scores: torch.Tensor, what: str):
+    """[..., K] scores as rows the kernels address: (tensor [N, K] with unit stride along K, row stride)."""
+    if not isinstance(scores, torch.Tensor):
+        raise ValueError(f"{what}: scores must be a tensor")
+    if scores.dtype not in _lib.SCORE_TYPES:
+        raise ValueError(f"{what}: scores must be float32, float16 or bfloat16, got {scores.dtype}")
+    if scores.dim() < 1 or scores.shape[-1] < 1:
+        raise ValueError(f"{what}: scores must be [..., K] with K >= 1")
+    s = scores if scores.dim() == 2 else scores.reshape(-1, scores.shape[-1])
+    N, K = s.shape
+    if K > 1 and s.stride(1) != 1:
+        s = s.contiguous()
+    return s, (s.stride(0) if N > 1 else K)
+
+
+class _CodeBalance(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, scores, ld, codes, slots, keep):
+        N, K = scores.shape
+        dev = scores.device
+        lib = _lib.load()
+        nbytes = lib.lbm_code_balance_workspace_bytes(N, K)
+        if nbytes == 0:
+            raise NotImplementedError(f"code_balance_loss supports K <= 8192 (got K={K})")
+        ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        mean = torch.empty((K,), dtype=torch.float32, device=dev)
+        counts = torch.empty((K,), dtype=torch.int64, device=dev)
+        stat = torch.empty((N, 2), dtype=torch.float32, device=dev)
+        totals = torch.empty((2,), dtype=torch.float64, device=dev)
+        dtype = _lib.SCORE_TYPES[scores.dtype]
+        _lib.check(lib.lbm_code_balance(_lib.ptr(scores), dtype, ld, _lib.ptr(codes), slots, _lib.ptr(keep), _lib.ptr(loss), _lib.ptr(counts),
+                                        _lib.ptr(mean), _lib.ptr(stat), _lib.ptr(totals), _lib.ptr(ws), N, K, _lib.stream_ptr()),
+                   "lbm_code_balance")
+        ctx.save_for_backward(scores, stat, counts, totals)
+        ctx.ld = ld
+        ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
+        return loss, counts, mean
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_loss, _g_counts, g_mean):
+        scores, stat, counts, totals = ctx.saved_tensors
+        N, K = scores.shape
+        ds = torch.empty((N, K), dtype=scores.dtype, device=scores.device)
+        g_loss = None if g_loss is None else g_loss.to(torch.float32).contiguous()
+        g_mean = None if g_mean is None else g_mean.to(torch.float32).contiguous()
+        _lib.check(_lib.load().lbm_code_balance_grad(_lib.ptr(scores), _lib.SCORE_TYPES[scores.dtype], ctx.ld, _lib.ptr(stat), _lib.ptr(counts),
+                                                     _lib.ptr(totals), _lib.ptr(g_loss), _lib.ptr(g_mean), _lib.ptr(ds), N, K,
+                                                     _lib.stream_ptr()), "lbm_code_balance_grad")
+        return ds, None, None, None, None
+
+
+@_lib.on_tensor_device
+def code_balance_loss(scores: torch.Tensor, codes: torch.Tensor = None, keep: torch.Tensor = None):
+    """Usage balance over rows of scores: ``(loss, counts, mean_probs)``.
+
+    With p = softmax(scores) over the last dimension, over the M rows that count: ``mean_probs[k]`` = mean of p[., k] (float32 [K]),
+    ``counts[k]`` = how often code k was picked (int64 [K]), ``loss = K * sum_k counts[k] / sum(counts) * mean_probs[k]`` (float32 scalar: 1
+    where use is even, up to K where one code takes everything).  Differentiable in ``scores`` through ``loss`` and ``mean_probs`` (an entropy
+    of the latter, say); counts are constants.
+
+    ``scores``: [..., K] float32, float16 or bfloat16 (K <= 8192).  ``codes``: integer [...] or [..., slots], the picks of each row (several for
+    routers that pick several; negative ones, as ``sample_codes`` answers for empty rows, and ones >= K are not counted); without them the
+    best score counts, lowest index first.  ``keep``: bool [...], rows to count (the pipeline's artifact mask, padding); the others' scores are
+    not read and their gradient is 0.  A row of nothing but -inf does not count either.  Where no row counts everything is 0."""
+    s, ld = _score_rows(scores, "code_balance_loss")
+    lead = tuple(scores.shape[:-1])
+    N = s.shape[0]
+    slots = 0
+    if codes is not None:
+        if codes.is_floating_point() or codes.dtype == torch.bool:
+            raise ValueError("code_balance_loss: codes must be integers")
+        if tuple(codes.shape) == lead:
+            slots = 1
+        elif tuple(codes.shape[:-1]) == lead and codes.shape[-1] >= 1:
+            slots = int(codes.shape[-1])
+        else:
+            raise ValueError(f"code_balance_loss: codes {tuple(codes.shape)} do not fit scores {tuple(scores.shape)}")
+        codes = codes.to(device=s.device, dtype=torch.int64).contiguous()
+    if keep is not None:
+        if keep.dtype not in (torch.bool, torch.uint8) or tuple(keep.shape) != lead:
+            raise ValueError(f"code_balance_loss: keep must be a bool tensor of shape {lead}")
+        keep = keep.to(device=s.device).contiguous().view(torch.uint8)
+    return _CodeBalance.apply(s, ld, codes, slots, keep)
+
+
+# ------------------------------------------------------------------------------------------------------------- sampling
+@dataclass
+class CodeSampling:
+    """Settings of a draw (``sample_codes``), for ``VQVAE.encode(sampling=...)``.  The temperature is that of ``exp(-distance / T)``."""
+    temperature: float = 1.0
+    top_k: int = 0
+    top_p: float = 1.0
+    min_p: float = 0.0
+    allowed: Optional[torch.Tensor] = None
+
+
+def _setting(value, name, lead, device, dtype, lo, hi):
+    """(per-row tensor or None, value): a number is checked here, a tensor has one entry per row and is read on the device."""
+    if isinstance(value, torch.Tensor) and value.dim() > 0:
+        if tuple(value.shape) != lead:
+            raise ValueError(f"sample_codes: {name} must be a number or a tensor of shape {lead}, got {tuple(value.shape)}")
+        if dtype is torch.int32 and (value.is_floating_point() or value.dtype == torch.bool):
+            raise ValueError(f"sample_codes: {name} must be integers")
+        if dtype is torch.int32 and value.dtype == torch.int64:
+            value = value.clamp(-1, 2 ** 31 - 1)
+        return value.to(device=device, dtype=dtype).contiguous(), 0
+    v = int(value) if dtype is torch.int32 else float(value)
+    if dtype is torch.int32 and v != value:
+        raise ValueError(f"sample_codes: {name} must be an integer")
+    if not (lo <= v <= hi):
+        raise ValueError(f"sample_codes: {name} = {value} is outside [{lo}, {hi}]")
+    return None, (min(v, 2 ** 31 - 1) if dtype is torch.int32 else v)
+
+
+@torch.no_grad()
+@_lib.on_tensor_device
+def sample_codes(scores: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, allowed: torch.Tensor = None,
+                 hist: torch.Tensor = None) -> torch.Tensor:
+    """One code per row of ``scores`` [..., K], drawn with the uniform numbers ``u`` [...] of [0, 1): int64 [...].
+
+    Weights are exp((s - max s) / ``temperature``) in 64 bits.  ``top_k`` > 0 keeps the k best scores (equal ones: lowest index first);
+    ``top_p`` < 1 then keeps, in descending order, every code before which less than that share of the kept weight lies; ``min_p`` then keeps
+    codes of at least that share of the best code's weight; the answer is the first index whose running sum exceeds u times the total.
+    ``temperature`` 0 answers the best code, lowest index first.  Each setting is a number, or a tensor [...] with one per row (on the
+    device, unchecked: temperatures that are not positive mean 0, top_k <= 0 and top_p >= 1 mean all codes).
+
+    ``scores``: float32, float16 or bfloat16, K <= 8192.  ``allowed``: bool [K] or [..., K], codes that may be drawn.  Scores of +inf share all
+    the weight, NaN counts as -inf; a row with nothing to draw from answers -1.  ``hist`` ([K] int64) is ADDED to when given."""
+    s, ld = _score_rows(scores, "sample_codes")
+    lead = tuple(scores.shape[:-1])
+    N, K = s.shape
+    dev = s.device
+    if not isinstance(u, torch.Tensor) or not u.is_floating_point() or tuple(u.shape) != lead:
+        raise ValueError(f"sample_codes: u must be a floating-point tensor of shape {lead}")
+    u = u.to(device=dev, dtype=torch.float32).contiguous()
+    t_row, t = _setting(temperature, "temperature", lead, dev, torch.float32, 0.0, math.inf)
+    k_row, k = _setting(top_k, "top_k", lead, dev, torch.int32, 0, math.inf)
+    p_row, p = _setting(top_p, "top_p", lead, dev, torch.float32, 0.0, 1.0)
+    m_row, m = _setting(min_p, "min_p", lead, dev, torch.float32, 0.0, 1.0)
+    allowed_ld = 0
+    if allowed is not None:
+        if allowed.dtype not in (torch.bool, torch.uint8):
+            raise ValueError("sample_codes: allowed must be a bool tensor")
+        if tuple(allowed.shape) == (K,):
+            allowed_ld = 0
+        elif tuple(allowed.shape) == tuple(scores.shape):
+            allowed_ld = K
+        else:
+            raise ValueError(f"sample_codes: allowed must be [{K}] or {tuple(scores.shape)}, got {tuple(allowed.shape)}")
+        allowed = allowed.to(device=dev).contiguous().view(torch.uint8)
+    if hist is not None and (hist.dtype != torch.int64 or hist.numel() != K or not hist.is_contiguous()):
+        raise ValueError("hist must be a contiguous int64 tensor of K entries")
+    out = torch.empty((N,), dtype=torch.int64, device=dev)
+    _lib.check(_lib.load().lbm_code_sample(_lib.ptr(s), _lib.SCORE_TYPES[s.dtype], ld, _lib.ptr(u), _lib.ptr(t_row), t, _lib.ptr(k_row), k,
+                                           _lib.ptr(p_row), p, _lib.ptr(m_row), m, _lib.ptr(allowed), allowed_ld, _lib.ptr(out),
+                                           _lib.ptr(hist), N, K, _lib.stream_ptr()), "lbm_code_sample")
+    return out.reshape(lead)

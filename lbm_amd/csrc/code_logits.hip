@@ -1,0 +1,381 @@
+// Scores of every code for every row, and their gradients: three fp32 matrix products on one tile kernel.
+//
+//   s[n, k]  = (2 x_n . e_k - |e_k|^2) / T                 forward   [N, D] x [K, D]^T
+//   dx[n, d] = (2 / T) sum_k g[n, k] e_k[d]                 rows      [N, K] x [K, D]
+//   de[k, d] = (2 / T) (sum_n g[n, k] x_n[d] - c_k e_k[d])  codebook  [N, K]^T x [N, D],  c_k = sum_n g[n, k]
+//
+// s is minus the squared distance over the temperature without its row constant |x_n|^2 / T, which softmax, argmax and every ordering
+// of a row ignore and whose size would only cost the differences their low bits.
+//
+// Bound: the fp32 matrix pipe (64 FLOP per cycle and SIMD) -- an output element costs 2 D FLOP for 4 bytes of store, 128 FLOP per byte at
+// D = 256 against the 20 FLOP per byte where the pipe and HBM balance.  That is also why the scores are stored at all: forming them a second
+// time for the gradient costs more than writing and reading them.
+//
+// Tile: 4 waves, each (TM/2) x (TN/2) outputs in 32 x 32 accumulators of v_mfma_f32_32x32x2_f32 (exact fmaf chains).  The contraction
+// runs 32 steps at a time: operands are requested into registers while the previous 32 steps' products run from LDS.  An operand that is
+// contiguous along the contraction sits in LDS as [row][32 + 4] and is read four steps at a time (ds_read_b128); one that is contiguous
+// along its rows (the codebook in dx, both operands in de, a channel-major x) sits as [step][rows + 2] and is read one step at a time, which
+// the 64-cycle MFMA hides.  Lane half h takes steps h*16 .. h*16 + 15 of both.
+#include "common.h"
+
+namespace {
+
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+
+constexpr int kThreads = 256;
+constexpr int kBK = 32;
+
+enum { KC = 0, MC = 1 };   // operand contiguous along the contraction / along its rows
+
+// Operand `rows x steps`: element (r, k) is p[off(r) + k * ldk] (MC; off(r) = r, or b * pitch + s for channel-major rows r = (b, s)) or
+// p[r * ld + k] (KC).
+struct Operand {
+    const float* p;
+    int64_t ld;       // KC: row stride; MC: stride of one contraction step
+    int64_t S, pitch; // MC: rows r = b * S + s start at b * pitch + s (S = 0: at r)
+    int64_t rows;
+    int vec;          // KC: 16-byte loads allowed (aligned base and row stride)
+};
+
+template <int T, int MODE>
+struct Stage {
+    static constexpr int kPitch = MODE == KC ? kBK + 4 : T + 2;
+    static constexpr int kFloats = MODE == KC ? T * kPitch : kBK * kPitch;
+    static constexpr int kRegs = T * kBK / kThreads;
+    float v[kRegs];
+    const float* base[MODE == KC ? kRegs / 4 : 1];
+    bool ok[MODE == KC ? kRegs / 4 : 1];
+
+    __device__ __forceinline__ void init(const Operand& o, int64_t r0) {
+        if constexpr (MODE == KC) {
+#pragma unroll
+            for (int i = 0; i < kRegs / 4; ++i) {
+                const int64_t r = r0 + (threadIdx.x >> 3) + 32 * i;
+                ok[i] = r < o.rows;
+                base[i] = o.p + (ok[i] ? r : 0) * o.ld + (threadIdx.x & 7) * 4;
+            }
+        } else {
+            const int64_t r = r0 + threadIdx.x % T;
+            ok[0] = r < o.rows;
+            const int64_t rc = ok[0] ? r : 0;
+            base[0] = o.p + (o.S > 0 ? (rc / o.S) * o.pitch + rc % o.S : rc);
+        }
+    }
+    // contraction steps k0 .. k0 + 31, zeros from step kend and for rows past the operand's last
+    __device__ __forceinline__ void load(const Operand& o, int64_t k0, int64_t kend) {
+        if constexpr (MODE == KC) {
+            const int64_t k = k0 + (threadIdx.x & 7) * 4;
+#pragma unroll
+            for (int i = 0; i < kRegs / 4; ++i) {
+                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+                const float* q = base[i] + k0;
+                if (o.vec && k + 3 < kend) {
+                    if (ok[i]) f = *reinterpret_cast<const float4*>(q);
+                } else if (ok[i]) {
+                    if (k < kend) f.x = q[0];
+                    if (k + 1 < kend) f.y = q[1];
+                    if (k + 2 < kend) f.z = q[2];
+                    if (k + 3 < kend) f.w = q[3];
+                }
+                v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+            }
+        } else {
+            const int ks = threadIdx.x / T;
+            const float* q = base[0] + (k0 + ks) * o.ld;
+#pragma unroll
+            for (int i = 0; i < kRegs; ++i) {
+                const int64_t k = k0 + ks + i * (kThreads / T);
+                v[i] = (ok[0] && k < kend) ? q[(int64_t)i * (kThreads / T) * o.ld] : 0.f;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(float* s) const {
+        if constexpr (MODE == KC) {
+#pragma unroll
+            for (int i = 0; i < kRegs / 4; ++i)
+                *reinterpret_cast<float4*>(s + ((threadIdx.x >> 3) + 32 * i) * kPitch + (threadIdx.x & 7) * 4) =
+                    make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kRegs; ++i) s[(threadIdx.x / T + i * (kThreads / T)) * kPitch + threadIdx.x % T] = v[i];
+        }
+    }
+    // four steps (4q .. 4q+3 of this lane half) of row r
+    static __device__ __forceinline__ void frag(const float* s, int r, int h, int q, float* f) {
+        if constexpr (MODE == KC) {
+            const float4 t = *reinterpret_cast<const float4*>(s + r * kPitch + h * 16 + 4 * q);
+            f[0] = t.x; f[1] = t.y; f[2] = t.z; f[3] = t.w;
+        } else {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) f[u] = s[(h * 16 + 4 * q + u) * kPitch + r];
+        }
+    }
+};
+
+enum { EPI_SCORES = 0, EPI_SCALE = 1, EPI_PARTIAL = 2 };
+
+struct Tiles {
+    int64_t mt;     // tiles along the rows of A
+    int nt;         // tiles along the rows of B
+    int splits;     // pieces of the contraction (EPI_PARTIAL)
+    int64_t piece;  // steps of one piece
+};
+
+// out[m, n] over the contraction; EPI_SCORES: out = (2 acc - e_n) * scale, e_n = sqnorm[n] or, where that is NULL, the square sum of B's
+// row n taken from its staged values; EPI_SCALE: out = acc * scale; EPI_PARTIAL: piece z's sums to out[z][m][n] and A's row sums over
+// the piece to rowsum[z][m].
+template <int TM, int TN, int AM, int BM, int EPI>
+__global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand b, float* __restrict__ out, int64_t ldo, int64_t depth,
+                                                              Tiles t, float scale, const float* __restrict__ sqnorm,
+                                                              float* __restrict__ rowsum) {
+    using SA = Stage<TM, AM>;
+    using SB = Stage<TN, BM>;
+    constexpr int MI = TM / 64, NI = TN / 64;
+    __shared__ __align__(16) float s_a[SA::kFloats];
+    __shared__ __align__(16) float s_b[SB::kFloats];
+    __shared__ float s_n[TN];
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int j = lane & 31, h = lane >> 5;
+    const int wm = (wave >> 1) * (TM / 2), wn = (wave & 1) * (TN / 2);
+
+    // workgroups go round the 8 XCDs: give each XCD a contiguous run of tiles, B tiles fastest, so that the tiles that share A's rows
+    // meet in one L2
+    const int64_t total = t.mt * t.nt, per = total / 8, rem = total % 8;
+    const int64_t xcd = blockIdx.x % 8, slot = blockIdx.x / 8;
+    const int64_t tile = xcd * per + (xcd < rem ? xcd : rem) + slot;
+    const int64_t m0 = tile / t.nt * TM, n0 = tile % t.nt * TN;
+    const int64_t kbeg = (int64_t)blockIdx.y * t.piece;
+    const int64_t kend = kbeg + t.piece < depth ? kbeg + t.piece : depth;
+
+    SA sa;
+    SB sb;
+    sa.init(a, m0);
+    sb.init(b, n0);
+    f32x16 acc[MI][NI];
+#pragma unroll
+    for (int x = 0; x < MI; ++x)
+#pragma unroll
+        for (int y = 0; y < NI; ++y)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
+    float sq[EPI == EPI_SCORES ? SB::kRegs / 4 : 1] = {};
+    float asum[MI] = {};
+
+    sa.load(a, kbeg, kend);
+    sb.load(b, kbeg, kend);
+    for (int64_t k0 = kbeg; k0 < kend; k0 += kBK) {
+        __syncthreads();   // the previous steps' fragments are read
+        sa.store(s_a);
+        sb.store(s_b);
+        if constexpr (EPI == EPI_SCORES) {
+#pragma unroll
+            for (int i = 0; i < SB::kRegs / 4; ++i)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) sq[i] = fmaf(sb.v[4 * i + u], sb.v[4 * i + u], sq[i]);
+        }
+        __syncthreads();
+        if (k0 + kBK < kend) {
+            sa.load(a, k0 + kBK, kend);
+            sb.load(b, k0 + kBK, kend);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float fa[MI][4], fb[NI][4];
+#pragma unroll
+            for (int x = 0; x < MI; ++x) SA::frag(s_a, wm + 32 * x + j, h, q, fa[x]);
+#pragma unroll
+            for (int y = 0; y < NI; ++y) SB::frag(s_b, wn + 32 * y + j, h, q, fb[y]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int x = 0; x < MI; ++x)
+#pragma unroll
+                    for (int y = 0; y < NI; ++y)
+                        acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[x][u], fb[y][u], acc[x][y], 0, 0, 0);
+            if constexpr (EPI == EPI_PARTIAL) {
+#pragma unroll
+                for (int x = 0; x < MI; ++x) asum[x] += (fa[x][0] + fa[x][1]) + (fa[x][2] + fa[x][3]);
+            }
+        }
+    }
+
+    if constexpr (EPI == EPI_SCORES) {
+        if (sqnorm != nullptr) {
+            if (threadIdx.x < TN) s_n[threadIdx.x] = n0 + threadIdx.x < b.rows ? sqnorm[n0 + threadIdx.x] : 0.f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < SB::kRegs / 4; ++i) {
+                float s = sq[i];   // the eight lanes that staged one row of B
+                s += __shfl_xor(s, 1, 64);
+                s += __shfl_xor(s, 2, 64);
+                s += __shfl_xor(s, 4, 64);
+                if ((threadIdx.x & 7) == 0) s_n[(threadIdx.x >> 3) + 32 * i] = s;
+            }
+        }
+        __syncthreads();
+    }
+    if constexpr (EPI == EPI_PARTIAL) {
+        out += (int64_t)blockIdx.y * a.rows * ldo;
+        if (n0 == 0 && wn == 0) {
+#pragma unroll
+            for (int x = 0; x < MI; ++x) {
+                const float s = asum[x] + __shfl_xor(asum[x], 32, 64);
+                const int64_t m = m0 + wm + 32 * x + j;
+                if (h == 0 && m < a.rows) rowsum[(int64_t)blockIdx.y * a.rows + m] = s;
+            }
+        }
+    }
+#pragma unroll
+    for (int x = 0; x < MI; ++x)
+#pragma unroll
+        for (int y = 0; y < NI; ++y) {
+            const int nl = wn + 32 * y + j;
+            const int64_t n = n0 + nl;
+            if (n < b.rows) {
+                const float e = EPI == EPI_SCORES ? s_n[nl] : 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int64_t m = m0 + wm + 32 * x + (r & 3) + 8 * (r >> 2) + 4 * h;
+                    if (m < a.rows) {
+                        float v = acc[x][y][r];
+                        if constexpr (EPI == EPI_SCORES) v = (2.f * v - e) * scale;
+                        if constexpr (EPI == EPI_SCALE) v = v * scale;
+                        out[m * ldo + n] = v;
+                    }
+                }
+            }
+        }
+}
+
+// de[k, d] = scale * (sum_z part[z][k][d] - (sum_z rowsum[z][k]) * e[k][d]); pieces in order
+__global__ __launch_bounds__(256) void code_grad_join_kernel(const float* __restrict__ part, const float* __restrict__ rowsum,
+                                                             const float* __restrict__ codebook, float* __restrict__ de, int splits,
+                                                             int64_t K, int64_t D, float scale, int with_norm) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= K * D) return;
+    const int64_t k = i / D;
+    double s = 0.0, c = 0.0;
+    for (int z = 0; z < splits; ++z) s += (double)part[(int64_t)z * K * D + i];
+    if (with_norm) {
+        for (int z = 0; z < splits; ++z) c += (double)rowsum[(int64_t)z * K + k];
+        s -= c * (double)codebook[i];
+    }
+    de[i] = (float)(s * (double)scale);
+}
+
+bool aligned16(const float* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
+
+template <int AM, int BM, int EPI>
+int launch_mm(const char* what, const Operand& a, const Operand& b, float* out, int64_t ldo, int64_t depth, int splits, int64_t piece,
+              float scale, const float* sqnorm, float* rowsum, hipStream_t st) {
+    // 128 x 128 tiles while they fill the 256 CUs; 64 x 64 (a quarter of the work each) below that
+    const int64_t big = ((a.rows + 127) / 128) * ((b.rows + 127) / 128) * splits;
+    const int T = big >= 256 ? 128 : 64;
+    Tiles t;
+    t.mt = (a.rows + T - 1) / T;
+    t.nt = (int)((b.rows + T - 1) / T);
+    t.splits = splits;
+    t.piece = piece;
+    const int64_t blocks = t.mt * t.nt;
+    if (blocks > 0x7fffffffLL) return lbm::fail(LBM_EUNSUPPORTED, "%s: grid too large", what);
+    const dim3 grid((unsigned)blocks, (unsigned)splits);
+    if (T == 128)
+        hipLaunchKernelGGL((code_mm_kernel<128, 128, AM, BM, EPI>), grid, dim3(kThreads), 0, st, a, b, out, ldo, depth, t, scale, sqnorm, rowsum);
+    else
+        hipLaunchKernelGGL((code_mm_kernel<64, 64, AM, BM, EPI>), grid, dim3(kThreads), 0, st, a, b, out, ldo, depth, t, scale, sqnorm, rowsum);
+    return lbm::check_launch(what);
+}
+
+constexpr int64_t kMaxPiece = 32768;   // rows of one fp32 accumulator chain in the codebook's gradient; pieces are joined in 64 bits
+
+// pieces of the N rows: enough tiles for two rounds of the chip, at least 128 rows each
+void plan_split(int64_t N, int32_t D, int32_t K, int* splits, int64_t* piece) {
+    const int64_t tiles = (((int64_t)K + 127) / 128) * (((int64_t)D + 127) / 128);
+    int64_t s = (512 + tiles - 1) / tiles;
+    if (s > (N + 127) / 128) s = (N + 127) / 128;
+    if (s < (N + kMaxPiece - 1) / kMaxPiece) s = (N + kMaxPiece - 1) / kMaxPiece;
+    if (s < 1) s = 1;
+    int64_t p = (N + s - 1) / s;
+    p = (p + kBK - 1) / kBK * kBK;
+    if (p < kBK) p = kBK;
+    *piece = p;
+    *splits = (int)((N + p - 1) / p);
+    if (*splits < 1) *splits = 1;
+}
+
+}  // namespace
+
+extern "C" int lbm_code_logits_f32(const float* x, int64_t ldx, int32_t layout, int64_t S, const float* codebook,
+                                   const float* e_sqnorm_or_null, float* logits, int64_t ldl, int64_t N, int32_t D, int32_t K,
+                                   double temperature, lbm_stream_t stream) {
+    const char* what = "lbm_code_logits_f32";
+    LBM_REQUIRE(N >= 0 && D >= 1 && K >= 1, LBM_EINVAL, "%s: bad sizes (N=%lld D=%d K=%d)", what, (long long)N, D, K);
+    LBM_REQUIRE(temperature > 0.0 && temperature < INFINITY, LBM_EINVAL, "%s: temperature must be positive and finite", what);
+    LBM_REQUIRE(layout == LBM_VQ_ROWS || layout == LBM_VQ_CHANNEL_MAJOR, LBM_EINVAL, "%s: unknown layout %d", what, layout);
+    if (N == 0) return LBM_OK;
+    LBM_REQUIRE(x && codebook && logits, LBM_EINVAL, "%s: NULL pointer", what);
+    LBM_REQUIRE(ldl >= K, LBM_EINVAL, "%s: ldl (%lld) < K (%d)", what, (long long)ldl, K);
+    if (layout == LBM_VQ_ROWS)
+        LBM_REQUIRE(ldx >= D, LBM_EINVAL, "%s: ldx (%lld) < D (%d)", what, (long long)ldx, D);
+    else
+        LBM_REQUIRE(S >= 1 && ldx >= S && N % S == 0, LBM_EINVAL,
+                    "%s: channel-major needs 1 <= S <= ldx and N %% S == 0 (N=%lld, S=%lld, ldx=%lld)", what, (long long)N, (long long)S,
+                    (long long)ldx);
+    const Operand b{codebook, D, 0, 0, K, aligned16(codebook, D)};
+    const float scale = (float)(1.0 / temperature);
+    if (layout == LBM_VQ_ROWS) {
+        const Operand a{x, ldx, 0, 0, N, aligned16(x, ldx)};
+        return launch_mm<KC, KC, EPI_SCORES>(what, a, b, logits, ldl, D, 1, D, scale, e_sqnorm_or_null, nullptr, lbm::as_stream(stream));
+    }
+    const Operand a{x, ldx, S, (int64_t)D * ldx, N, 0};
+    return launch_mm<MC, KC, EPI_SCORES>(what, a, b, logits, ldl, D, 1, D, scale, e_sqnorm_or_null, nullptr, lbm::as_stream(stream));
+}
+
+extern "C" size_t lbm_code_logits_grad_workspace_bytes(int64_t N, int32_t D, int32_t K) {
+    if (N < 0 || D < 1 || K < 1) return 0;
+    int splits;
+    int64_t piece;
+    plan_split(N, D, K, &splits, &piece);
+    return (size_t)splits * (size_t)K * (size_t)(D + 1) * sizeof(float);
+}
+
+extern "C" int lbm_code_logits_grad_f32(const float* g, int64_t ldg, const float* x, int64_t ldx, const float* codebook, float* dx_or_null,
+                                        float* de_or_null, int32_t norm_grad, void* workspace, int64_t N, int32_t D, int32_t K,
+                                        double temperature, lbm_stream_t stream) {
+    const char* what = "lbm_code_logits_grad_f32";
+    LBM_REQUIRE(N >= 0 && D >= 1 && K >= 1, LBM_EINVAL, "%s: bad sizes (N=%lld D=%d K=%d)", what, (long long)N, D, K);
+    LBM_REQUIRE(temperature > 0.0 && temperature < INFINITY, LBM_EINVAL, "%s: temperature must be positive and finite", what);
+    LBM_REQUIRE(codebook && (N == 0 || g), LBM_EINVAL, "%s: NULL pointer", what);
+    LBM_REQUIRE(N == 0 || ldg >= K, LBM_EINVAL, "%s: ldg (%lld) < K (%d)", what, (long long)ldg, K);
+    LBM_REQUIRE(de_or_null == nullptr || ((N == 0 || x) && workspace), LBM_EINVAL, "%s: the codebook's gradient needs x and a workspace", what);
+    LBM_REQUIRE(de_or_null == nullptr || N == 0 || ldx >= D, LBM_EINVAL, "%s: ldx (%lld) < D (%d)", what, (long long)ldx, D);
+    LBM_REQUIRE(((uintptr_t)workspace & 15) == 0, LBM_EINVAL, "%s: workspace must be 16-byte aligned", what);
+    hipStream_t st = lbm::as_stream(stream);
+    const float scale = (float)(2.0 / temperature);
+    if (dx_or_null != nullptr && N > 0) {
+        const Operand a{g, ldg, 0, 0, N, aligned16(g, ldg)};
+        const Operand b{codebook, D, 0, 0, D, 0};
+        const int rc = launch_mm<KC, MC, EPI_SCALE>(what, a, b, dx_or_null, D, K, 1, K, scale, nullptr, nullptr, st);
+        if (rc != LBM_OK) return rc;
+    }
+    if (de_or_null != nullptr) {
+        int splits = 0;
+        int64_t piece = kBK;
+        float* part = static_cast<float*>(workspace);
+        float* rowsum = part;
+        if (N > 0) {
+            plan_split(N, D, K, &splits, &piece);
+            rowsum = part + (int64_t)splits * K * D;
+            const Operand a{g, ldg, 0, 0, K, 0};
+            const Operand b{x, ldx, 0, 0, D, 0};
+            const int rc = launch_mm<MC, MC, EPI_PARTIAL>(what, a, b, part, D, N, splits, piece, 1.f, nullptr, rowsum, st);
+            if (rc != LBM_OK) return rc;
+        }
+        const int64_t total = (int64_t)K * D;
+        hipLaunchKernelGGL(code_grad_join_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, part, rowsum, codebook, de_or_null,
+                           splits, K, D, scale, norm_grad);
+        return lbm::check_launch(what);
+    }
+    return LBM_OK;
+}

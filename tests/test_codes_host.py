@@ -1,0 +1,137 @@
+"""Refusals of the code-score operators (code_logits, code_balance_loss, sample_codes) and of their C entry points: no GPU, no launch."""
+import math
+
+import pytest
+import torch
+
+import lbm_amd
+from lbm_amd import _lib
+
+EINVAL, EUNSUPPORTED = -1, -2
+P = 4096      # stands for a device pointer in calls that are refused before it is used
+
+
+def _err():
+    return _lib.load().lbm_last_error().decode()
+
+
+def _logits(x=P, ldx=8, layout=0, S=0, cb=P, ee=None, out=P, ldl=16, N=4, D=8, K=16, T=1.0):
+    return _lib.load().lbm_code_logits_f32(x, ldx, layout, S, cb, ee, out, ldl, N, D, K, T, None)
+
+
+@pytest.mark.parametrize("kw", [dict(N=-1), dict(D=0), dict(K=0), dict(T=0.0), dict(T=-1.0), dict(T=math.inf), dict(T=math.nan), dict(layout=2),
+                                dict(layout=-1), dict(x=None), dict(cb=None), dict(out=None), dict(ldl=15), dict(ldx=7),
+                                dict(layout=1, S=0), dict(layout=1, S=3), dict(layout=1, S=4, ldx=3)])
+def test_logits_entry_refuses(kw):
+    assert _logits(**kw) == EINVAL and "lbm_code_logits_f32" in _err()
+
+
+def test_logits_entry_empty():
+    assert _logits(N=0, x=None, out=None) == 0
+
+
+def _grad(g=P, ldg=16, x=P, ldx=8, cb=P, dx=P, de=P, norm=1, ws=P, N=4, D=8, K=16, T=1.0):
+    return _lib.load().lbm_code_logits_grad_f32(g, ldg, x, ldx, cb, dx, de, norm, ws, N, D, K, T, None)
+
+
+@pytest.mark.parametrize("kw", [dict(N=-1), dict(D=0), dict(K=0), dict(T=0.0), dict(T=math.nan), dict(g=None), dict(cb=None), dict(ldg=15),
+                                dict(x=None), dict(ws=None), dict(ldx=7), dict(ws=P + 8)])
+def test_logits_grad_entry_refuses(kw):
+    assert _grad(**kw) == EINVAL and "lbm_code_logits_grad_f32" in _err()
+
+
+def test_logits_grad_entry_without_outputs():
+    assert _grad(dx=None, de=None, x=None, ws=None) == 0
+    assert _lib.load().lbm_code_logits_grad_workspace_bytes(-1, 8, 16) == 0
+    assert _lib.load().lbm_code_logits_grad_workspace_bytes(0, 8, 16) > 0
+
+
+def _balance(s=P, dt=0, lds=16, codes=P, slots=1, keep=None, loss=P, counts=P, mean=P, stat=P, tot=P, ws=P, N=4, K=16):
+    return _lib.load().lbm_code_balance(s, dt, lds, codes, slots, keep, loss, counts, mean, stat, tot, ws, N, K, None)
+
+
+@pytest.mark.parametrize("kw,rc", [(dict(N=-1), EINVAL), (dict(K=0), EINVAL), (dict(K=8193), EUNSUPPORTED), (dict(dt=3), EINVAL),
+                                   (dict(dt=-1), EINVAL), (dict(s=None), EINVAL), (dict(loss=None), EINVAL), (dict(counts=None), EINVAL),
+                                   (dict(mean=None), EINVAL), (dict(stat=None), EINVAL), (dict(stat=P + 4), EINVAL), (dict(tot=None), EINVAL),
+                                   (dict(ws=None), EINVAL), (dict(ws=P + 8), EINVAL), (dict(lds=-16), EINVAL), (dict(slots=0), EINVAL)])
+def test_balance_entry_refuses(kw, rc):
+    assert _balance(**kw) == rc and "lbm_code_balance" in _err()
+
+
+def _balance_grad(s=P, dt=0, lds=16, stat=P, counts=P, tot=P, gl=P, gm=P, ds=P, N=4, K=16):
+    return _lib.load().lbm_code_balance_grad(s, dt, lds, stat, counts, tot, gl, gm, ds, N, K, None)
+
+
+@pytest.mark.parametrize("kw,rc", [(dict(N=-1), EINVAL), (dict(K=0), EINVAL), (dict(K=8193), EUNSUPPORTED), (dict(dt=7), EINVAL),
+                                   (dict(s=None), EINVAL), (dict(stat=None), EINVAL), (dict(counts=None), EINVAL), (dict(tot=None), EINVAL),
+                                   (dict(ds=None), EINVAL), (dict(lds=-1), EINVAL)])
+def test_balance_grad_entry_refuses(kw, rc):
+    assert _balance_grad(**kw) == rc and "lbm_code_balance_grad" in _err()
+
+
+def test_balance_grad_entry_empty():
+    assert _balance_grad(N=0, s=None, stat=None, ds=None) == 0
+    lib = _lib.load()
+    assert lib.lbm_code_balance_workspace_bytes(1, 8193) == 0 and lib.lbm_code_balance_workspace_bytes(-1, 8) == 0
+    assert lib.lbm_code_balance_workspace_bytes(0, 8) > 0
+
+
+def _sample(s=P, dt=0, lds=16, u=P, tr=None, t=1.0, kr=None, k=0, pr=None, p=1.0, mr=None, m=0.0, al=None, ald=0, out=P, hist=None, N=4, K=16):
+    return _lib.load().lbm_code_sample(s, dt, lds, u, tr, t, kr, k, pr, p, mr, m, al, ald, out, hist, N, K, None)
+
+
+@pytest.mark.parametrize("kw,rc", [(dict(N=-1), EINVAL), (dict(K=0), EINVAL), (dict(K=8193), EUNSUPPORTED), (dict(dt=3), EINVAL),
+                                   (dict(t=-0.5), EINVAL), (dict(t=math.nan), EINVAL), (dict(k=-1), EINVAL), (dict(p=-0.1), EINVAL),
+                                   (dict(p=1.1), EINVAL), (dict(p=math.nan), EINVAL), (dict(m=-0.1), EINVAL), (dict(m=1.5), EINVAL),
+                                   (dict(s=None), EINVAL), (dict(u=None), EINVAL), (dict(out=None), EINVAL), (dict(lds=-16), EINVAL),
+                                   (dict(al=P, ald=-16), EINVAL), (dict(N=1 << 31), EUNSUPPORTED)])
+def test_sample_entry_refuses(kw, rc):
+    assert _sample(**kw) == rc and "lbm_code_sample" in _err()
+
+
+def test_sample_entry_empty():
+    assert _sample(N=0, s=None, u=None, out=None) == 0
+
+
+# ---- the Python surface: every refusal comes before a tensor is touched, so CPU tensors do
+S = torch.zeros((4, 16))
+U = torch.zeros((4,))
+
+
+@pytest.mark.parametrize("call", [
+    lambda: lbm_amd.sample_codes(S, torch.zeros((5,))),
+    lambda: lbm_amd.sample_codes(S, torch.zeros((4,), dtype=torch.int64)),
+    lambda: lbm_amd.sample_codes(S.double(), U),
+    lambda: lbm_amd.sample_codes(torch.zeros((4, 0)), U),
+    lambda: lbm_amd.sample_codes(S, U, temperature=-1.0),
+    lambda: lbm_amd.sample_codes(S, U, temperature=math.nan),
+    lambda: lbm_amd.sample_codes(S, U, temperature=torch.ones((3,))),
+    lambda: lbm_amd.sample_codes(S, U, top_k=-1),
+    lambda: lbm_amd.sample_codes(S, U, top_k=2.5),
+    lambda: lbm_amd.sample_codes(S, U, top_k=torch.ones((4,))),
+    lambda: lbm_amd.sample_codes(S, U, top_p=1.5),
+    lambda: lbm_amd.sample_codes(S, U, min_p=-0.1),
+    lambda: lbm_amd.sample_codes(S, U, allowed=torch.ones((15,), dtype=torch.bool)),
+    lambda: lbm_amd.sample_codes(S, U, allowed=torch.ones((16,))),
+    lambda: lbm_amd.sample_codes(S, U, hist=torch.zeros((16,))),
+    lambda: lbm_amd.code_balance_loss(S.double()),
+    lambda: lbm_amd.code_balance_loss([1.0, 2.0]),
+    lambda: lbm_amd.code_balance_loss(S, torch.zeros((4,))),
+    lambda: lbm_amd.code_balance_loss(S, torch.zeros((3,), dtype=torch.int64)),
+    lambda: lbm_amd.code_balance_loss(S, torch.zeros((4, 0), dtype=torch.int64)),
+    lambda: lbm_amd.code_balance_loss(S, keep=torch.ones((4,))),
+    lambda: lbm_amd.code_balance_loss(S, keep=torch.ones((3,), dtype=torch.bool)),
+    lambda: lbm_amd.code_logits(S, S, temperature=0.0),
+    lambda: lbm_amd.code_logits(S, S, temperature=math.inf),
+])
+def test_python_surface_refuses(call):
+    with pytest.raises(ValueError):
+        call()
+
+
+def test_python_surface_refuses_cpu_tensors():
+    for call in (lambda: lbm_amd.sample_codes(S, U), lambda: lbm_amd.code_balance_loss(S)):
+        with pytest.raises(_lib.LbmError, match="CUDA/ROCm"):
+            call()
+    with pytest.raises(NotImplementedError, match="8192"):
+        lbm_amd.code_balance_loss(torch.zeros((1, 8193)))
