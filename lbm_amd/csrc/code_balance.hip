@@ -82,9 +82,9 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void balance_rows_kernel(con
             m = fmaxf(m, v[i]);
             nan |= v[i] != v[i];
         }
-        m = lbm::team_reduce<float, W>(m, s_f, rf, OpMax());
+        m = lbm::team_join<float, W>(lbm::wave_best(m), s_f, rf, OpMax());
         if (m == -INFINITY) {                            // nothing but -inf (does not count) or NaN (its sums are NaN, as softmax's)
-            const int any = lbm::team_reduce<int, W>(nan ? 1 : 0, s_i, ri, OpMax());
+            const int any = lbm::team_join<int, W>(__any(nan) ? 1 : 0, s_i, ri, OpMax());
             if (any == 0) {
                 if (t == 0) stat[row] = make_float2(0.f, 0.f);
                 continue;
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void balance_rows_kernel(con
             e[i] = lbm::exp_f32(v[i] - m);
             s += e[i];
         }
-        s = lbm::team_reduce<float, W>(s, s_f, rf, OpAdd());
+        s = lbm::team_join<float, W>(lbm::wave_total(s), s_f, rf, OpAdd());
         const float r = 1.f / s;
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = fmaf(e[i], r, acc[i]);
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void balance_rows_kernel(con
             int best = 0x7fffffff;                       // lowest column that holds the maximum
 #pragma unroll
             for (int i = V - 1; i >= 0; --i) best = v[i] == m ? ((i >> 2) * 64 * W + t) * 4 + (i & 3) : best;
-            best = lbm::team_reduce<int, W>(best, s_i, ri, OpMin());
+            best = lbm::team_join<int, W>(lbm::wave_first(best), s_i, ri, OpMin());
             if (t == 0 && best < K) atomicAdd(&s_cnt[best], 1u);
         }
     }
@@ -238,14 +238,14 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void balance_grad_kernel(con
             lbm::load_row<T, V, W>(scores + row * lds, K, t, vec, v);
 #pragma unroll
             for (int i = 0; i < V; ++i) ref = v[i] == m ? fmaxf(ref, a[i]) : ref;
-            ref = lbm::team_reduce<float, W>(ref, s_f, rf, OpMax());
+            ref = lbm::team_join<float, W>(lbm::wave_best(ref), s_f, rf, OpMax());
             float dot = 0.f;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 d[i] = lbm::exp_f32(v[i] - m) * r;
                 dot = fmaf(d[i], a[i] - ref, dot);
             }
-            dot = lbm::team_reduce<float, W>(dot, s_f, rf, OpAdd());
+            dot = lbm::team_join<float, W>(lbm::wave_total(dot), s_f, rf, OpAdd());
 #pragma unroll
             for (int i = 0; i < V; ++i) d[i] = d[i] * ((a[i] - ref) - dot) * inv_m;
         }

@@ -55,31 +55,43 @@ __device__ __forceinline__ void load_row(const T* __restrict__ row, int K, int t
     }
 }
 
-// reductions over a team, the result in every thread.  W = 1: one wave, no barrier.  W > 1: the team is the workgroup; s holds two rounds
-// of W values and `round` alternates between them, so one barrier per reduction suffices (a slot is rewritten only after the next one).
-template <typename A, int W, typename Op>
-__device__ __forceinline__ A team_reduce(A v, A* s, int& round, Op op) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o, 64));
-    if constexpr (W > 1) {
-        A* slot = s + round * W;
-        round ^= 1;
-        if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = v;
-        __syncthreads();
-        v = slot[0];
-#pragma unroll
-        for (int w = 1; w < W; ++w) v = op(v, slot[w]);
-    }
-    return v;
+// Sums and maxima over a wave by DPP moves (4 shifts inside rows of 16 lanes, 2 row broadcasts), no LDS.  All 64 lanes must be active.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_move(float old, float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(old), __float_as_int(x), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_move(int old, int x) {
+    return __builtin_amdgcn_update_dpp(old, x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_move(double old, double x) {
+    return __hiloint2double(dpp_move<CTRL, ROWS>(__double2hiint(old), __double2hiint(x)),
+                            dpp_move<CTRL, ROWS>(__double2loint(old), __double2loint(x)));
+}
+__device__ __forceinline__ float lane_value(float x, int lane) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane)); }
+__device__ __forceinline__ int lane_value(int x, int lane) { return __builtin_amdgcn_readlane(x, lane); }
+__device__ __forceinline__ double lane_value(double x, int lane) {
+    return __hiloint2double(lane_value(__double2hiint(x), lane), lane_value(__double2loint(x), lane));
+}
+// inclusive running value over the lanes; `none` is op's neutral element
+template <typename A, typename Op>
+__device__ __forceinline__ A wave_scan(A x, A none, Op op) {
+    x = op(x, dpp_move<0x111, 0xf>(none, x));
+    x = op(x, dpp_move<0x112, 0xf>(none, x));
+    x = op(x, dpp_move<0x114, 0xf>(none, x));
+    x = op(x, dpp_move<0x118, 0xf>(none, x));
+    x = op(x, dpp_move<0x142, 0xa>(none, x));
+    x = op(x, dpp_move<0x143, 0xc>(none, x));
+    return x;
 }
 
-struct OpMax {
-    template <typename A>
-    __device__ __forceinline__ A operator()(A a, A b) const { return a > b ? a : b; }
+struct OpMax {      // floats: NaN loses
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+    __device__ __forceinline__ int operator()(int a, int b) const { return a > b ? a : b; }
 };
 struct OpMin {
-    template <typename A>
-    __device__ __forceinline__ A operator()(A a, A b) const { return a < b ? a : b; }
+    __device__ __forceinline__ int operator()(int a, int b) const { return a < b ? a : b; }
 };
 struct OpAdd {
     template <typename A>
@@ -94,6 +106,27 @@ __device__ __forceinline__ float exp_f32(float x) {
     const float r = fmaf(x, kLog2eLo, fmaf(x, kLog2e, -t));
     const float e = __builtin_amdgcn_exp2f(t);
     return fmaf(e, r * kLn2, e);
+}
+
+template <typename A>
+__device__ __forceinline__ A wave_total(A x) { return lane_value(wave_scan<A>(x, A(0), OpAdd()), 63); }
+__device__ __forceinline__ float wave_best(float x) { return lane_value(wave_scan<float>(x, -INFINITY, OpMax()), 63); }
+__device__ __forceinline__ int wave_first(int x) { return lane_value(wave_scan<int>(x, 0x7fffffff, OpMin()), 63); }
+
+// one value per wave of a workgroup of W waves -> all of them, through s ([2][W] in LDS, `round` alternates between the halves: one barrier
+// per exchange, since a half is rewritten only after the next exchange's barrier)
+template <typename A, int W, typename Op>
+__device__ __forceinline__ A team_join(A x, A* s, int& round, Op op) {
+    if constexpr (W > 1) {
+        A* slot = s + round * W;
+        round ^= 1;
+        if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = x;
+        __syncthreads();
+        x = slot[0];
+#pragma unroll
+        for (int w = 1; w < W; ++w) x = op(x, slot[w]);
+    }
+    return x;
 }
 
 }  // namespace lbm
