@@ -422,13 +422,14 @@ int lbm_code_balance_grad(const void* scores, int32_t dtype, int64_t lds, const 
                           const double* totals, const float* g_loss_or_null, const float* g_mean_or_null, void* dscores, int64_t N,
                           int32_t K, lbm_stream_t stream);
 
-/* lbm_code_sample: codes[n] = one code drawn from row n of scores [N, K] (types as above, K <= 8192) with the uniform number u[n] of [0, 1).
+/* lbm_code_sample: codes[n] = one code drawn from row n of scores [N, K] (types as above, K <= 2^24) with the uniform number u[n] of [0, 1).
  *   w_k = exp((s_k - max s) / temperature) in 64 bits; top_k > 0 keeps the k best (equal scores: lowest index first); top_p < 1 then keeps, in
  *   descending order, each code before which less than top_p of the kept weight lies; min_p then keeps w_k >= min_p; the answer is the first
  *   index whose running sum exceeds u times the total.  temperature 0: the best code, lowest index first.  Each setting is one value, or one
  *   per row where the *_row pointer is given (a temperature there that is not > 0 means 0, top_k <= 0 and top_p >= 1 mean all).
  *   allowed_or_null: bytes, 0 = the code may not be drawn; row n at allowed + n * allowed_ld (allowed_ld 0: one mask for all rows).
- *   Scores of +inf share all the weight; NaN counts as -inf; a row with nothing to draw from answers -1.  hist_or_null [K]: codes are counted into it (ADDED; -1 is not). */
+ *   Scores of +inf share all the weight; NaN counts as -inf; a row with nothing to draw from answers -1.  hist_or_null [K], K <= 32768: codes are counted into it (ADDED;
+ *   -1 is not). */
 int lbm_code_sample(const void* scores, int32_t dtype, int64_t lds, const float* u, const float* temperature_row_or_null,
                     double temperature, const int32_t* top_k_row_or_null, int32_t top_k, const float* top_p_row_or_null, double top_p,
                     const float* min_p_row_or_null, double min_p, const uint8_t* allowed_or_null, int64_t allowed_ld, int64_t* codes,

@@ -234,8 +234,8 @@ def sample_codes(scores: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_
     ``temperature`` 0 answers the best code, lowest index first.  Each setting is a number, or a tensor [...] with one per row (on the
     device, unchecked: temperatures that are not positive mean 0, top_k <= 0 and top_p >= 1 mean all codes).
 
-    ``scores``: float32, float16 or bfloat16, K <= 8192.  ``allowed``: bool [K] or [..., K], codes that may be drawn.  Scores of +inf share all
-    the weight, NaN counts as -inf; a row with nothing to draw from answers -1.  ``hist`` ([K] int64) is ADDED to when given."""
+    ``scores``: float32, float16 or bfloat16.  ``allowed``: bool [K] or [..., K], codes that may be drawn.  Scores of +inf share all
+    the weight, NaN counts as -inf; a row with nothing to draw from answers -1.  ``hist`` ([K] int64, K <= 32768) is ADDED to when given."""
     s, ld = _score_rows(scores, "sample_codes")
     lead = tuple(scores.shape[:-1])
     N, K = s.shape

@@ -54,50 +54,35 @@ __device__ __forceinline__ double exp2_f64(double t) {
     return ldexp(p, (int)n);
 }
 
-// A row in the registers of a team of W waves, V scores a thread; slots ascend by chunk of 256 W, thread, i.
-template <int V, int W>
+// Scores in the registers of one wave, V a lane; slots ascend by chunk of 256, lane, i.
+template <int V>
 struct Row {
     float v[V];           // -inf once a code is out
     double w[V];
-    int t;                // thread of the team
-    double* s_d;          // LDS, W > 1: [2][W], [2][W], [V / 4][W]
-    int* s_i;
-    double* s_tot;
-    int rd = 0, ri = 0;
 
-    __device__ __forceinline__ int slot(int i) const { return ((i >> 2) * 64 * W + t) * 4 + (i & 3); }
-    __device__ __forceinline__ int lane() const { return threadIdx.x & 63; }
-    __device__ __forceinline__ int wave() const { return W == 1 ? 0 : (int)(threadIdx.x >> 6); }
+    static __device__ __forceinline__ int lane() { return threadIdx.x & 63; }
+    static __device__ __forceinline__ int slot(int i) { return ((i >> 2) * 64 + lane()) * 4 + (i & 3); }
 
-    __device__ __forceinline__ int join(int c) { return lbm::team_join<int, W>(c, s_i, ri, lbm::OpAdd()); }
-    __device__ __forceinline__ double sum(double x) { return lbm::team_join<double, W>(lbm::wave_total(x), s_d, rd, lbm::OpAdd()); }
-    __device__ __forceinline__ float best(float x) {
-        x = lbm::wave_best(x);
-        if constexpr (W > 1) x = __int_as_float(lbm::team_join<int, W>(__float_as_int(x), s_i, ri, [](int a, int b) {
-            return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b)));
-        }));
-        return x;
-    }
-    __device__ __forceinline__ int count_from(float x) {          // scores >= x
+    __device__ __forceinline__ int count_from(float x) const {    // scores >= x
         int c = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) c += __popcll(__ballot(v[i] >= x));
-        return join(c);
+        return c;
     }
-    __device__ __forceinline__ int count_equal(float x) {
+    __device__ __forceinline__ int count_equal(float x) const {
         int c = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) c += __popcll(__ballot(v[i] == x));
-        return join(c);
+        return c;
     }
-    __device__ __forceinline__ double weight_above(float x) {
+    __device__ __forceinline__ double weight_above(float x) const {
         double s = 0.0;
 #pragma unroll
         for (int i = 0; i < V; ++i) s += v[i] > x ? w[i] : 0.0;
-        return sum(s);
+        return lbm::wave_total(s);
     }
     // fp32 weight (from the copies wf) and number of the scores >= x
-    __device__ __forceinline__ float probe(const float* wf, float x, int* n) {
+    __device__ __forceinline__ float probe(const float* wf, float x, int* n) const {
         float s = 0.f;
         int c = 0;
 #pragma unroll
@@ -106,29 +91,27 @@ struct Row {
             s += in ? wf[i] : 0.f;
             c += __popcll(__ballot(in));
         }
-        s = lbm::wave_total(s);
-        if constexpr (W > 1) {                                    // both in one exchange
-            const double both = lbm::team_join<double, W>(__hiloint2double(c, __float_as_int(s)), s_d, rd, [](double a, double b) {
-                return __hiloint2double(__double2hiint(a) + __double2hiint(b),
-                                        __float_as_int(__int_as_float(__double2loint(a)) + __int_as_float(__double2loint(b))));
-            });
-            c = __double2hiint(both);
-            s = __int_as_float(__double2loint(both));
-        }
         *n = c;
-        return s;
+        return lbm::wave_total(s);
     }
-    __device__ __forceinline__ float next_below(float x) {
+    __device__ __forceinline__ float next_below(float x) const {
         float b = -INFINITY;
 #pragma unroll
         for (int i = 0; i < V; ++i) b = fmaxf(b, v[i] < x ? v[i] : -INFINITY);
-        return best(b);
+        return lbm::wave_best(b);
     }
-    __device__ __forceinline__ float next_above(float x) {
+    // lowest score >= x
+    __device__ __forceinline__ float next_from(float x) const {
+        float b = -INFINITY;                                      // of the negatives
+#pragma unroll
+        for (int i = 0; i < V; ++i) b = fmaxf(b, v[i] >= x ? -v[i] : -INFINITY);
+        return -lbm::wave_best(b);
+    }
+    __device__ __forceinline__ float next_above(float x) const {
         float b = -INFINITY;                                      // of the negatives
 #pragma unroll
         for (int i = 0; i < V; ++i) b = fmaxf(b, v[i] > x ? -v[i] : -INFINITY);
-        return -best(b);
+        return -lbm::wave_best(b);
     }
     __device__ __forceinline__ void drop_below(float x) {
 #pragma unroll
@@ -146,19 +129,7 @@ struct Row {
 #pragma unroll
             for (int i = 0; i < 4; ++i) mine += v[4 * c + i] == x ? 1 : 0;
             const int scan = lbm::wave_scan<int>(mine, 0, lbm::OpAdd());
-            int before = base + scan - mine, total = lbm::lane_value(scan, 63);
-            if constexpr (W > 1) {
-                int* s = s_i + ri * W;
-                ri ^= 1;
-                if (lane() == 0) s[wave()] = total;
-                __syncthreads();
-                total = 0;
-#pragma unroll
-                for (int q = 0; q < W; ++q) {
-                    if (q < wave()) before += s[q];
-                    total += s[q];
-                }
-            }
+            int before = base + scan - mine;
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (v[4 * c + i] == x) {
@@ -168,7 +139,7 @@ struct Row {
                     }
                     ++before;
                 }
-            base += total;
+            base += lbm::lane_value(scan, 63);
         }
     }
     // m: the best score; c = log2(e) / T
@@ -181,50 +152,49 @@ struct Row {
             for (int i = 0; i < V; ++i) w[i] = exp2_f64(((double)v[i] - (double)m) * c);
         }
     }
-    __device__ __forceinline__ double weight() {
+    __device__ __forceinline__ double weight() const {
         double s = 0.0;
 #pragma unroll
         for (int i = 0; i < V; ++i) s += w[i];
-        return sum(s);
+        return lbm::wave_total(s);
     }
 };
 
-constexpr int kByValue = 12;             // steps that halve by value; 32 by bit pattern end the search whatever the scores
-constexpr int kSteps = kByValue + 32;
+constexpr int kByValue = 10;             // trial scores that halve by value; then by ordered bit pattern, which 32 end whatever the scores
+constexpr int kSteps = 64;
 
-// trial score of step `it` strictly inside (lo, hi); false when no number lies between
-__device__ __forceinline__ bool trial(int it, float lo, float hi, float* mid) {
+// trial score of (lo, hi]: lo < hi
+__device__ __forceinline__ float trial(int it, float lo, float hi) {
     if (it < kByValue) {
-        *mid = 0.5f * lo + 0.5f * hi;
-        if (*mid > lo && *mid < hi) return true;
+        const float mid = 0.5f * lo + 0.5f * hi;
+        if (mid > lo && mid <= hi) return mid;
     }
     const unsigned kl = order_key(lo), kh = order_key(hi);
-    if (kh - kl <= 1u) return false;
-    *mid = key_score(kl + (kh - kl) / 2);
-    return true;
+    return key_score(kl + (kh - kl + 1u) / 2);
 }
 
-// the k best scores stay; lo: the lowest score, m: the best one
-template <int V, int W>
-__device__ __forceinline__ void keep_top_k(Row<V, W>& R, float lo, float m, int k) {
-    int c = R.count_from(m);
-    float b = m;
-    if (c < k) {
-        float hi = m;                    // fewer than k from hi on
-        c = 0;
-        for (int it = 0; it < kSteps; ++it) {
-            float mid;
-            if (!trial(it, lo, hi, &mid)) break;
-            c = R.count_from(mid);
-            if (c >= k) lo = mid;
-            else hi = mid;
-            if (c == k) break;
+// the k best scores stay; lo: a score at or below all of them, m: the best one
+template <int V>
+__device__ __forceinline__ void keep_top_k(Row<V>& R, float lo, float m, int k) {
+    float hi = m;                        // the border is one of the scores in [lo, hi]
+    int c = 0;
+    for (int it = 0; it < kSteps && lo < hi; ++it) {
+        const float mid = it == 0 ? hi : trial(it, lo, hi);
+        c = R.count_from(mid);
+        if (c >= k) lo = mid;
+        else hi = it < kByValue ? mid : R.next_below(mid);
+        if (c == k || (it == 0 && c >= k)) break;
+        if (it >= kByValue - 1) {        // from here on between scores that are there: equal ones end the search
+            hi = it == kByValue - 1 ? R.next_below(hi) : hi;
+            lo = R.next_from(lo);
         }
-        b = lo;
-        if (c != k) c = R.count_from(b);
     }
-    if (c > k) R.keep_first_equal(b, k - (c - R.count_equal(b)));
-    R.drop_below(b);
+    if (c != k) c = R.count_from(lo);
+    if (c > k) {
+        lo = R.next_from(lo);
+        R.keep_first_equal(lo, k - (c - R.count_equal(lo)));
+    }
+    R.drop_below(lo);
 }
 
 // scores below this one weigh together less than (1 - p) of a total that is 1 at least: K exp((s - m) / T) < 1 - p, with room for the rounding
@@ -234,18 +204,18 @@ __device__ __forceinline__ float top_p_floor(float m, float lo, double temp, dou
 }
 
 // the codes of the smallest descending prefix that reaches `target` stay; the scores >= lo reach it, lo <= m
-template <int V, int W>
-__device__ __forceinline__ void keep_top_p(Row<V, W>& R, float lo, float m, double target, double c) {
+template <int V>
+__device__ __forceinline__ void keep_top_p(Row<V>& R, float lo, float m, double target, double c) {
     float wf[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) wf[i] = (float)R.w[i];
-    float l = lo, hi = m, b = m;
+    float l = lo, hi = m, b = m;         // the target is reached at l and not at hi
     int n_hi;
     if (R.probe(wf, m, &n_hi) < (float)target) {
-        for (int it = 0; it < kSteps; ++it) {
-            float mid;
+        for (int it = 0; it < kByValue; ++it) {
+            const float mid = trial(it, l, hi);
+            if (mid >= hi) break;
             int n;
-            if (!trial(it, l, hi, &mid)) break;
             if (R.probe(wf, mid, &n) >= (float)target) {
                 l = mid;
                 if (n - n_hi == 1) break;
@@ -255,6 +225,13 @@ __device__ __forceinline__ void keep_top_p(Row<V, W>& R, float lo, float m, doub
             }
         }
         b = R.next_below(hi);
+        l = R.next_from(l);
+        for (int it = kByValue; it < kSteps && l < b; ++it) {     // between scores that are there: equal ones end the search
+            const float mid = trial(it, l, b);
+            int n;
+            if (R.probe(wf, mid, &n) >= (float)target) l = R.next_from(mid);
+            else b = R.next_below(mid);
+        }
     }
     // the 64-bit sums decide: above b lies less than the target, with b's scores at least it
     double above = 0.0, wb = 1.0;
@@ -277,18 +254,13 @@ __device__ __forceinline__ void keep_top_p(Row<V, W>& R, float lo, float m, doub
         }
     }
     if (!settled) {                      // fp32 sums led too far astray (a border among weights below 1e-7 of the total): search on the 64-bit sums
-        l = lo;
-        hi = m;
-        for (int it = 0; it < kSteps; ++it) {
-            float mid;
-            if (!trial(it, l, hi, &mid)) break;
-            double s = 0.0;
-#pragma unroll
-            for (int i = 0; i < V; ++i) s += R.v[i] >= mid ? R.w[i] : 0.0;
-            if (R.sum(s) >= target) l = mid;
-            else hi = mid;
+        l = R.next_from(lo);
+        b = m;
+        for (int it = 0; it < kSteps && l < b; ++it) {
+            const float mid = trial(it, l, b);
+            if (R.weight_above(R.next_below(mid)) >= target) l = R.next_from(mid);
+            else b = R.next_below(mid);
         }
-        b = R.next_below(hi);
         above = R.weight_above(b);
         eq = R.count_equal(b);
         wb = exp2_f64(((double)b - (double)m) * c);
@@ -299,64 +271,50 @@ __device__ __forceinline__ void keep_top_p(Row<V, W>& R, float lo, float m, doub
     R.drop_below(b);
 }
 
+// four weights at lane `first` that carry a running sum past the goal: which of them does (its last one where rounding keeps all from it)
+__device__ __forceinline__ int crossing(double run, double goal, const double* w4, int first) {
+    int at = 0;
+    bool done = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const double w = lbm::lane_value(w4[i], first);
+        run += w;
+        if (!done && w > 0.0) {
+            at = i;
+            done = run > goal;
+        }
+    }
+    return at;
+}
+
 // the slot the draw falls on
-template <int V, int W>
-__device__ __forceinline__ int draw(Row<V, W>& R, double u) {
-    double inc[V / 4], s4[V / 4], base[V / 4], total = 0.0;
+template <int V>
+__device__ __forceinline__ int draw(Row<V>& R, double u) {
+    double inc[V / 4], s4[V / 4], total = 0.0;
 #pragma unroll
     for (int c = 0; c < V / 4; ++c) {
         s4[c] = (R.w[4 * c] + R.w[4 * c + 1]) + (R.w[4 * c + 2] + R.w[4 * c + 3]);
         inc[c] = lbm::wave_scan<double>(s4[c], 0.0, lbm::OpAdd());
-    }
-    if constexpr (W == 1) {
-#pragma unroll
-        for (int c = 0; c < V / 4; ++c) {
-            base[c] = total;
-            total += lbm::lane_value(inc[c], 63);
-        }
-    } else {
-        if (R.lane() == 63)
-#pragma unroll
-            for (int c = 0; c < V / 4; ++c) R.s_tot[c * W + R.wave()] = inc[c];
-        __syncthreads();
-#pragma unroll
-        for (int c = 0; c < V / 4; ++c)
-#pragma unroll
-            for (int q = 0; q < W; ++q) {
-                if (q == R.wave()) base[c] = total;
-                total += R.s_tot[c * W + q];
-            }
+        total += lbm::lane_value(inc[c], 63);
     }
     const double goal = u * total;
-    int hit = 0x7fffffff;
+    double base = 0.0;
+    int hit = -1;
 #pragma unroll
     for (int c = 0; c < V / 4; ++c) {
-        const unsigned long long over = __ballot(base[c] + inc[c] > goal && s4[c] > 0.0);
-        if (hit == 0x7fffffff && over != 0) {
+        const unsigned long long over = __ballot(base + inc[c] > goal && s4[c] > 0.0);
+        if (hit < 0 && over != 0) {
             const int first = __ffsll((long long)over) - 1;
-            // in that lane: the first weight that carries the sum past the goal, or its last one where rounding keeps all from it
-            double run = base[c] + (first == 0 ? 0.0 : lbm::lane_value(inc[c], first == 0 ? 0 : first - 1));
-            int at = 0;
-            bool done = false;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const double w = lbm::lane_value(R.w[4 * c + i], first);
-                run += w;
-                if (!done && w > 0.0) {
-                    at = i;
-                    done = run > goal;
-                }
-            }
-            hit = (c * 64 * W + R.wave() * 64 + first) * 4 + at;
+            const double run = base + (first == 0 ? 0.0 : lbm::lane_value(inc[c], first == 0 ? 0 : first - 1));
+            hit = (c * 64 + first) * 4 + crossing(run, goal, R.w + 4 * c, first);
         }
+        base += lbm::lane_value(inc[c], 63);
     }
-    hit = lbm::team_join<int, W>(hit, R.s_i, R.ri, lbm::OpMin());
-    if (hit == 0x7fffffff) {             // u of 1 or more, or NaN: the last code that stayed
+    if (hit < 0) {                       // u of 1 or more, or NaN: the last code that stayed
         int last = -1;
 #pragma unroll
         for (int i = 0; i < V; ++i) last = R.w[i] > 0.0 ? R.slot(i) : last;
-        last = -lbm::wave_first(-last);
-        hit = lbm::team_join<int, W>(last, R.s_i, R.ri, lbm::OpMax());
+        hit = -lbm::wave_first(-last);
     }
     return hit;
 }
@@ -364,21 +322,38 @@ __device__ __forceinline__ int draw(Row<V, W>& R, double u) {
 struct Setting {
     double temp, c, top_p, min_p, u;
     int top_k;
+    bool by_k, by_p;
 };
 
-// everything behind the best score m; lo: the lowest score above -inf; total: the weight top-p refers to where it is not that of this row's
-// own scores (negative: it is)
-template <int V, int W>
-__device__ __forceinline__ int settle(Row<V, W>& R, const Setting& s, float lo, float m, int K, bool weighed, double total) {
-    if (s.top_k > 0 && s.top_k < K) keep_top_k<V, W>(R, lo, m, s.top_k);
-    if (!weighed) R.weigh(m, s.c);
-    if (s.top_p < 1.0) {
-        if (total < 0.0) total = R.weight();
+__device__ __forceinline__ Setting row_setting(const Params& par, const float* u, int64_t row, int K) {
+    Setting s;
+    s.temp = par.T_row != nullptr ? (double)par.T_row[row] : par.T;
+    s.c = fmin(1.4426950408889634 / s.temp, 1e300);
+    s.top_p = par.p_row != nullptr ? (double)par.p_row[row] : par.top_p;
+    s.min_p = par.min_row != nullptr ? (double)par.min_row[row] : par.min_p;
+    s.top_k = par.k_row != nullptr ? par.k_row[row] : par.top_k;
+    s.u = (double)u[row];
+    s.by_k = s.top_k > 0 && s.top_k < K;
+    s.by_p = s.top_p < 1.0;
+    return s;
+}
+
+// everything behind the best score m; lo: a score at or below all others; total: the weight that top-p refers to where the scores here are
+// not all of them (negative: they are).  -1: they do not reach top-p's share of that total.
+template <int V>
+__device__ __forceinline__ int settle(Row<V>& R, const Setting& s, float lo, float m, int K, double total) {
+    if (s.by_k) keep_top_k<V>(R, lo, m, s.top_k);
+    R.weigh(m, s.c);
+    if (s.by_p) {
+        const double here = R.weight();
+        if (total < 0.0) total = here;
+        const double target = s.top_p * total;
+        if (here < target) return -1;
         if (m == INFINITY) {             // equal weights of 1
-            const double keep = ceil(s.top_p * total);
+            const double keep = ceil(target);
             R.keep_first_equal(m, keep < 1.0 ? 1 : (int)keep);
         } else {
-            keep_top_p<V, W>(R, top_p_floor(m, lo, s.temp, s.top_p, K), m, s.top_p * total, s.c);
+            keep_top_p<V>(R, top_p_floor(m, lo, s.temp, s.top_p, K), m, target, s.c);
         }
     }
     if (s.min_p > 0.0) {
@@ -386,41 +361,25 @@ __device__ __forceinline__ int settle(Row<V, W>& R, const Setting& s, float lo, 
 #pragma unroll
         for (int i = 0; i < V; ++i) R.w[i] = R.w[i] >= lim ? R.w[i] : 0.0;
     }
-    return draw<V, W>(R, s.u);
+    return draw<V>(R, s.u);
 }
 
-constexpr int kCand = 512;               // scores one wave finishes alone (8 a lane)
-
-template <typename T, int V, int W>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void code_sample_kernel(const T* __restrict__ scores, int64_t lds, int vec,
-                                                                           const float* __restrict__ u, Params par,
-                                                                           const uint8_t* __restrict__ allowed, int64_t allowed_ld,
-                                                                           int64_t* __restrict__ out, int64_t N, int K) {
-    __shared__ double s_d[2 * W];
-    __shared__ int s_i[2 * W];
-    __shared__ double s_tot[V / 4 * W];
-    const int team = W == 1 ? threadIdx.x >> 6 : 0;
-    const int64_t row = (int64_t)blockIdx.x * (W == 1 ? 4 : 1) + team;
-    if (row >= N) return;                // W = 1: a whole wave, and no barriers follow
-    Row<V, W> R;
-    R.t = W == 1 ? threadIdx.x & 63 : threadIdx.x;
-    R.s_d = s_d;
-    R.s_i = s_i;
-    R.s_tot = s_tot;
-    lbm::load_row<T, V, W>(scores + row * lds, K, R.t, vec, R.v);
+// K <= 64 V: the whole row in registers
+template <typename T, int V>
+__global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ scores, int64_t lds, int vec, const float* __restrict__ u,
+                                                          Params par, const uint8_t* __restrict__ allowed, int64_t allowed_ld,
+                                                          int64_t* __restrict__ out, int64_t N, int K) {
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= N) return;                // a whole wave
+    Row<V> R;
+    lbm::load_row<T, V, 1>(scores + row * lds, K, R.lane(), vec, R.v);
     if (allowed != nullptr) {
         const uint8_t* a = allowed + row * allowed_ld;
 #pragma unroll
         for (int i = 0; i < V; ++i)
             if (R.slot(i) < K && a[R.slot(i)] == 0) R.v[i] = -INFINITY;
     }
-    Setting s;
-    s.temp = par.T_row != nullptr ? (double)par.T_row[row] : par.T;
-    s.top_p = par.p_row != nullptr ? (double)par.p_row[row] : par.top_p;
-    s.min_p = par.min_row != nullptr ? (double)par.min_row[row] : par.min_p;
-    s.top_k = par.k_row != nullptr ? par.k_row[row] : par.top_k;
-    s.u = (double)u[row];
-
+    const Setting s = row_setting(par, u, row, K);
     float m = -INFINITY, lo = INFINITY;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -428,24 +387,376 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void code_sample_kernel(cons
         m = fmaxf(m, R.v[i]);
         lo = fminf(lo, R.v[i] == -INFINITY ? INFINITY : R.v[i]);
     }
-    m = R.best(m);
+    m = lbm::wave_best(m);
+    int hit;
     if (m == -INFINITY) {
-        if (R.t == 0) out[row] = -1;
-        return;
-    }
-    if (!(s.temp > 0.0)) {
+        hit = -1;
+    } else if (!(s.temp > 0.0)) {
         int first = 0x7fffffff;
 #pragma unroll
         for (int i = V - 1; i >= 0; --i) first = R.v[i] == m ? R.slot(i) : first;
-        first = lbm::team_join<int, W>(lbm::wave_first(first), R.s_i, R.ri, lbm::OpMin());
-        if (R.t == 0) out[row] = first;
-        return;
+        hit = lbm::wave_first(first);
+    } else {
+        if (s.by_k || s.by_p) lo = -lbm::wave_best(-lo);
+        hit = settle<V>(R, s, lo, m, K, -1.0);
     }
-    s.c = fmin(1.4426950408889634 / s.temp, 1e300);
-    const bool by_k = s.top_k > 0 && s.top_k < K;
-    if (by_k || s.top_p < 1.0) lo = -R.best(-lo);
-    const int hit = settle<V, W>(R, s, lo, m, K, false, -1.0);
-    if (R.t == 0) out[row] = hit;
+    if (R.lane() == 0) out[row] = hit;
+}
+
+// ---- longer rows: one wave still, which reads the row in chunks of 256 and keeps only what can be drawn.
+//
+// 512 samples of the row give a score t that a few hundred scores reach; one pass takes the best score, the total weight where top-p asks for
+// it, and the scores >= t with their columns into LDS, where they are a short row again: up to 512 in registers (8 a lane), up to kCand by
+// passes over LDS.  The pass is repeated with a corrected t where too many or too few came, and a row whose nucleus does not fit (or that has
+// no filter at all) is answered by the same passes over memory.  No barrier anywhere: rows do not wait for each other.
+constexpr int kReg = 512, kCand = 1536;
+
+// passes over scores of a row, in memory or taken into LDS
+template <typename S>
+struct Passes {
+    static __device__ __forceinline__ int lane() { return threadIdx.x & 63; }
+    __device__ __forceinline__ const S& self() const { return *static_cast<const S*>(this); }
+
+    // f(four scores, slot of the first) in index order across calls
+    template <typename F>
+    __device__ __forceinline__ void each(F f) const {
+#pragma unroll 4
+        for (int c = 0; c < self().n; c += 256) {
+            float q[4];
+            self().four(c + lane() * 4, q);
+            f(q, c + lane() * 4);
+        }
+    }
+    // scores above x and equal to it
+    __device__ void counts(float x, int* above, int* equal) const {
+        int a = 0, e = 0;
+        each([&](const float* q, int) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a += q[i] > x ? 1 : 0, e += q[i] == x ? 1 : 0;
+        });
+        *above = lbm::wave_total(a);
+        *equal = lbm::wave_total(e);
+    }
+    __device__ double weight_above(float x, float m, double c) const {
+        double s = 0.0;
+        each([&](const float* q, int) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s += q[i] > x ? exp2_f64(((double)q[i] - (double)m) * c) : 0.0;
+        });
+        return lbm::wave_total(s);
+    }
+    // the highest score x with reached(scores >= x): one of those in [lo, hi], reached(lo).  add(q) is summed over the scores >= the trial.
+    template <typename A, typename Add, typename Reached>
+    __device__ __forceinline__ float border(float lo, float hi, Add add, Reached reached) const {
+        for (int it = 0; it < kSteps && lo < hi; ++it) {
+            const float mid = it == 0 ? hi : trial(it, lo, hi);
+            A sum = A(0);
+            float from = -INFINITY, below = -INFINITY;            // from: of the negatives
+            each([&](const float* q, int) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = q[i] >= mid;
+                    sum += in ? add(q[i]) : A(0);
+                    from = fmaxf(from, in ? -q[i] : -INFINITY);
+                    below = fmaxf(below, in ? -INFINITY : q[i]);
+                }
+            });
+            if (reached(lbm::wave_total(sum))) lo = -lbm::wave_best(from);
+            else hi = lbm::wave_best(below);
+        }
+        return lo;
+    }
+    // slot of the j-th (from 0) score equal to x; -1: there are fewer
+    __device__ int nth_equal(float x, int j) const {
+        for (int c = 0; c < self().n; c += 256) {
+            float q[4];
+            self().four(c + lane() * 4, q);
+            int mine = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mine += q[i] == x ? 1 : 0;
+            const int scan = lbm::wave_scan<int>(mine, 0, lbm::OpAdd()), here = lbm::lane_value(scan, 63);
+            if (j < here) {
+                int before = scan - mine, at = 0x7fffffff;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (q[i] == x && before++ == j) at = c + lane() * 4 + i;
+                return lbm::wave_first(at);
+            }
+            j -= here;
+        }
+        return -1;
+    }
+};
+
+template <typename T>
+struct Memory : Passes<Memory<T>> {
+    const T* row;
+    const uint8_t* allowed;
+    int n, vec;
+
+    __device__ __forceinline__ float one(int col) const {
+        const float f = lbm::score_to_f32<T>(row[col]) + 0.f;
+        return f != f || (allowed != nullptr && allowed[col] == 0) ? -INFINITY : f;
+    }
+    __device__ __forceinline__ void four(int col, float* f) const {       // -inf past the row's end
+        if (vec && col < n) {
+            const lbm::Quad<T> q = *reinterpret_cast<const lbm::Quad<T>*>(row + col);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = lbm::score_to_f32<T>(q.v[i]) + 0.f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = col + i < n ? lbm::score_to_f32<T>(row[col + i]) + 0.f : -INFINITY;
+        }
+        if (allowed != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (col + i < n && allowed[col + i] == 0) f[i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = f[i] != f[i] ? -INFINITY : f[i];
+    }
+};
+
+struct Taken : Passes<Taken> {
+    const float* val;     // LDS
+    int n;
+    __device__ __forceinline__ void four(int at, float* f) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = at + i < n ? val[at + i] : -INFINITY;
+    }
+};
+
+// the draw by passes; lo, m: lowest and best score; total as for settle (-1 likewise)
+template <typename S>
+__device__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, int K, double total) {
+    int above, equal;
+    if (m == INFINITY) {                 // equal weights of 1
+        R.counts(m, &above, &equal);
+        double n = s.by_k && s.top_k < equal ? s.top_k : equal;
+        if (s.by_p) n = fmax(1.0, ceil(s.top_p * n));
+        const double j = floor(s.u * n);
+        return R.nth_equal(m, j >= 0.0 && j < n ? (int)j : (s.u < 0.0 ? 0 : (int)n - 1));
+    }
+    auto weight = [&](float q) { return exp2_f64(((double)q - (double)m) * s.c); };
+    // what stays: scores above b and the first `keep` of those equal to it
+    float b = -INFINITY;
+    int keep = 0;
+    if (s.by_k) {
+        b = R.template border<int>(lo, m, [](float) { return 1; }, [&](int c) { return c >= s.top_k; });
+        R.counts(b, &above, &equal);
+        keep = s.top_k - above < equal ? s.top_k - above : equal;
+    }
+    double here = R.weight_above(b, m, s.c) + (b == -INFINITY ? 0.0 : keep * weight(b));
+    if (s.by_p) {
+        const double target = s.top_p * (total < 0.0 ? here : total);
+        if (here < target) return -1;
+        const float l = fmaxf(b == -INFINITY ? lo : b, top_p_floor(m, lo, s.temp, s.top_p, K));
+        const float x = R.template border<double>(l, m, weight, [&](double w) { return w >= target; });
+        if (x > b) {
+            b = x;
+            R.counts(b, &above, &equal);
+            keep = equal;
+        }
+        const double over = R.weight_above(b, m, s.c), wb = weight(b), n = ceil((target - over) / wb);
+        keep = n >= 1.0 ? (n < keep ? (int)n : keep) : 1;
+        here = over + keep * wb;
+    }
+    const double lim = s.min_p > 0.0 ? fmin(s.min_p, 1.0) : 0.0;
+    // weights that stay, four at a time; `seen` counts the equals of b so far
+    auto weights = [&](const float* q, double* w, int& seen) {
+        int mine = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine += q[i] == b ? 1 : 0;
+        const int scan = lbm::wave_scan<int>(mine, 0, lbm::OpAdd());
+        int before = seen + scan - mine;
+        seen += lbm::lane_value(scan, 63);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool in = q[i] > b || (q[i] == b && before < keep);
+            before += q[i] == b ? 1 : 0;
+            w[i] = weight(q[i]);
+            w[i] = in && w[i] >= lim ? w[i] : 0.0;
+        }
+    };
+    if (lim > 0.0) {
+        double sum = 0.0;
+        int seen = 0;
+        R.each([&](const float* q, int) {
+            double w[4];
+            weights(q, w, seen);
+            sum += (w[0] + w[1]) + (w[2] + w[3]);
+        });
+        here = lbm::wave_total(sum);
+    }
+    const double goal = s.u * here;
+    double base = 0.0;
+    int seen = 0, last = -1;
+    for (int c = 0; c < R.n; c += 256) {
+        float q[4];
+        double w[4];
+        R.four(c + R.lane() * 4, q);
+        weights(q, w, seen);
+        const double s4 = (w[0] + w[1]) + (w[2] + w[3]);
+        const double inc = lbm::wave_scan<double>(s4, 0.0, lbm::OpAdd());
+        const unsigned long long over = __ballot(base + inc > goal && s4 > 0.0);
+        if (over != 0) {
+            const int first = __ffsll((long long)over) - 1;
+            const double run = base + (first == 0 ? 0.0 : lbm::lane_value(inc, first == 0 ? 0 : first - 1));
+            return c + first * 4 + crossing(run, goal, w, first);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) last = w[i] > 0.0 ? c + R.lane() * 4 + i : last;
+        base += lbm::lane_value(inc, 63);
+    }
+    return -lbm::wave_first(-last);      // u of 1 or more, NaN, or a goal that rounding keeps out of reach: the last code that stayed
+}
+
+constexpr float kLowest = -3.402823466e+38f;
+
+template <typename T>
+__global__ __launch_bounds__(256) void code_sample_long_kernel(const T* __restrict__ scores, int64_t lds, int vec, const float* __restrict__ u,
+                                                               Params par, const uint8_t* __restrict__ allowed, int64_t allowed_ld,
+                                                               int64_t* __restrict__ out, int64_t N, int K) {
+    __shared__ float s_val[4][kCand];
+    __shared__ int s_col[4][kCand];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+    if (row >= N) return;                // a whole wave
+    Memory<T> S;
+    S.row = scores + row * lds;
+    S.allowed = allowed != nullptr ? allowed + row * allowed_ld : nullptr;
+    S.n = K;
+    S.vec = vec;
+    const Setting s = row_setting(par, u, row, K);
+    float* val = s_val[wave];
+    int* col = s_col[wave];
+    constexpr int V = kReg / 64;
+    int hit = -2;                        // not answered yet
+    float m = -INFINITY, lo = INFINITY;
+    const bool greedy = !(s.temp > 0.0), p_alone = s.by_p && !s.by_k;
+    if (!greedy && (s.by_k ? s.top_k <= 1280 : s.by_p || s.min_p > 0.0)) {
+        Row<V> R;                        // samples: every (K / 512)-th score
+        float t_lo = INFINITY, t_hi = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            R.v[i] = S.one((int)((int64_t)(lane + 64 * i) * K / kReg));
+            t_hi = fmaxf(t_hi, R.v[i]);
+            t_lo = fminf(t_lo, R.v[i] == -INFINITY ? INFINITY : R.v[i]);
+        }
+        t_hi = lbm::wave_best(t_hi);
+        t_lo = -lbm::wave_best(-t_lo);
+        const float ref = t_hi;          // weights of the pass are relative to the best sample
+        // how many scores to take: what top-k needs and as much again, at most what fits; the square root of the samples that reach t is
+        // their spread, a sixth at 320 of 8192
+        int aim = !s.by_k ? 320 : (s.top_k <= 128 ? 256 : (s.top_k <= 384 ? (s.top_k + kReg) / 2 : (s.top_k + kCand) / 2));
+        int want = (int)fmax(1.f, (float)aim * kReg / (float)K);
+        for (int tries = 0; tries < 3 && hit == -2; ++tries) {
+            float t = kLowest, l = t_lo, h = t_hi;
+            if (R.count_from(t_lo) > want) {
+                for (int it = 0; it < kByValue && l < h; ++it) {
+                    t = trial(it, l, h);
+                    const int c = R.count_from(t);
+                    if (c > want + want / 8) l = t;
+                    else if (c < want - want / 8) h = t;
+                    else break;
+                }
+            }
+            int n = 0;
+            double sum = 0.0;
+            m = -INFINITY;
+            S.each([&](const float* q, int c) {
+                int pre = 0, tot = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    m = fmaxf(m, q[i]);
+                    const unsigned long long b = __ballot(q[i] >= t);
+                    pre = __builtin_amdgcn_mbcnt_hi((unsigned)(b >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)b, pre));
+                    tot += __popcll(b);
+                }
+                if (p_alone) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum += exp2_f64(((double)q[i] - (double)ref) * s.c);
+                }
+                if (tot != 0 && n + tot <= kCand) {
+                    int at = n + pre;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (q[i] >= t) {
+                            val[at] = q[i];
+                            col[at] = c + i;
+                            ++at;
+                        }
+                }
+                n += tot;
+            });
+            m = lbm::wave_best(m);
+            if (m == -INFINITY) {
+                hit = -1;
+                break;
+            }
+            if (m == INFINITY) break;
+            int next = want;
+            if (n > kCand || (s.by_k && n < s.top_k && t > kLowest)) {
+                next = (int)fmin(fmax(1.f, (float)want * (float)aim / (float)(n > 0 ? n : 1)), (float)kReg);
+            } else {
+                double total = -1.0;
+                if (p_alone) {
+                    total = lbm::wave_total(sum) * exp2_f64(((double)ref - (double)m) * s.c);
+                    if (!(total < 1e300)) break;       // the best sample lies too far below the best score
+                }
+                // min-p alone: everything it leaves must have been taken
+                const bool all = s.by_k || s.by_p || t == kLowest || exp2_f64(((double)t - (double)m) * s.c) < fmin(s.min_p, 1.0);
+                int at = -1;
+                if (all) {
+                    // LDS serves a wave's accesses in order: the compiler only has to keep the order too
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    lo = INFINITY;
+                    if (n <= kReg) {
+                        Row<V> Q;
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            const bool in = Row<V>::slot(i) < n;
+                            Q.v[i] = in ? val[Row<V>::slot(i)] : -INFINITY;
+                            lo = fminf(lo, in ? Q.v[i] : INFINITY);
+                        }
+                        at = settle<V>(Q, s, -lbm::wave_best(-lo), m, K, total);
+                    } else {
+                        Taken Q;
+                        Q.val = val;
+                        Q.n = n;
+                        for (int i = lane; i < n; i += 64) lo = fminf(lo, val[i]);
+                        at = draw_by_passes(Q, s, -lbm::wave_best(-lo), m, K, total);
+                    }
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                }
+                if (at >= 0) {
+                    hit = col[at];
+                    break;
+                }
+                aim = kCand * 3 / 4;     // the nucleus is larger
+                next = (int)fmax(1.f, (float)aim * kReg / (float)K);
+            }
+            if (next == want) break;
+            want = next;
+        }
+    }
+    if (hit == -2) {
+        m = -INFINITY;
+        lo = INFINITY;
+        S.each([&](const float* q, int) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                m = fmaxf(m, q[i]);
+                lo = fminf(lo, q[i] == -INFINITY ? INFINITY : q[i]);
+            }
+        });
+        m = lbm::wave_best(m);
+        lo = -lbm::wave_best(-lo);
+        if (m == -INFINITY) hit = -1;
+        else if (greedy) hit = S.nth_equal(m, 0);
+        else hit = draw_by_passes(S, s, lo, m, K, -1.0);
+    }
+    if (lane == 0) out[row] = hit;
 }
 
 template <typename T>
@@ -453,20 +764,17 @@ int run_sample(const void* scores, int64_t lds, const float* u, const Params& pa
                int64_t N, int K, hipStream_t st) {
     const T* s = static_cast<const T*>(scores);
     const int vec = ((uintptr_t)scores % (4 * sizeof(T))) == 0 && (lds & 3) == 0 && (K & 3) == 0 ? 1 : 0;
-#define LBM_SAMPLE(V, W)                                                                                                                  \
-    hipLaunchKernelGGL((code_sample_kernel<T, V, W>), dim3((unsigned)(W == 1 ? (N + 3) / 4 : N)), dim3(W == 1 ? 256 : 64 * W), 0, st, s, lds, \
-                       vec, u, par, allowed, allowed_ld, out, N, K)
-    if (K <= 256) LBM_SAMPLE(4, 1);
-    else if (K <= 512) LBM_SAMPLE(8, 1);
-    else if (K <= 1024) LBM_SAMPLE(16, 1);
-    else if (K <= 2048) LBM_SAMPLE(8, 4);
-    else if (K <= 4096) LBM_SAMPLE(16, 4);
-    else LBM_SAMPLE(8, 16);
+    const dim3 grid((unsigned)((N + 3) / 4)), block(256);
+#define LBM_SAMPLE(kernel) hipLaunchKernelGGL((kernel), grid, block, 0, st, s, lds, vec, u, par, allowed, allowed_ld, out, N, K)
+    if (K <= 256) LBM_SAMPLE((code_sample_kernel<T, 4>));
+    else if (K <= 512) LBM_SAMPLE((code_sample_kernel<T, 8>));
+    else if (K <= 1024) LBM_SAMPLE((code_sample_kernel<T, 16>));
+    else LBM_SAMPLE((code_sample_long_kernel<T>));
 #undef LBM_SAMPLE
     return lbm::check_launch("lbm_code_sample");
 }
 
-constexpr int kMaxK = 8192;   // 16 waves x 64 lanes x 8 scores
+constexpr int kMaxK = 1 << 24;
 
 }  // namespace
 
@@ -486,6 +794,7 @@ extern "C" int lbm_code_sample(const void* scores, int32_t dtype, int64_t lds, c
     LBM_REQUIRE(top_k_row_or_null || top_k >= 0, LBM_EINVAL, "%s: top_k must be >= 0 (0: all codes)", what);
     LBM_REQUIRE(top_p_row_or_null || (top_p >= 0.0 && top_p <= 1.0), LBM_EINVAL, "%s: top_p must lie in [0, 1]", what);
     LBM_REQUIRE(min_p_row_or_null || (min_p >= 0.0 && min_p <= 1.0), LBM_EINVAL, "%s: min_p must lie in [0, 1]", what);
+    LBM_REQUIRE(hist_or_null == nullptr || K <= 32768, LBM_EUNSUPPORTED, "%s: histogram supports K <= 32768", what);
     if (N == 0) return LBM_OK;
     LBM_REQUIRE(scores && u && codes, LBM_EINVAL, "%s: NULL pointer", what);
     LBM_REQUIRE(N <= 0x7fffffffLL, LBM_EUNSUPPORTED, "%s: N must be < 2^31", what);

@@ -80,8 +80,8 @@ def _sample(s=P, dt=0, lds=16, u=P, tr=None, t=1.0, kr=None, k=0, pr=None, p=1.0
     return _lib.load().lbm_code_sample(s, dt, lds, u, tr, t, kr, k, pr, p, mr, m, al, ald, out, hist, N, K, None)
 
 
-@pytest.mark.parametrize("kw,rc", [(dict(N=-1), EINVAL), (dict(K=0), EINVAL), (dict(K=8193), EUNSUPPORTED), (dict(dt=3), EINVAL),
-                                   (dict(t=-0.5), EINVAL), (dict(t=math.nan), EINVAL), (dict(k=-1), EINVAL), (dict(p=-0.1), EINVAL),
+@pytest.mark.parametrize("kw,rc", [(dict(N=-1), EINVAL), (dict(K=0), EINVAL), (dict(K=(1 << 24) + 1), EUNSUPPORTED),
+                                   (dict(K=32769, hist=P), EUNSUPPORTED), (dict(dt=3), EINVAL), (dict(t=-0.5), EINVAL), (dict(t=math.nan), EINVAL), (dict(k=-1), EINVAL), (dict(p=-0.1), EINVAL),
                                    (dict(p=1.1), EINVAL), (dict(p=math.nan), EINVAL), (dict(m=-0.1), EINVAL), (dict(m=1.5), EINVAL),
                                    (dict(s=None), EINVAL), (dict(u=None), EINVAL), (dict(out=None), EINVAL), (dict(lds=-16), EINVAL),
                                    (dict(al=P, ald=-16), EINVAL), (dict(N=1 << 31), EUNSUPPORTED)])

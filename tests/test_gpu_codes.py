@@ -337,12 +337,13 @@ def check_sample(s, u, allowed=None, **kw):
 
 SETTINGS = [dict(), dict(temperature=0.0), dict(temperature=0.3), dict(top_k=1), dict(top_k=7), dict(top_p=0.9), dict(top_p=0.0), dict(min_p=0.05),
             dict(min_p=1.0), dict(temperature=0.7, top_k=40, top_p=0.95, min_p=0.02), dict(temperature=5.0, top_p=0.5, min_p=0.3),
-            dict(temperature=1.5, top_k=5, top_p=0.99)]
+            dict(temperature=1.5, top_k=5, top_p=0.99), dict(top_k=380), dict(top_k=1000), dict(temperature=3.0, top_p=0.999),
+            dict(temperature=4.0, top_k=900, top_p=0.97, min_p=0.001)]
 
 
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("N,K", [(1, 1), (1, 512), (5, 2), (66, 61), (40, 256), (41, 258), (200, 512), (50, 1023), (30, 2048), (20, 2049), (17, 4100),
-                                 (12, 8192), (7, 8191)])
+                                 (12, 8192), (7, 8191), (3, 70001)])
 def test_sample_sizes_types_settings(kind, N, K):
     g = gen(N * 31 + K)
     s = (torch.randn((N, K), generator=g) * 3).to(TYPES[kind])
@@ -401,9 +402,28 @@ def test_sample_masks_and_extremes():
         assert (check_sample(s, u, allowed=torch.zeros((K,), dtype=torch.bool)) == -1).all()
 
 
+@pytest.mark.parametrize("K", [1500, 8192])
+def test_sample_long_rows_of_every_shape(K):
+    """Rows whose order or spread misleads a look at a few of their scores."""
+    g = gen(K + 1)
+    r = torch.arange(K).float()
+    s = torch.stack([r / K * 20, -r / K * 20, torch.randn((K,), generator=g) * 1e-3, torch.randn((K,), generator=g) * 1e3,
+                     torch.where(r % 16 == 3, torch.randn((K,), generator=g) + 30, torch.randn((K,), generator=g)),      # all good ones between
+                     torch.where(r < K // 2, torch.zeros(K), torch.full((K,), float("-inf"))),
+                     torch.where(r == K - 2, torch.full((K,), 900.0), torch.randn((K,), generator=g)),
+                     torch.where(r >= K - 600, torch.full((K,), 5.0), torch.randn((K,), generator=g)),
+                     torch.where(r % 100 == 7, torch.randn((K,), generator=g), torch.full((K,), float("-inf"))),
+                     torch.where(r % 4 == 1, torch.full((K,), float("nan")), torch.randn((K,), generator=g))])
+    for seed in range(3):
+        u = torch.rand((len(s),), generator=gen(seed))
+        for kw in SETTINGS:
+            check_sample(s, u, **kw)
+            check_sample(s.bfloat16(), u, **kw)
+
+
 def test_sample_per_row_settings():
     g = gen(12)
-    for N, K in ((300, 512), (40, 8192), (65, 77)):
+    for N, K in ((300, 512), (60, 1500), (40, 8192), (65, 77)):
         s = torch.randn((N, K), generator=g) * 2
         u = torch.rand((N,), generator=g)
         t = torch.rand((N,), generator=g) * 2
