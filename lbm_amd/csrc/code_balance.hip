@@ -6,29 +6,29 @@
 //
 // A row counts if its keep flag is set and it holds a score above -inf.  Both passes are bound by HBM: the forward reads the scores once
 // (4 operations per score), the gradient reads them again and writes as much.  A row lives in registers between its load, its maximum, its
-// sum and its use; every thread adds p of its own columns over all rows it sees, so the column sums cost no traffic until the end, where
-// each workgroup leaves one partial row.  Partial sums are joined in a fixed order in 64 bits: results do not change from run to run.
+// sum and its use, the next row's load runs under that, and every thread adds p of its own columns over all rows it sees, so the column
+// sums cost no traffic until the end, where each workgroup leaves one partial row.  Partial sums are joined in a fixed order in 64 bits:
+// results do not change from run to run.  Up to 2048 codes a wave holds a row (no barrier); above that four waves share one and exchange
+// their maxima and sums once per row.
 // The gradient takes a relative to its value at the row's best score: where one p is near 1 its a - p.a is a difference of near equals
 // otherwise, and loses what it should return.
 #include "code_rows.h"
 
 namespace {
 
-using lbm::OpAdd;
 using lbm::OpMax;
 using lbm::OpMin;
 
 constexpr int kMaxK = 8192;   // a workgroup counts picks in LDS
+constexpr int kJoinCols = 64;
 
-// per row (float2): maximum, 1 / sum (0: the row does not count)
-// workspace of the forward pass: partial sums [G][K] f32, partial counts [G][K] u32, rows counted [G] u32
+// workspace of the forward pass: partial sums [G][K] f32, partial counts [G][K] u32, rows counted [G] u32; second stage: sums [S][K] f64,
+// counts [S][K] u64
 struct Plan {
     int64_t G;
-    size_t off_cnt, off_rows, total;
+    int S;            // pieces of the G partial rows in the second stage
+    size_t off_cnt, off_rows, off_sum2, off_cnt2, total;
 };
-
-template <int W>
-constexpr int teams() { return W == 1 ? 4 : 1; }   // rows a workgroup works on at a time
 
 int waves_for(int K) { return K <= 2048 ? 1 : 4; }
 
@@ -36,255 +36,390 @@ Plan make_plan(int64_t N, int K) {
     const int T = waves_for(K) == 1 ? 4 : 1;
     Plan p;
     p.G = (N + 8 * T - 1) / (8 * T);      // eight rows per team at least, so that the partial rows stay small beside the scores
-    const int64_t cap = T == 4 ? 2048 : 1024;
+    const int64_t cap = T == 4 ? 2048 : 768;
     if (p.G > cap) p.G = cap;
     if (p.G < 1) p.G = 1;
+    const int groups = (K + kJoinCols - 1) / kJoinCols;
+    p.S = 256 / groups;                   // one workgroup per CU
+    if (p.S > (p.G + 15) / 16) p.S = (int)((p.G + 15) / 16);
+    if (p.S < 1) p.S = 1;
     auto up = [](size_t v) { return (v + 255) & ~(size_t)255; };
     size_t o = up((size_t)p.G * K * sizeof(float));
-    p.off_cnt = o;
-    o = up(o + (size_t)p.G * K * sizeof(unsigned));
-    p.off_rows = o;
-    o = up(o + (size_t)p.G * sizeof(unsigned));
+    p.off_cnt = o;  o = up(o + (size_t)p.G * K * sizeof(unsigned));
+    p.off_rows = o; o = up(o + (size_t)p.G * sizeof(unsigned));
+    p.off_sum2 = o; o = up(o + (size_t)p.S * K * sizeof(double));
+    p.off_cnt2 = o; o = up(o + (size_t)p.S * K * sizeof(unsigned long long));
     p.total = o;
     return p;
 }
 
-template <typename T, int V, int W>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void balance_rows_kernel(const T* __restrict__ scores, int64_t lds, int vec,
-                                                                            const int64_t* __restrict__ codes, int slots,
-                                                                            const uint8_t* __restrict__ keep, float2* __restrict__ stat,
-                                                                            float* __restrict__ part, unsigned* __restrict__ part_cnt,
-                                                                            unsigned* __restrict__ part_rows, int64_t N, int K) {
-    constexpr int TEAMS = teams<W>();
+// A row's scores as loaded, 16 bytes at a time: value E c + i of thread t is column (c * 64 W + t) * E + i
+template <typename T, int V, int W, bool VEC>
+struct Held {
+    static constexpr int E = 16 / sizeof(T);
+    struct alignas(16) Pack { T v[E]; };
+    Pack q[V / E];
+
+    static __device__ __forceinline__ int column(int i, int t) { return ((i / E) * 64 * W + t) * E + i % E; }
+    __device__ __forceinline__ void load(const T* __restrict__ row, int K, int t) {
+#pragma unroll
+        for (int c = 0; c < V / E; ++c) {
+            const int col = (c * 64 * W + t) * E;
+            if (VEC && col < K) {
+                q[c] = *reinterpret_cast<const Pack*>(row + col);
+            } else {
+#pragma unroll
+                for (int i = 0; i < E; ++i) q[c].v[i] = !VEC && col + i < K ? row[col + i] : lbm::score_from_f32<T>(-INFINITY);
+            }
+        }
+    }
+    __device__ __forceinline__ float at(int i) const { return lbm::score_to_f32<T>(q[i / E].v[i % E]); }
+};
+
+// exp(x), x <= 0: the difference, the product and the exponential round once each, (2 |x| + 2) 2^-24 relative
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
+
+template <typename T, int V, int W, bool VEC>
+__global__ __launch_bounds__(256, 4) void balance_rows_kernel(const T* __restrict__ scores, int64_t lds, const int64_t* __restrict__ codes,
+                                                           int slots, const uint8_t* __restrict__ keep, float2* __restrict__ stat,
+                                                           float* __restrict__ part, unsigned* __restrict__ part_cnt,
+                                                           unsigned* __restrict__ part_rows, int64_t N, int K) {
+    constexpr int TEAMS = W == 1 ? 4 : 1;
+    using H = Held<T, V, W, VEC>;
     extern __shared__ unsigned s_cnt[];                  // [K] picks; then, W == 1, the teams' column sums one after the other
-    __shared__ float s_f[2 * W];
-    __shared__ int s_i[2 * W];
-    const int team = W == 1 ? threadIdx.x >> 6 : 0, t = W == 1 ? threadIdx.x & 63 : threadIdx.x;
-    int rf = 0, ri = 0;
-    for (int k = threadIdx.x; k < K; k += blockDim.x) s_cnt[k] = 0u;
+    __shared__ float2 s_ms[2][W];                        // W > 1: (maximum, sum) of each wave
+    __shared__ int s_best[2][W];
+    __shared__ unsigned s_rows[4];
+    const int wave = threadIdx.x >> 6;
+    const int t = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int64_t step = (int64_t)gridDim.x * TEAMS;
+    for (int k = threadIdx.x; k < K; k += 256) s_cnt[k] = 0u;
     __syncthreads();
 
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
     unsigned rows = 0;
-    for (int64_t row = (int64_t)blockIdx.x * TEAMS + team; row < N; row += (int64_t)gridDim.x * TEAMS) {
-        if (keep != nullptr && keep[row] == 0) {
+    int round = 0;
+    auto kept = [&](int64_t r) { return r < N && (keep == nullptr || keep[r] != 0); };
+    int64_t row = (int64_t)blockIdx.x * TEAMS + (W == 1 ? wave : 0);
+    bool on = kept(row), on_next = kept(row + step);
+    H held;
+    if (on) held.load(scores + row * lds, K, t);
+    for (; row < N; row += step) {
+        const bool now = on;
+        float e[V];
+        if (now) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) e[i] = held.at(i);
+        }
+        on = on_next;
+        if (on) held.load(scores + (row + step) * lds, K, t);
+        on_next = kept(row + 2 * step);
+        if (!now) {
             if (t == 0) stat[row] = make_float2(0.f, 0.f);
             continue;
         }
-        float v[V];
-        lbm::load_row<T, V, W>(scores + row * lds, K, t, vec, v);
+        int64_t pick = -1;
+        if (codes != nullptr && t < slots) pick = codes[row * slots + t];
         float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < V; ++i) m = fmaxf(m, e[i]);
+        m = lbm::wave_best(m);
+        int best = 0x7fffffff;
+        if (codes == nullptr && m > -INFINITY) {         // lowest column that holds the (wave's) maximum
+#pragma unroll
+            for (int i = V - 1; i >= 0; --i) best = e[i] == m ? H::column(i, t) : best;
+            best = lbm::wave_first(best);
+        }
+        float s = 0.f, scale;
         bool nan = false;
+        if (m == -INFINITY) {                            // nothing but -inf, or NaN, which shows
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            m = fmaxf(m, v[i]);
-            nan |= v[i] != v[i];
-        }
-        m = lbm::team_join<float, W>(lbm::wave_best(m), s_f, rf, OpMax());
-        if (m == -INFINITY) {                            // nothing but -inf (does not count) or NaN (its sums are NaN, as softmax's)
-            const int any = lbm::team_join<int, W>(__any(nan) ? 1 : 0, s_i, ri, OpMax());
-            if (any == 0) {
-                if (t == 0) stat[row] = make_float2(0.f, 0.f);
-                continue;
+            for (int i = 0; i < V; ++i) {
+                nan |= e[i] != e[i];
+                e[i] = e[i] != e[i] ? e[i] : 0.f;
             }
-        }
-        float e[V], s = 0.f;
+            s = __any(nan) ? NAN : 0.f;
+        } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            e[i] = lbm::exp_f32(v[i] - m);
-            s += e[i];
+            for (int i = 0; i < V; ++i) {
+                e[i] = exp_neg(e[i] - m);
+                s += e[i];
+            }
+            s = lbm::wave_total(s);
         }
-        s = lbm::team_join<float, W>(lbm::wave_total(s), s_f, rf, OpAdd());
+        if constexpr (W > 1) {                           // the waves' pairs joined: one barrier per row, since the other half of s_ms is
+            if ((threadIdx.x & 63) == 0) {               // written only behind the next row's
+                s_ms[round][wave] = make_float2(m, s);
+                s_best[round][wave] = best;
+            }
+            __syncthreads();
+            const float m_wave = m;
+            float2 ms[W];
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                ms[w] = s_ms[round][w];
+                m = fmaxf(m, ms[w].x);
+            }
+            s = 0.f;
+            best = 0x7fffffff;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                s += ms[w].x == m ? ms[w].y : ms[w].y * exp_neg(ms[w].x - m);
+                const int bw = s_best[round][w];
+                best = ms[w].x == m && bw < best ? bw : best;
+            }
+            round ^= 1;
+            scale = m_wave == m ? 1.f : exp_neg(m_wave - m);
+        } else {
+            scale = 1.f;
+        }
+        if (m == -INFINITY && s == 0.f) {
+            if (t == 0) stat[row] = make_float2(0.f, 0.f);
+            continue;
+        }
         const float r = 1.f / s;
+        scale *= r;
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(e[i], r, acc[i]);
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(e[i], scale, acc[i]);
         ++rows;
         if (t == 0) stat[row] = make_float2(m, r);
         if (codes != nullptr) {
-            for (int q = t; q < slots; q += 64 * W) {
+            if (pick >= 0 && pick < K) atomicAdd(&s_cnt[(int)pick], 1u);
+            for (int q = t + 64 * W; q < slots; q += 64 * W) {
                 const int64_t k = codes[row * slots + q];
                 if (k >= 0 && k < K) atomicAdd(&s_cnt[(int)k], 1u);
             }
-        } else {
-            int best = 0x7fffffff;                       // lowest column that holds the maximum
-#pragma unroll
-            for (int i = V - 1; i >= 0; --i) best = v[i] == m ? ((i >> 2) * 64 * W + t) * 4 + (i & 3) : best;
-            best = lbm::team_join<int, W>(lbm::wave_first(best), s_i, ri, OpMin());
-            if (t == 0 && best < K) atomicAdd(&s_cnt[best], 1u);
+        } else if (t == 0 && best < K) {
+            atomicAdd(&s_cnt[best], 1u);
         }
     }
     __syncthreads();
     unsigned* pc = part_cnt + (int64_t)blockIdx.x * K;
-    for (int k = threadIdx.x; k < K; k += blockDim.x) pc[k] = s_cnt[k];
+    for (int k = threadIdx.x; k < K; k += 256) pc[k] = s_cnt[k];
     float* pp = part + (int64_t)blockIdx.x * K;
     if constexpr (W == 1) {
-        __shared__ unsigned s_rows[4];
         float* s_sum = reinterpret_cast<float*>(s_cnt);
-        if (t == 0) s_rows[team] = rows;
+        if (t == 0) s_rows[wave] = rows;
         for (int g = 0; g < TEAMS; ++g) {                // the teams in order
             __syncthreads();
-            if (team == g) {
+            if (wave == g) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const int k = ((i >> 2) * 64 + t) * 4 + (i & 3);
+                    const int k = H::column(i, t);
                     if (k < K) s_sum[k] = g == 0 ? acc[i] : s_sum[k] + acc[i];
                 }
             }
         }
         __syncthreads();
-        for (int k = threadIdx.x; k < K; k += blockDim.x) pp[k] = s_sum[k];
+        for (int k = threadIdx.x; k < K; k += 256) pp[k] = s_sum[k];
         if (threadIdx.x == 0) part_rows[blockIdx.x] = (s_rows[0] + s_rows[1]) + (s_rows[2] + s_rows[3]);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const int k = ((i >> 2) * 64 * W + t) * 4 + (i & 3);
+            const int k = H::column(i, t);
             if (k < K) pp[k] = acc[i];
         }
         if (t == 0) part_rows[blockIdx.x] = rows;
     }
 }
 
-// column sums over the partial rows, 16 columns x 16 groups of rows per workgroup; totals[0] = rows counted (every workgroup adds them up
-// for itself, workgroup 0 leaves them)
+// column sums over the G partial rows: workgroup (64 columns, piece of the rows)
 __global__ __launch_bounds__(256) void balance_join_kernel(const float* __restrict__ part, const unsigned* __restrict__ part_cnt,
-                                                           const unsigned* __restrict__ part_rows, float* __restrict__ mean,
-                                                           int64_t* __restrict__ counts, double* __restrict__ totals, int64_t G, int K) {
-    __shared__ double s_p[16][17];
-    __shared__ unsigned long long s_c[16][17];
-    __shared__ unsigned long long s_m[4];
-    unsigned long long m = 0;
-    for (int64_t g = threadIdx.x; g < G; g += 256) m += part_rows[g];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) m += __shfl_xor(m, o, 64);
-    if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = m;
-    const int col = threadIdx.x & 15, grp = threadIdx.x >> 4;
-    const int k = blockIdx.x * 16 + col;
+                                                           double* __restrict__ sum2, unsigned long long* __restrict__ cnt2, int64_t G, int K) {
+    __shared__ double s_p[4][kJoinCols];
+    __shared__ unsigned long long s_c[4][kJoinCols];
+    const int S = gridDim.y, piece = blockIdx.y, col = threadIdx.x & 63, grp = threadIdx.x >> 6;
+    const int k = blockIdx.x * kJoinCols + col;
+    const int64_t g0 = G * piece / S, g1 = G * (piece + 1) / S;
     double p = 0.0;
     unsigned long long c = 0;
-    if (k < K)
-        for (int64_t g = grp; g < G; g += 16) {
+    if (k < K) {
+        int64_t g = g0 + grp;
+        for (; g + 12 < g1; g += 16) {                   // four loads of each kind on their way at a time
+            float f[4];
+            unsigned n[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                f[u] = part[(g + 4 * u) * K + k];
+                n[u] = part_cnt[(g + 4 * u) * K + k];
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                p += (double)f[u];
+                c += n[u];
+            }
+        }
+        for (; g < g1; g += 4) {
             p += (double)part[g * K + k];
             c += part_cnt[g * K + k];
         }
+    }
     s_p[grp][col] = p;
     s_c[grp][col] = c;
     __syncthreads();
-    m = (s_m[0] + s_m[1]) + (s_m[2] + s_m[3]);
-    if (threadIdx.x < 16 && k < K) {
-        for (int g = 1; g < 16; ++g) {
-            p += s_p[g][col];
-            c += s_c[g][col];
-        }
-        mean[k] = m > 0 ? (float)(p / (double)m) : 0.f;
-        counts[k] = (int64_t)c;
+    if (threadIdx.x < kJoinCols && k < K) {
+        sum2[(int64_t)piece * K + k] = (s_p[0][col] + s_p[1][col]) + (s_p[2][col] + s_p[3][col]);
+        cnt2[(int64_t)piece * K + k] = (s_c[0][col] + s_c[1][col]) + (s_c[2][col] + s_c[3][col]);
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) totals[0] = (double)m;
 }
 
+constexpr int kFinish = 1024;
+
 __device__ __forceinline__ double block_sum(double v, double* s) {
-    v = lbm::wave_sum(v);
+    v = lbm::wave_total(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (s[0] + s[1]) + (s[2] + s[3]);
+    v = 0.0;
+#pragma unroll
+    for (int w = 0; w < kFinish / 64; ++w) v += s[w];
+    return v;
 }
 
-// loss = K sum f P; totals[1] = picks counted
-__global__ __launch_bounds__(256) void balance_loss_kernel(const float* __restrict__ mean, const int64_t* __restrict__ counts,
-                                                           float* __restrict__ loss, double* __restrict__ totals, int K) {
-    __shared__ double s[4];
-    double c = 0.0, l = 0.0;
-    for (int k = threadIdx.x; k < K; k += 256) {
-        c += (double)counts[k];
-        l += (double)counts[k] * (double)mean[k];
+// one workgroup: the pieces joined in order, the means, the loss; totals: rows that count, picks that count.  (A last-workgroup-to-arrive
+// join inside the kernel above cost more than this launch: 33 us against 8 at 24000 x 512, its fences write an XCD's L2 back.)
+__global__ __launch_bounds__(kFinish) void balance_finish_kernel(const double* __restrict__ sum2, const unsigned long long* __restrict__ cnt2,
+                                                                 const unsigned* __restrict__ part_rows, float* __restrict__ mean,
+                                                                 int64_t* __restrict__ counts, float* __restrict__ loss,
+                                                                 double* __restrict__ totals, int S, int64_t G, int K) {
+    __shared__ double s_sum[kFinish / 64];
+    double m = 0.0;
+    for (int64_t g = threadIdx.x; g < G; g += kFinish) m += (double)part_rows[g];
+    m = block_sum(m, s_sum);
+    double picks = 0.0, l = 0.0;
+    for (int k = threadIdx.x; k < K; k += kFinish) {
+        double p = 0.0;
+        unsigned long long c = 0;
+        for (int z = 0; z < S; ++z) {
+            p += sum2[(int64_t)z * K + k];
+            c += cnt2[(int64_t)z * K + k];
+        }
+        const float f = m > 0.0 ? (float)(p / m) : 0.f;
+        mean[k] = f;
+        counts[k] = (int64_t)c;
+        picks += (double)c;
+        l += (double)c * (double)f;
     }
-    c = block_sum(c, s);
-    l = block_sum(l, s);
+    picks = block_sum(picks, s_sum);
+    l = block_sum(l, s_sum);
     if (threadIdx.x == 0) {
-        loss[0] = (float)((double)K * l / (c > 0.0 ? c : 1.0));   // NaN in mean shows even where nothing was picked
-        totals[1] = c;
+        loss[0] = (float)((double)K * l / (picks > 0.0 ? picks : 1.0));   // NaN in mean shows even where nothing was picked
+        totals[0] = m;
+        totals[1] = picks;
     }
 }
 
-template <typename T, int V, int W>
-__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void balance_grad_kernel(const T* __restrict__ scores, int64_t lds, int vec,
-                                                                            const float2* __restrict__ stat, const int64_t* __restrict__ counts,
-                                                                            const double* __restrict__ totals, const float* __restrict__ g_loss,
-                                                                            const float* __restrict__ g_mean, T* __restrict__ ds, int vec_out,
-                                                                            int64_t N, int K) {
-    constexpr int TEAMS = teams<W>();
-    __shared__ float s_f[2 * W];
-    const int team = W == 1 ? threadIdx.x >> 6 : 0, t = W == 1 ? threadIdx.x & 63 : threadIdx.x;
-    int rf = 0;
+template <typename T, int V, int W, bool VEC>
+__global__ __launch_bounds__(256, 4) void balance_grad_kernel(const T* __restrict__ scores, int64_t lds, const float2* __restrict__ stat,
+                                                           const int64_t* __restrict__ counts, const double* __restrict__ totals,
+                                                           const float* __restrict__ g_loss, const float* __restrict__ g_mean,
+                                                           T* __restrict__ ds, int64_t N, int K) {
+    constexpr int TEAMS = W == 1 ? 4 : 1;
+    using H = Held<T, V, W, VEC>;
+    __shared__ float4 s_x[2][W];                         // W > 1: each wave's p.(a - ref), its sum of p, its ref, whether it holds the best
+    const int wave = threadIdx.x >> 6;
+    const int t = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int64_t step = (int64_t)gridDim.x * TEAMS;
     const double M = totals[0], C = totals[1];
     const double gl = g_loss != nullptr && C > 0.0 ? (double)g_loss[0] * K / C : 0.0;
     const float inv_m = M > 0.0 ? (float)(1.0 / M) : 0.f;
     float a[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int k = ((i >> 2) * 64 * W + t) * 4 + (i & 3);
+        const int k = H::column(i, t);
         a[i] = k < K ? (float)(gl * (double)counts[k] + (g_mean != nullptr ? (double)g_mean[k] : 0.0)) : 0.f;
     }
-    for (int64_t row = (int64_t)blockIdx.x * TEAMS + team; row < N; row += (int64_t)gridDim.x * TEAMS) {
-        const float m = stat[row].x, r = stat[row].y;
+    int round = 0;
+    int64_t row = (int64_t)blockIdx.x * TEAMS + (W == 1 ? wave : 0);
+    const float2 off = make_float2(0.f, 0.f);
+    float2 st = row < N ? stat[row] : off, st_next = row + step < N ? stat[row + step] : off;
+    H held;
+    if (st.y != 0.f) held.load(scores + row * lds, K, t);
+    for (; row < N; row += step) {
+        const float m = st.x, r = st.y;
         float d[V];
+        if (r != 0.f) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) d[i] = held.at(i);
+        }
+        st = st_next;
+        if (st.y != 0.f) held.load(scores + (row + step) * lds, K, t);
+        st_next = row + 2 * step < N ? stat[row + 2 * step] : off;
         if (r == 0.f) {
 #pragma unroll
             for (int i = 0; i < V; ++i) d[i] = 0.f;
         } else {
-            float v[V], ref = -INFINITY;
-            lbm::load_row<T, V, W>(scores + row * lds, K, t, vec, v);
+            float ref = -INFINITY, dot = 0.f, mass = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) ref = v[i] == m ? fmaxf(ref, a[i]) : ref;
-            ref = lbm::team_join<float, W>(lbm::wave_best(ref), s_f, rf, OpMax());
-            float dot = 0.f;
+            for (int i = 0; i < V; ++i) ref = d[i] == m ? fmaxf(ref, a[i]) : ref;
+            ref = lbm::wave_best(ref);
+            const bool best = ref > -INFINITY;
+            if (W > 1 && !best) ref = 0.f;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                d[i] = lbm::exp_f32(v[i] - m) * r;
+                d[i] = exp_neg(d[i] - m) * r;
                 dot = fmaf(d[i], a[i] - ref, dot);
+                if constexpr (W > 1) mass += d[i];
             }
-            dot = lbm::team_join<float, W>(lbm::wave_total(dot), s_f, rf, OpAdd());
+            dot = lbm::wave_total(dot);
+            if constexpr (W > 1) {                       // p.(a - ref of the best score), from each wave's own reference
+                mass = lbm::wave_total(mass);
+                if ((threadIdx.x & 63) == 0) s_x[round][wave] = make_float4(dot, mass, ref, best ? 1.f : 0.f);
+                __syncthreads();
+                float4 x[W];
+                ref = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    x[w] = s_x[round][w];
+                    ref = x[w].w != 0.f ? fmaxf(ref, x[w].z) : ref;
+                }
+                dot = 0.f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) dot += fmaf(x[w].z - ref, x[w].y, x[w].x);
+                round ^= 1;
+            }
 #pragma unroll
             for (int i = 0; i < V; ++i) d[i] = d[i] * ((a[i] - ref) - dot) * inv_m;
         }
         T* out = ds + row * (int64_t)K;
 #pragma unroll
-        for (int c = 0; c < V / 4; ++c) {
-            const int col = (c * 64 * W + t) * 4;
-            if (vec_out) {
+        for (int c = 0; c < V / H::E; ++c) {
+            const int col = (c * 64 * W + t) * H::E;
+            if constexpr (VEC) {
                 if (col < K) {
-                    lbm::Quad<T> q;
+                    typename H::Pack q;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) q.v[i] = lbm::score_from_f32<T>(d[4 * c + i]);
-                    *reinterpret_cast<lbm::Quad<T>*>(out + col) = q;
+                    for (int i = 0; i < H::E; ++i) q.v[i] = lbm::score_from_f32<T>(d[H::E * c + i]);
+                    *reinterpret_cast<typename H::Pack*>(out + col) = q;
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (col + i < K) out[col + i] = lbm::score_from_f32<T>(d[4 * c + i]);
+                for (int i = 0; i < H::E; ++i)
+                    if (col + i < K) out[col + i] = lbm::score_from_f32<T>(d[H::E * c + i]);
             }
         }
     }
 }
 
+// 16 bytes at a time: aligned base and rows, and the last 16 bytes of a row end with it
 template <typename T>
-int vec_ok(const void* p, int64_t ld, int K) {
-    return ((uintptr_t)p % (4 * sizeof(T))) == 0 && (ld & 3) == 0 && (K & 3) == 0 ? 1 : 0;
+bool vec_ok(const void* p, int64_t ld, int K) {
+    constexpr int E = 16 / sizeof(T);
+    return ((uintptr_t)p & 15) == 0 && ld % E == 0 && K % E == 0;
 }
 
 template <typename T>
 int run_rows(const void* scores, int64_t lds, const int64_t* codes, int slots, const uint8_t* keep, float2* stat, float* part, unsigned* cnt,
              unsigned* rows, int64_t G, int64_t N, int K, hipStream_t st) {
     const T* s = static_cast<const T*>(scores);
-    const int vec = vec_ok<T>(scores, lds, K);
+    const bool vec = vec_ok<T>(scores, lds, K);
     const size_t shm = (size_t)K * 4;
-#define LBM_ROWS(V, W)                                                                                                                     \
-    hipLaunchKernelGGL((balance_rows_kernel<T, V, W>), dim3((unsigned)G), dim3(W == 1 ? 256 : 64 * W), shm, st, s, lds, vec, codes, slots, \
-                       keep, stat, part, cnt, rows, N, K)
-    if (K <= 256) LBM_ROWS(4, 1);
-    else if (K <= 512) LBM_ROWS(8, 1);
+#define LBM_ROWS(V, W)                                                                                                              \
+    hipLaunchKernelGGL((vec ? balance_rows_kernel<T, V, W, true> : balance_rows_kernel<T, V, W, false>), dim3((unsigned)G), dim3(256), \
+                       shm, st, s, lds, codes, slots, keep, stat, part, cnt, rows, N, K)
+    if (K <= 512) LBM_ROWS(8, 1);
     else if (K <= 1024) LBM_ROWS(16, 1);
     else if (K <= 2048) LBM_ROWS(32, 1);
     else if (K <= 4096) LBM_ROWS(16, 4);
@@ -298,12 +433,11 @@ int run_grad(const void* scores, int64_t lds, const float2* stat, const int64_t*
              const float* g_mean, void* ds, int64_t G, int64_t N, int K, hipStream_t st) {
     const T* s = static_cast<const T*>(scores);
     T* o = static_cast<T*>(ds);
-    const int vec = vec_ok<T>(scores, lds, K), vo = vec_ok<T>(ds, K, K);
-#define LBM_GRAD(V, W)                                                                                                                       \
-    hipLaunchKernelGGL((balance_grad_kernel<T, V, W>), dim3((unsigned)G), dim3(W == 1 ? 256 : 64 * W), 0, st, s, lds, vec, stat, counts, totals, \
-                       g_loss, g_mean, o, vo, N, K)
-    if (K <= 256) LBM_GRAD(4, 1);
-    else if (K <= 512) LBM_GRAD(8, 1);
+    const bool vec = vec_ok<T>(scores, lds, K) && vec_ok<T>(ds, K, K);
+#define LBM_GRAD(V, W)                                                                                                              \
+    hipLaunchKernelGGL((vec ? balance_grad_kernel<T, V, W, true> : balance_grad_kernel<T, V, W, false>), dim3((unsigned)G), dim3(256), \
+                       0, st, s, lds, stat, counts, totals, g_loss, g_mean, o, N, K)
+    if (K <= 512) LBM_GRAD(8, 1);
     else if (K <= 1024) LBM_GRAD(16, 1);
     else if (K <= 2048) LBM_GRAD(32, 1);
     else if (K <= 4096) LBM_GRAD(16, 4);
@@ -337,14 +471,17 @@ extern "C" int lbm_code_balance(const void* scores, int32_t dtype, int64_t lds, 
     float* part = reinterpret_cast<float*>(ws);
     unsigned* cnt = reinterpret_cast<unsigned*>(ws + p.off_cnt);
     unsigned* rows = reinterpret_cast<unsigned*>(ws + p.off_rows);
+    double* sum2 = reinterpret_cast<double*>(ws + p.off_sum2);
+    unsigned long long* cnt2 = reinterpret_cast<unsigned long long*>(ws + p.off_cnt2);
+    const int groups = (K + kJoinCols - 1) / kJoinCols;
     hipStream_t st = lbm::as_stream(stream);
     int rc = LBM_OK;
 #define LBM_CALL(T) rc = run_rows<T>(scores, lds, codes_or_null, slots, keep_or_null, reinterpret_cast<float2*>(row_stat), part, cnt, rows, p.G, N, K, st)
     LBM_CODE_TYPES(dtype, LBM_CALL);
 #undef LBM_CALL
     if (rc != LBM_OK) return rc;
-    hipLaunchKernelGGL(balance_join_kernel, dim3((unsigned)((K + 15) / 16)), dim3(256), 0, st, part, cnt, rows, mean, counts, totals, p.G, K);
-    hipLaunchKernelGGL(balance_loss_kernel, dim3(1), dim3(256), 0, st, mean, counts, loss, totals, K);
+    hipLaunchKernelGGL(balance_join_kernel, dim3((unsigned)groups, (unsigned)p.S), dim3(256), 0, st, part, cnt, sum2, cnt2, p.G, K);
+    hipLaunchKernelGGL(balance_finish_kernel, dim3(1), dim3(kFinish), 0, st, sum2, cnt2, rows, mean, counts, loss, totals, p.S, p.G, K);
     return lbm::check_launch(what);
 }
 

@@ -98,15 +98,6 @@ struct OpAdd {
     __device__ __forceinline__ A operator()(A a, A b) const { return a + b; }
 };
 
-// exp(x) for x <= 0 to about 1.5 ulp, NaN for NaN: the part of x log2(e) that its product rounds away is added back behind the exponential
-__device__ __forceinline__ float exp_f32(float x) {
-    constexpr float kLog2e = 1.44269502e+0f, kLog2eLo = 1.92596303e-8f, kLn2 = 0.693147182f;
-    x = x < -150.f ? -150.f : x;     // 2^-216: zero in fp32 either way, and -inf would make the residual NaN
-    const float t = x * kLog2e;
-    const float r = fmaf(x, kLog2eLo, fmaf(x, kLog2e, -t));
-    const float e = __builtin_amdgcn_exp2f(t);
-    return fmaf(e, r * kLn2, e);
-}
 
 template <typename A>
 __device__ __forceinline__ A wave_total(A x) { return lane_value(wave_scan<A>(x, A(0), OpAdd()), 63); }
