@@ -115,7 +115,7 @@ def check(rc: int, what: str = ""):
 def stream_ptr() -> int:
     """The current stream of the CURRENT device: launches go to the current HIP device, so every tensor handed to a call
     must live there (``ptr`` checks it)."""
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())     # the handle alone: 0.5 us for 2.7 through a Stream object
 
 
 def ptr(t):

@@ -121,6 +121,7 @@ def _score_rows(scores: torch.Tensor, what: str):
 
 
 class _CodeBalance(torch.autograd.Function):
+    # Host time counts at training sizes (the kernels take some 60 us): one device check, as few allocations as the lifetimes allow.
     @staticmethod
     def forward(ctx, scores, ld, codes, slots, keep):
         N, K = scores.shape
@@ -129,17 +130,17 @@ class _CodeBalance(torch.autograd.Function):
         nbytes = lib.lbm_code_balance_workspace_bytes(N, K)
         if nbytes == 0:
             raise NotImplementedError(f"code_balance_loss supports K <= 8192 (got K={K})")
+        sp = _lib.ptr(scores)                        # checks the device; codes and keep were moved to it
         ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
         mean = torch.empty((K,), dtype=torch.float32, device=dev)
         counts = torch.empty((K,), dtype=torch.int64, device=dev)
-        stat = torch.empty((N, 2), dtype=torch.float32, device=dev)
-        totals = torch.empty((2,), dtype=torch.float64, device=dev)
-        dtype = _lib.SCORE_TYPES[scores.dtype]
-        _lib.check(lib.lbm_code_balance(_lib.ptr(scores), dtype, ld, _lib.ptr(codes), slots, _lib.ptr(keep), _lib.ptr(loss), _lib.ptr(counts),
-                                        _lib.ptr(mean), _lib.ptr(stat), _lib.ptr(totals), _lib.ptr(ws), N, K, _lib.stream_ptr()),
-                   "lbm_code_balance")
-        ctx.save_for_backward(scores, stat, counts, totals)
+        saved = torch.empty((2 + N,), dtype=torch.float64, device=dev)      # totals, then (maximum, 1 / sum) of each row
+        at = saved.data_ptr()
+        _lib.check(lib.lbm_code_balance(sp, _lib.SCORE_TYPES[scores.dtype], ld, None if codes is None else codes.data_ptr(), slots,
+                                        None if keep is None else keep.data_ptr(), loss.data_ptr(), counts.data_ptr(), mean.data_ptr(),
+                                        at + 16, at, ws.data_ptr(), N, K, _lib.stream_ptr()), "lbm_code_balance")
+        ctx.save_for_backward(scores, saved, counts)
         ctx.ld = ld
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
@@ -148,14 +149,16 @@ class _CodeBalance(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, _g_counts, g_mean):
-        scores, stat, counts, totals = ctx.saved_tensors
+        scores, saved, counts = ctx.saved_tensors
         N, K = scores.shape
         ds = torch.empty((N, K), dtype=scores.dtype, device=scores.device)
-        g_loss = None if g_loss is None else g_loss.to(torch.float32).contiguous()
-        g_mean = None if g_mean is None else g_mean.to(torch.float32).contiguous()
-        _lib.check(_lib.load().lbm_code_balance_grad(_lib.ptr(scores), _lib.SCORE_TYPES[scores.dtype], ctx.ld, _lib.ptr(stat), _lib.ptr(counts),
-                                                     _lib.ptr(totals), _lib.ptr(g_loss), _lib.ptr(g_mean), _lib.ptr(ds), N, K,
-                                                     _lib.stream_ptr()), "lbm_code_balance_grad")
+        if g_mean is not None:
+            g_mean = g_mean.contiguous()
+        at = saved.data_ptr()
+        _lib.check(_lib.load().lbm_code_balance_grad(_lib.ptr(scores), _lib.SCORE_TYPES[scores.dtype], ctx.ld, at + 16, counts.data_ptr(), at,
+                                                     None if g_loss is None else g_loss.data_ptr(),
+                                                     None if g_mean is None else g_mean.data_ptr(), ds.data_ptr(), N, K, _lib.stream_ptr()),
+                   "lbm_code_balance_grad")
         return ds, None, None, None, None
 
 

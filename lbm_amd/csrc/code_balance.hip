@@ -8,8 +8,8 @@
 // (4 operations per score), the gradient reads them again and writes as much.  A row lives in registers between its load, its maximum, its
 // sum and its use, the next row's load runs under that, and every thread adds p of its own columns over all rows it sees, so the column
 // sums cost no traffic until the end, where each workgroup leaves one partial row.  Partial sums are joined in a fixed order in 64 bits:
-// results do not change from run to run.  Up to 2048 codes a wave holds a row (no barrier); above that four waves share one and exchange
-// their maxima and sums once per row.
+// results do not change from run to run.  Up to 1024 codes a wave holds a row (no barrier); above that four waves share one and
+// exchange their maxima and sums once per row (eight waves with half the registers each: 217 us for 172 at 40000 x 8192 bf16).
 // The gradient takes a relative to its value at the row's best score: where one p is near 1 its a - p.a is a difference of near equals
 // otherwise, and loses what it should return.
 #include "code_rows.h"
@@ -30,13 +30,18 @@ struct Plan {
     size_t off_cnt, off_rows, off_sum2, off_cnt2, total;
 };
 
-int waves_for(int K) { return K <= 2048 ? 1 : 4; }
+int waves_for(int K) { return K <= 1024 ? 1 : 4; }
 
 Plan make_plan(int64_t N, int K) {
     const int T = waves_for(K) == 1 ? 4 : 1;
     Plan p;
-    p.G = (N + 8 * T - 1) / (8 * T);      // eight rows per team at least, so that the partial rows stay small beside the scores
-    const int64_t cap = T == 4 ? 2048 : 768;
+    // eight rows per team at least, so that the partial rows stay small beside the scores -- two where that leaves CUs without work
+    p.G = (N + 8 * T - 1) / (8 * T);
+    if (p.G < 512) {
+        p.G = (N + 2 * T - 1) / (2 * T);
+        if (p.G > 512) p.G = 512;
+    }
+    const int64_t cap = T == 4 ? 2048 : (K <= 4096 ? 1024 : 768);   // as many as run at a time
     if (p.G > cap) p.G = cap;
     if (p.G < 1) p.G = 1;
     const int groups = (K + kJoinCols - 1) / kJoinCols;
@@ -76,11 +81,27 @@ struct Held {
     __device__ __forceinline__ float at(int i) const { return lbm::score_to_f32<T>(q[i / E].v[i % E]); }
 };
 
+// 16 bytes of scores, each rounded once to the nearest
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float* f) {
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            w[i] = __float_as_uint(f[i]);
+        } else {
+            const T a = lbm::score_from_f32<T>(f[2 * i]), b = lbm::score_from_f32<T>(f[2 * i + 1]);
+            w[i] = (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // exp(x), x <= 0: the difference, the product and the exponential round once each, (2 |x| + 2) 2^-24 relative
 __device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
 
 template <typename T, int V, int W, bool VEC>
-__global__ __launch_bounds__(256, 4) void balance_rows_kernel(const T* __restrict__ scores, int64_t lds, const int64_t* __restrict__ codes,
+__global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_rows_kernel(const T* __restrict__ scores, int64_t lds, const int64_t* __restrict__ codes,
                                                            int slots, const uint8_t* __restrict__ keep, float2* __restrict__ stat,
                                                            float* __restrict__ part, unsigned* __restrict__ part_cnt,
                                                            unsigned* __restrict__ part_rows, int64_t N, int K) {
@@ -279,7 +300,7 @@ __device__ __forceinline__ double block_sum(double v, double* s) {
 }
 
 // one workgroup: the pieces joined in order, the means, the loss; totals: rows that count, picks that count.  (A last-workgroup-to-arrive
-// join inside the kernel above cost more than this launch: 33 us against 8 at 24000 x 512, its fences write an XCD's L2 back.)
+// join inside the kernel above cost more than this launch: 33 us for both against 9 at 24000 x 512, its fences write an XCD's L2 back.)
 __global__ __launch_bounds__(kFinish) void balance_finish_kernel(const double* __restrict__ sum2, const unsigned long long* __restrict__ cnt2,
                                                                  const unsigned* __restrict__ part_rows, float* __restrict__ mean,
                                                                  int64_t* __restrict__ counts, float* __restrict__ loss,
@@ -292,9 +313,20 @@ __global__ __launch_bounds__(kFinish) void balance_finish_kernel(const double* _
     for (int k = threadIdx.x; k < K; k += kFinish) {
         double p = 0.0;
         unsigned long long c = 0;
-        for (int z = 0; z < S; ++z) {
-            p += sum2[(int64_t)z * K + k];
-            c += cnt2[(int64_t)z * K + k];
+        for (int z0 = 0; z0 < S; z0 += 8) {              // eight of each kind on their way at a time
+            double f[8];
+            unsigned long long n[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int z = z0 + u < S ? z0 + u : S - 1;
+                f[u] = sum2[(int64_t)z * K + k];
+                n[u] = cnt2[(int64_t)z * K + k];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                p += z0 + u < S ? f[u] : 0.0;
+                c += z0 + u < S ? n[u] : 0ull;
+            }
         }
         const float f = m > 0.0 ? (float)(p / m) : 0.f;
         mean[k] = f;
@@ -312,7 +344,7 @@ __global__ __launch_bounds__(kFinish) void balance_finish_kernel(const double* _
 }
 
 template <typename T, int V, int W, bool VEC>
-__global__ __launch_bounds__(256, 4) void balance_grad_kernel(const T* __restrict__ scores, int64_t lds, const float2* __restrict__ stat,
+__global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_grad_kernel(const T* __restrict__ scores, int64_t lds, const float2* __restrict__ stat,
                                                            const int64_t* __restrict__ counts, const double* __restrict__ totals,
                                                            const float* __restrict__ g_loss, const float* __restrict__ g_mean,
                                                            T* __restrict__ ds, int64_t N, int K) {
@@ -333,8 +365,12 @@ __global__ __launch_bounds__(256, 4) void balance_grad_kernel(const T* __restric
     }
     int round = 0;
     int64_t row = (int64_t)blockIdx.x * TEAMS + (W == 1 ? wave : 0);
-    const float2 off = make_float2(0.f, 0.f);
-    float2 st = row < N ? stat[row] : off, st_next = row + step < N ? stat[row + step] : off;
+    auto row_stat = [&](int64_t q) {
+        float2 v = make_float2(0.f, 0.f);
+        if (q < N) v = stat[q];
+        return v;
+    };
+    float2 st = row_stat(row), st_next = row_stat(row + step);
     H held;
     if (st.y != 0.f) held.load(scores + row * lds, K, t);
     for (; row < N; row += step) {
@@ -346,7 +382,7 @@ __global__ __launch_bounds__(256, 4) void balance_grad_kernel(const T* __restric
         }
         st = st_next;
         if (st.y != 0.f) held.load(scores + (row + step) * lds, K, t);
-        st_next = row + 2 * step < N ? stat[row + 2 * step] : off;
+        st_next = row_stat(row + 2 * step);
         if (r == 0.f) {
 #pragma unroll
             for (int i = 0; i < V; ++i) d[i] = 0.f;
@@ -389,10 +425,7 @@ __global__ __launch_bounds__(256, 4) void balance_grad_kernel(const T* __restric
             const int col = (c * 64 * W + t) * H::E;
             if constexpr (VEC) {
                 if (col < K) {
-                    typename H::Pack q;
-#pragma unroll
-                    for (int i = 0; i < H::E; ++i) q.v[i] = lbm::score_from_f32<T>(d[H::E * c + i]);
-                    *reinterpret_cast<typename H::Pack*>(out + col) = q;
+                    *reinterpret_cast<uint4*>(out + col) = pack16<T>(d + H::E * c);
                 }
             } else {
 #pragma unroll
@@ -421,7 +454,7 @@ int run_rows(const void* scores, int64_t lds, const int64_t* codes, int slots, c
                        shm, st, s, lds, codes, slots, keep, stat, part, cnt, rows, N, K)
     if (K <= 512) LBM_ROWS(8, 1);
     else if (K <= 1024) LBM_ROWS(16, 1);
-    else if (K <= 2048) LBM_ROWS(32, 1);
+    else if (K <= 2048) LBM_ROWS(8, 4);
     else if (K <= 4096) LBM_ROWS(16, 4);
     else LBM_ROWS(32, 4);
 #undef LBM_ROWS
@@ -439,7 +472,7 @@ int run_grad(const void* scores, int64_t lds, const float2* stat, const int64_t*
                        0, st, s, lds, stat, counts, totals, g_loss, g_mean, o, N, K)
     if (K <= 512) LBM_GRAD(8, 1);
     else if (K <= 1024) LBM_GRAD(16, 1);
-    else if (K <= 2048) LBM_GRAD(32, 1);
+    else if (K <= 2048) LBM_GRAD(8, 4);
     else if (K <= 4096) LBM_GRAD(16, 4);
     else LBM_GRAD(32, 4);
 #undef LBM_GRAD
@@ -495,7 +528,7 @@ extern "C" int lbm_code_balance_grad(const void* scores, int32_t dtype, int64_t 
     if (N == 0) return LBM_OK;
     LBM_REQUIRE(scores && row_stat && counts && totals && dscores, LBM_EINVAL, "%s: NULL pointer", what);
     LBM_REQUIRE(N <= 1 || lds >= 0, LBM_EINVAL, "%s: negative row stride", what);
-    const int64_t T = waves_for(K) == 1 ? 4 : 1, cap = T == 4 ? 2048 : 1024;
+    const int64_t T = waves_for(K) == 1 ? 4 : 1, cap = T == 4 ? 2048 : (K <= 4096 ? 1024 : 512);
     int64_t G = (N + T - 1) / T;
     if (G > cap) G = cap;
     int rc = LBM_OK;
