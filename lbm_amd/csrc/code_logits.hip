@@ -25,84 +25,115 @@ using f32x16 = __attribute__((ext_vector_type(16))) float;
 constexpr int kThreads = 256;
 constexpr int kBK = 32;
 
-enum { KC = 0, MC = 1 };   // operand contiguous along the contraction / along its rows
+// operand contiguous along the contraction (KC) or along its rows (MC), read 4 bytes or (V) 16 bytes at a time
+enum { KC = 0, MC = 1, KCV = 2, MCV = 3 };
+constexpr bool along_k(int mode) { return (mode & 1) == 0; }
+constexpr bool wide(int mode) { return (mode & 2) != 0; }
 
-// Operand `rows x steps`: element (r, k) is p[off(r) + k * ldk] (MC; off(r) = r, or b * pitch + s for channel-major rows r = (b, s)) or
-// p[r * ld + k] (KC).
+// Operand `rows x steps`: element (r, k) is p[r * ld + k] (KC) or p[off(r) + k * ld] (MC; off(r) = r, or b * pitch + s for channel-major rows
+// r = b * S + s).
 struct Operand {
     const float* p;
     int64_t ld;       // KC: row stride; MC: stride of one contraction step
-    int64_t S, pitch; // MC: rows r = b * S + s start at b * pitch + s (S = 0: at r)
+    int64_t S, pitch; // MC: S = 0: rows are contiguous
     int64_t rows;
-    int vec;          // KC: 16-byte loads allowed (aligned base and row stride)
 };
 
+// One operand's share of a tile: 32 contraction steps of T rows, in registers on the way from memory to LDS.  Rows past the operand's last
+// repeat it (what they give is not stored); steps past the end are zeros and come from load_tail only, so that load has no branch in it.
 template <int T, int MODE>
 struct Stage {
-    static constexpr int kPitch = MODE == KC ? kBK + 4 : T + 2;
-    static constexpr int kFloats = MODE == KC ? T * kPitch : kBK * kPitch;
-    static constexpr int kRegs = T * kBK / kThreads;
-    float v[kRegs];
-    const float* base[MODE == KC ? kRegs / 4 : 1];
-    bool ok[MODE == KC ? kRegs / 4 : 1];
+    static constexpr bool K = along_k(MODE), WIDE = wide(MODE);
+    static constexpr int kPitch = K ? kBK + 4 : T + 4;
+    static constexpr int kFloats = K ? T * kPitch : kBK * kPitch;
+    static constexpr int kQuads = T * kBK / 4 / kThreads;
+    // K: thread has steps 4 (t % 8) .. + 3 of row t / 8 + 32 i.  else WIDE: rows 4 (t % (T / 4)) .. + 3 of step t / (T / 4) + .. i;
+    // not WIDE: row t % T of steps t / T + (kThreads / T) (4 i + u)
+    static constexpr int kPer = WIDE ? kThreads / (T / 4) : kThreads / T;
+    float v[kQuads][4];
+    const float* base[K ? kQuads : (WIDE ? 1 : 1)];
+    int64_t ld;
 
-    __device__ __forceinline__ void init(const Operand& o, int64_t r0) {
-        if constexpr (MODE == KC) {
+    __device__ __forceinline__ static int kstep(int i, int u) {
+        return WIDE ? threadIdx.x / (T / 4) + kPer * i : threadIdx.x / T + kPer * (4 * i + u);
+    }
+    __device__ __forceinline__ void init(const Operand& o, int64_t r0, int64_t k0) {
+        ld = o.ld;
+        if constexpr (K) {
 #pragma unroll
-            for (int i = 0; i < kRegs / 4; ++i) {
+            for (int i = 0; i < kQuads; ++i) {
                 const int64_t r = r0 + (threadIdx.x >> 3) + 32 * i;
-                ok[i] = r < o.rows;
-                base[i] = o.p + (ok[i] ? r : 0) * o.ld + (threadIdx.x & 7) * 4;
+                base[i] = o.p + (r < o.rows ? r : o.rows - 1) * o.ld + (threadIdx.x & 7) * 4 + k0;
             }
         } else {
-            const int64_t r = r0 + threadIdx.x % T;
-            ok[0] = r < o.rows;
-            const int64_t rc = ok[0] ? r : 0;
-            base[0] = o.p + (o.S > 0 ? (rc / o.S) * o.pitch + rc % o.S : rc);
+            int64_t r = r0 + (WIDE ? threadIdx.x % (T / 4) * 4 : threadIdx.x % T);
+            if (WIDE) r = r < o.rows ? r : 0;                      // rows % 4 == 0: four at a time are all in or all out
+            else r = r < o.rows ? r : o.rows - 1;
+            base[0] = o.p + (o.S > 0 ? (r / o.S) * o.pitch + r % o.S : r) + (k0 + kstep(0, 0)) * o.ld;
         }
     }
-    // contraction steps k0 .. k0 + 31, zeros from step kend and for rows past the operand's last
-    __device__ __forceinline__ void load(const Operand& o, int64_t k0, int64_t kend) {
-        if constexpr (MODE == KC) {
-            const int64_t k = k0 + (threadIdx.x & 7) * 4;
+    // 32 whole steps
+    __device__ __forceinline__ void load() {
+        if constexpr (K) {
 #pragma unroll
-            for (int i = 0; i < kRegs / 4; ++i) {
-                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                const float* q = base[i] + k0;
-                if (o.vec && k + 3 < kend) {
-                    if (ok[i]) f = *reinterpret_cast<const float4*>(q);
-                } else if (ok[i]) {
-                    if (k < kend) f.x = q[0];
-                    if (k + 1 < kend) f.y = q[1];
-                    if (k + 2 < kend) f.z = q[2];
-                    if (k + 3 < kend) f.w = q[3];
+            for (int i = 0; i < kQuads; ++i) {
+                if constexpr (WIDE) {
+                    const float4 f = *reinterpret_cast<const float4*>(base[i]);
+                    v[i][0] = f.x; v[i][1] = f.y; v[i][2] = f.z; v[i][3] = f.w;
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) v[i][u] = base[i][u];
                 }
-                v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+                base[i] += kBK;
             }
         } else {
-            const int ks = threadIdx.x / T;
-            const float* q = base[0] + (k0 + ks) * o.ld;
 #pragma unroll
-            for (int i = 0; i < kRegs; ++i) {
-                const int64_t k = k0 + ks + i * (kThreads / T);
-                v[i] = (ok[0] && k < kend) ? q[(int64_t)i * (kThreads / T) * o.ld] : 0.f;
+            for (int i = 0; i < kQuads; ++i) {
+                if constexpr (WIDE) {
+                    const float4 f = *reinterpret_cast<const float4*>(base[0] + (int64_t)(kPer * i) * ld);
+                    v[i][0] = f.x; v[i][1] = f.y; v[i][2] = f.z; v[i][3] = f.w;
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) v[i][u] = base[0][(int64_t)(kPer * (4 * i + u)) * ld];
+                }
             }
+            base[0] += (int64_t)kBK * ld;
         }
+    }
+    // the last `left` < 32 steps
+    __device__ __forceinline__ void load_tail(int left) {
+#pragma unroll
+        for (int i = 0; i < kQuads; ++i)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                float f = 0.f;
+                if constexpr (K) {
+                    if ((int)(threadIdx.x & 7) * 4 + u < left) f = base[i][u];
+                } else if constexpr (WIDE) {
+                    if (kstep(i, u) < left) f = base[0][(int64_t)(kPer * i) * ld + u];
+                } else {
+                    if (kstep(i, u) < left) f = base[0][(int64_t)(kPer * (4 * i + u)) * ld];
+                }
+                v[i][u] = f;
+            }
     }
     __device__ __forceinline__ void store(float* s) const {
-        if constexpr (MODE == KC) {
 #pragma unroll
-            for (int i = 0; i < kRegs / 4; ++i)
-                *reinterpret_cast<float4*>(s + ((threadIdx.x >> 3) + 32 * i) * kPitch + (threadIdx.x & 7) * 4) =
-                    make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        } else {
+        for (int i = 0; i < kQuads; ++i) {
+            const float4 f = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+            if constexpr (K) {
+                *reinterpret_cast<float4*>(s + ((threadIdx.x >> 3) + 32 * i) * kPitch + (threadIdx.x & 7) * 4) = f;
+            } else if constexpr (WIDE) {
+                *reinterpret_cast<float4*>(s + kstep(i, 0) * kPitch + threadIdx.x % (T / 4) * 4) = f;
+            } else {
 #pragma unroll
-            for (int i = 0; i < kRegs; ++i) s[(threadIdx.x / T + i * (kThreads / T)) * kPitch + threadIdx.x % T] = v[i];
+                for (int u = 0; u < 4; ++u) s[kstep(i, u) * kPitch + threadIdx.x % T] = v[i][u];
+            }
         }
     }
-    // four steps (4q .. 4q+3 of this lane half) of row r
+    // four steps (4q .. 4q+3 of lane half h) of row r
     static __device__ __forceinline__ void frag(const float* s, int r, int h, int q, float* f) {
-        if constexpr (MODE == KC) {
+        if constexpr (K) {
             const float4 t = *reinterpret_cast<const float4*>(s + r * kPitch + h * 16 + 4 * q);
             f[0] = t.x; f[1] = t.y; f[2] = t.z; f[3] = t.w;
         } else {
@@ -150,8 +181,8 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
 
     SA sa;
     SB sb;
-    sa.init(a, m0);
-    sb.init(b, n0);
+    sa.init(a, m0, kbeg);
+    sb.init(b, n0, kbeg);
     f32x16 acc[MI][NI];
 #pragma unroll
     for (int x = 0; x < MI; ++x)
@@ -159,26 +190,22 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
         for (int y = 0; y < NI; ++y)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
-    float sq[EPI == EPI_SCORES ? SB::kRegs / 4 : 1] = {};
+    float sq[SB::kQuads] = {};
     float asum[MI] = {};
 
-    sa.load(a, kbeg, kend);
-    sb.load(b, kbeg, kend);
-    for (int64_t k0 = kbeg; k0 < kend; k0 += kBK) {
+    auto put = [&] {
         __syncthreads();   // the previous steps' fragments are read
         sa.store(s_a);
         sb.store(s_b);
         if constexpr (EPI == EPI_SCORES) {
 #pragma unroll
-            for (int i = 0; i < SB::kRegs / 4; ++i)
+            for (int i = 0; i < SB::kQuads; ++i)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) sq[i] = fmaf(sb.v[4 * i + u], sb.v[4 * i + u], sq[i]);
+                for (int u = 0; u < 4; ++u) sq[i] = fmaf(sb.v[i][u], sb.v[i][u], sq[i]);
         }
         __syncthreads();
-        if (k0 + kBK < kend) {
-            sa.load(a, k0 + kBK, kend);
-            sb.load(b, k0 + kBK, kend);
-        }
+    };
+    auto products = [&] {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             float fa[MI][4], fb[NI][4];
@@ -198,6 +225,26 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
                 for (int x = 0; x < MI; ++x) asum[x] += (fa[x][0] + fa[x][1]) + (fa[x][2] + fa[x][3]);
             }
         }
+    };
+    const int whole = (int)((kend - kbeg) / kBK), left = (int)((kend - kbeg) % kBK);
+    if (whole > 0) {
+        sa.load();
+        sb.load();
+        for (int it = 1; it < whole; ++it) {
+            put();
+            sa.load();     // on their way while the products run
+            sb.load();
+            __builtin_amdgcn_sched_barrier(0);
+            products();
+        }
+        put();
+        products();
+    }
+    if (left > 0) {
+        sa.load_tail(left);
+        sb.load_tail(left);
+        put();
+        products();
     }
 
     if constexpr (EPI == EPI_SCORES) {
@@ -205,7 +252,7 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
             if (threadIdx.x < TN) s_n[threadIdx.x] = n0 + threadIdx.x < b.rows ? sqnorm[n0 + threadIdx.x] : 0.f;
         } else {
 #pragma unroll
-            for (int i = 0; i < SB::kRegs / 4; ++i) {
+            for (int i = 0; i < SB::kQuads; ++i) {
                 float s = sq[i];   // the eight lanes that staged one row of B
                 s += __shfl_xor(s, 1, 64);
                 s += __shfl_xor(s, 2, 64);
@@ -248,19 +295,29 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
         }
 }
 
-// de[k, d] = scale * (sum_z part[z][k][d] - (sum_z rowsum[z][k]) * e[k][d]); pieces in order
+// de[k, d] = scale * (sum_z part[z][k][d] - (sum_z rowsum[z][k]) * e[k][d]); pieces in order, eight loads on their way at a time
 __global__ __launch_bounds__(256) void code_grad_join_kernel(const float* __restrict__ part, const float* __restrict__ rowsum,
                                                              const float* __restrict__ codebook, float* __restrict__ de, int splits,
                                                              int64_t K, int64_t D, float scale, int with_norm) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= K * D) return;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = K * D;
+    if (i >= n) return;
     const int64_t k = i / D;
     double s = 0.0, c = 0.0;
-    for (int z = 0; z < splits; ++z) s += (double)part[(int64_t)z * K * D + i];
-    if (with_norm) {
-        for (int z = 0; z < splits; ++z) c += (double)rowsum[(int64_t)z * K + k];
-        s -= c * (double)codebook[i];
+    for (int z0 = 0; z0 < splits; z0 += 8) {
+        float p[8], r[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int z = z0 + u < splits ? z0 + u : splits - 1;
+            p[u] = part[z * n + i];
+            r[u] = rowsum[z * K + k];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            s += z0 + u < splits ? (double)p[u] : 0.0;
+            c += z0 + u < splits ? (double)r[u] : 0.0;
+        }
     }
+    if (with_norm) s -= c * (double)codebook[i];
     de[i] = (float)(s * (double)scale);
 }
 
@@ -322,14 +379,19 @@ extern "C" int lbm_code_logits_f32(const float* x, int64_t ldx, int32_t layout, 
         LBM_REQUIRE(S >= 1 && ldx >= S && N % S == 0, LBM_EINVAL,
                     "%s: channel-major needs 1 <= S <= ldx and N %% S == 0 (N=%lld, S=%lld, ldx=%lld)", what, (long long)N, (long long)S,
                     (long long)ldx);
-    const Operand b{codebook, D, 0, 0, K, aligned16(codebook, D)};
+    const Operand b{codebook, D, 0, 0, K};
+    const bool wide_b = aligned16(codebook, D);
     const float scale = (float)(1.0 / temperature);
+    hipStream_t st = lbm::as_stream(stream);
     if (layout == LBM_VQ_ROWS) {
-        const Operand a{x, ldx, 0, 0, N, aligned16(x, ldx)};
-        return launch_mm<KC, KC, EPI_SCORES>(what, a, b, logits, ldl, D, 1, D, scale, e_sqnorm_or_null, nullptr, lbm::as_stream(stream));
+        const Operand a{x, ldx, 0, 0, N};
+        return wide_b && aligned16(x, ldx)
+                   ? launch_mm<KCV, KCV, EPI_SCORES>(what, a, b, logits, ldl, D, 1, D, scale, e_sqnorm_or_null, nullptr, st)
+                   : launch_mm<KC, KC, EPI_SCORES>(what, a, b, logits, ldl, D, 1, D, scale, e_sqnorm_or_null, nullptr, st);
     }
-    const Operand a{x, ldx, S, (int64_t)D * ldx, N, 0};
-    return launch_mm<MC, KC, EPI_SCORES>(what, a, b, logits, ldl, D, 1, D, scale, e_sqnorm_or_null, nullptr, lbm::as_stream(stream));
+    const Operand a{x, ldx, S, (int64_t)D * ldx, N};
+    return wide_b ? launch_mm<MC, KCV, EPI_SCORES>(what, a, b, logits, ldl, D, 1, D, scale, e_sqnorm_or_null, nullptr, st)
+                  : launch_mm<MC, KC, EPI_SCORES>(what, a, b, logits, ldl, D, 1, D, scale, e_sqnorm_or_null, nullptr, st);
 }
 
 extern "C" size_t lbm_code_logits_grad_workspace_bytes(int64_t N, int32_t D, int32_t K) {
@@ -354,9 +416,10 @@ extern "C" int lbm_code_logits_grad_f32(const float* g, int64_t ldg, const float
     hipStream_t st = lbm::as_stream(stream);
     const float scale = (float)(2.0 / temperature);
     if (dx_or_null != nullptr && N > 0) {
-        const Operand a{g, ldg, 0, 0, N, aligned16(g, ldg)};
-        const Operand b{codebook, D, 0, 0, D, 0};
-        const int rc = launch_mm<KC, MC, EPI_SCALE>(what, a, b, dx_or_null, D, K, 1, K, scale, nullptr, nullptr, st);
+        const Operand a{g, ldg, 0, 0, N}, b{codebook, D, 0, 0, D};
+        const int rc = aligned16(g, ldg) && aligned16(codebook, D)
+                           ? launch_mm<KCV, MCV, EPI_SCALE>(what, a, b, dx_or_null, D, K, 1, K, scale, nullptr, nullptr, st)
+                           : launch_mm<KC, MC, EPI_SCALE>(what, a, b, dx_or_null, D, K, 1, K, scale, nullptr, nullptr, st);
         if (rc != LBM_OK) return rc;
     }
     if (de_or_null != nullptr) {
@@ -367,9 +430,11 @@ extern "C" int lbm_code_logits_grad_f32(const float* g, int64_t ldg, const float
         if (N > 0) {
             plan_split(N, D, K, &splits, &piece);
             rowsum = part + (int64_t)splits * K * D;
-            const Operand a{g, ldg, 0, 0, K, 0};
-            const Operand b{x, ldx, 0, 0, D, 0};
-            const int rc = launch_mm<MC, MC, EPI_PARTIAL>(what, a, b, part, D, N, splits, piece, 1.f, nullptr, rowsum, st);
+            const Operand a{g, ldg, 0, 0, K}, b{x, ldx, 0, 0, D};
+            // four rows of an operand at a time: their number has to be a multiple of four too
+            const int rc = aligned16(g, ldg) && aligned16(x, ldx) && ((K | D) & 3) == 0
+                               ? launch_mm<MCV, MCV, EPI_PARTIAL>(what, a, b, part, D, N, splits, piece, 1.f, nullptr, rowsum, st)
+                               : launch_mm<MC, MC, EPI_PARTIAL>(what, a, b, part, D, N, splits, piece, 1.f, nullptr, rowsum, st);
             if (rc != LBM_OK) return rc;
         }
         const int64_t total = (int64_t)K * D;
