@@ -25,7 +25,7 @@ class _CodeLogits(torch.autograd.Function):
         K = codebook.shape[0]
         out = torch.empty((N, K), dtype=torch.float32, device=x.device)
         _lib.check(_lib.load().lbm_code_logits_f32(_lib.ptr(x), x.stride(0) if N > 1 else D, _lib.VQ_ROWS, 0, _lib.ptr(codebook),
-                                                   _lib.ptr(e_sqnorm), _lib.ptr(out), K, N, D, K, temperature, _lib.stream_ptr()),
+                                                   _lib.ptr(e_sqnorm), out.data_ptr(), K, N, D, K, temperature, _lib.stream_ptr()),
                    "lbm_code_logits_f32")
         ctx.save_for_backward(x, codebook)
         ctx.temperature, ctx.norm_grad = temperature, e_sqnorm is None
@@ -42,11 +42,14 @@ class _CodeLogits(torch.autograd.Function):
             g = g.contiguous()
         lib = _lib.load()
         dx = torch.empty((N, D), dtype=torch.float32, device=x.device) if need_x else None
-        de = torch.empty((K, D), dtype=torch.float32, device=x.device) if need_e else None
-        ws = torch.empty((lib.lbm_code_logits_grad_workspace_bytes(N, D, K),), dtype=torch.uint8, device=x.device) if need_e else None
-        _lib.check(lib.lbm_code_logits_grad_f32(_lib.ptr(g), g.stride(0) if N > 1 else K, _lib.ptr(x), x.stride(0) if N > 1 else D,
-                                                _lib.ptr(codebook), _lib.ptr(dx), _lib.ptr(de), int(ctx.norm_grad), _lib.ptr(ws), N, D, K,
-                                                ctx.temperature, _lib.stream_ptr()), "lbm_code_logits_grad_f32")
+        de = ws = None
+        if need_e:
+            de = torch.empty((K, D), dtype=torch.float32, device=x.device)
+            ws = torch.empty((lib.lbm_code_logits_grad_workspace_bytes(N, D, K),), dtype=torch.uint8, device=x.device)
+        _lib.check(lib.lbm_code_logits_grad_f32(_lib.ptr(g), g.stride(0) if N > 1 else K, x.data_ptr(), x.stride(0) if N > 1 else D,
+                                                codebook.data_ptr(), dx.data_ptr() if need_x else None, de.data_ptr() if need_e else None,
+                                                int(ctx.norm_grad), ws.data_ptr() if need_e else None, N, D, K, ctx.temperature,
+                                                _lib.stream_ptr()), "lbm_code_logits_grad_f32")
         return dx, de, None, None
 
 
@@ -55,7 +58,7 @@ def _f32_param(t, what):
         return _lib.dev_f32(t)
     if not t.is_floating_point():
         raise ValueError(f"{what} must be a floating-point tensor")
-    return t.to(torch.float32)
+    return t if t.dtype is torch.float32 else t.to(torch.float32)
 
 
 @_lib.on_tensor_device

@@ -146,8 +146,7 @@ struct Stage {
 enum { EPI_SCORES = 0, EPI_SCALE = 1, EPI_PARTIAL = 2 };
 
 struct Tiles {
-    int64_t mt;     // tiles along the rows of A
-    int nt;         // tiles along the rows of B
+    int mt, nt;     // tiles along the rows of A and of B
     int splits;     // pieces of the contraction (EPI_PARTIAL)
     int64_t piece;  // steps of one piece
 };
@@ -170,66 +169,92 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
     const int j = lane & 31, h = lane >> 5;
     const int wm = (wave >> 1) * (TM / 2), wn = (wave & 1) * (TN / 2);
 
-    // workgroups go round the 8 XCDs: give each XCD a contiguous run of tiles, B tiles fastest, so that the tiles that share A's rows
-    // meet in one L2
-    const int64_t total = t.mt * t.nt, per = total / 8, rem = total % 8;
-    const int64_t xcd = blockIdx.x % 8, slot = blockIdx.x / 8;
-    const int64_t tile = xcd * per + (xcd < rem ? xcd : rem) + slot;
-    const int64_t m0 = tile / t.nt * TM, n0 = tile % t.nt * TN;
-    const int64_t kbeg = (int64_t)blockIdx.y * t.piece;
-    const int64_t kend = kbeg + t.piece < depth ? kbeg + t.piece : depth;
+    // Workgroups go round the 8 XCDs: each XCD works through a contiguous run of tiles, B tiles fastest, so that the tiles that share A's
+    // rows meet in one L2.  A workgroup takes every n-th tile of its XCD's run and requests the next tile's first steps before it stores
+    // the present one's results.
+    const int64_t total = (int64_t)t.mt * t.nt * t.splits;
+    const int xcd = blockIdx.x & 7, each = gridDim.x >> 3, more = gridDim.x & 7;
+    const int per_xcd = each + (xcd < more ? 1 : 0), before = xcd * each + (xcd < more ? xcd : more);
+    const int64_t run0 = total * before / gridDim.x, run1 = total * (before + per_xcd) / gridDim.x;
+    int64_t item = run0 + (blockIdx.x >> 3);
+    if (item >= run1) return;
 
     SA sa;
     SB sb;
-    sa.init(a, m0, kbeg);
-    sb.init(b, n0, kbeg);
-    f32x16 acc[MI][NI];
+    int64_t m0, n0;
+    int z, whole, left;
+    auto begin = [&](int64_t i) {
+        const int64_t tiles = (int64_t)t.mt * t.nt, tile = i % tiles;
+        z = (int)(i / tiles);
+        m0 = tile / t.nt * TM;
+        n0 = tile % t.nt * TN;
+        const int64_t kbeg = z * t.piece, kend = kbeg + t.piece < depth ? kbeg + t.piece : depth;
+        whole = (int)((kend - kbeg) / kBK);
+        left = (int)((kend - kbeg) % kBK);
+        sa.init(a, m0, kbeg);
+        sb.init(b, n0, kbeg);
+        if (whole > 0) {
+            sa.load();
+            sb.load();
+        }
+    };
+    begin(item);
+    for (;;) {
+        f32x16 acc[MI][NI];
 #pragma unroll
-    for (int x = 0; x < MI; ++x)
+        for (int x = 0; x < MI; ++x)
 #pragma unroll
-        for (int y = 0; y < NI; ++y)
+            for (int y = 0; y < NI; ++y)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
-    float sq[SB::kQuads] = {};
-    float asum[MI] = {};
+                for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
+        float sq[SB::kQuads] = {};
+        float asum[MI] = {};
 
-    auto put = [&] {
-        __syncthreads();   // the previous steps' fragments are read
-        sa.store(s_a);
-        sb.store(s_b);
-        if constexpr (EPI == EPI_SCORES) {
+        auto put = [&] {
+            // the waves that stage go before those that multiply: two workgroups share a SIMD, and the other one's products fill the
+            // gap (40000 x 8192 x 256: 1476 -> 1435 us)
+            __builtin_amdgcn_s_setprio(1);
+            __syncthreads();   // the previous steps' fragments are read
+            sa.store(s_a);
+            sb.store(s_b);
+            if constexpr (EPI == EPI_SCORES) {
 #pragma unroll
-            for (int i = 0; i < SB::kQuads; ++i)
+                for (int i = 0; i < SB::kQuads; ++i)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) sq[i] = fmaf(sb.v[i][u], sb.v[i][u], sq[i]);
-        }
-        __syncthreads();
-    };
-    auto products = [&] {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float fa[MI][4], fb[NI][4];
-#pragma unroll
-            for (int x = 0; x < MI; ++x) SA::frag(s_a, wm + 32 * x + j, h, q, fa[x]);
-#pragma unroll
-            for (int y = 0; y < NI; ++y) SB::frag(s_b, wn + 32 * y + j, h, q, fb[y]);
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int x = 0; x < MI; ++x)
-#pragma unroll
-                    for (int y = 0; y < NI; ++y)
-                        acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[x][u], fb[y][u], acc[x][y], 0, 0, 0);
-            if constexpr (EPI == EPI_PARTIAL) {
-#pragma unroll
-                for (int x = 0; x < MI; ++x) asum[x] += (fa[x][0] + fa[x][1]) + (fa[x][2] + fa[x][3]);
+                    for (int u = 0; u < 4; ++u) sq[i] = fmaf(sb.v[i][u], sb.v[i][u], sq[i]);
             }
-        }
-    };
-    const int whole = (int)((kend - kbeg) / kBK), left = (int)((kend - kbeg) % kBK);
-    if (whole > 0) {
-        sa.load();
-        sb.load();
+            __syncthreads();
+        };
+        auto products = [&] {
+            // fragments of the next four steps are read while the products of these run
+            float fa[2][MI][4], fb[2][NI][4];
+            auto read = [&](int q, int to) {
+#pragma unroll
+                for (int x = 0; x < MI; ++x) SA::frag(s_a, wm + 32 * x + j, h, q, fa[to][x]);
+#pragma unroll
+                for (int y = 0; y < NI; ++y) SB::frag(s_b, wn + 32 * y + j, h, q, fb[to][y]);
+            };
+            read(0, 0);
+            __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int c = q & 1;
+                if (q < 3) read(q + 1, c ^ 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int x = 0; x < MI; ++x)
+#pragma unroll
+                        for (int y = 0; y < NI; ++y)
+                            acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[c][x][u], fb[c][y][u], acc[x][y], 0, 0, 0);
+                if constexpr (EPI == EPI_PARTIAL) {
+#pragma unroll
+                    for (int x = 0; x < MI; ++x) asum[x] += (fa[c][x][0] + fa[c][x][1]) + (fa[c][x][2] + fa[c][x][3]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
         for (int it = 1; it < whole; ++it) {
             put();
             sa.load();     // on their way while the products run
@@ -237,62 +262,70 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
             __builtin_amdgcn_sched_barrier(0);
             products();
         }
-        put();
-        products();
-    }
-    if (left > 0) {
-        sa.load_tail(left);
-        sb.load_tail(left);
-        put();
-        products();
-    }
+        if (whole > 0) {
+            put();
+            products();
+        }
+        if (left > 0) {
+            sa.load_tail(left);
+            sb.load_tail(left);
+            put();
+            products();
+        }
+        const int64_t m0_now = m0, n0_now = n0;
+        const int z_now = z;
+        item += per_xcd;
+        if (item < run1) begin(item);
+        __builtin_amdgcn_sched_barrier(0);
 
-    if constexpr (EPI == EPI_SCORES) {
-        if (sqnorm != nullptr) {
-            if (threadIdx.x < TN) s_n[threadIdx.x] = n0 + threadIdx.x < b.rows ? sqnorm[n0 + threadIdx.x] : 0.f;
-        } else {
+        if constexpr (EPI == EPI_SCORES) {
+            if (sqnorm != nullptr) {
+                if (threadIdx.x < TN) s_n[threadIdx.x] = n0_now + threadIdx.x < b.rows ? sqnorm[n0_now + threadIdx.x] : 0.f;
+            } else {
 #pragma unroll
-            for (int i = 0; i < SB::kQuads; ++i) {
-                float s = sq[i];   // the eight lanes that staged one row of B
-                s += __shfl_xor(s, 1, 64);
-                s += __shfl_xor(s, 2, 64);
-                s += __shfl_xor(s, 4, 64);
-                if ((threadIdx.x & 7) == 0) s_n[(threadIdx.x >> 3) + 32 * i] = s;
+                for (int i = 0; i < SB::kQuads; ++i) {
+                    float s = sq[i];   // the eight lanes that staged one row of B
+                    s += __shfl_xor(s, 1, 64);
+                    s += __shfl_xor(s, 2, 64);
+                    s += __shfl_xor(s, 4, 64);
+                    if ((threadIdx.x & 7) == 0) s_n[(threadIdx.x >> 3) + 32 * i] = s;
+                }
             }
+            __syncthreads();           // (the next tile's first barrier keeps its s_n behind this one's reads)
         }
-        __syncthreads();
-    }
-    if constexpr (EPI == EPI_PARTIAL) {
-        out += (int64_t)blockIdx.y * a.rows * ldo;
-        if (n0 == 0 && wn == 0) {
+        float* o = out;
+        if constexpr (EPI == EPI_PARTIAL) {
+            o += (int64_t)z_now * a.rows * ldo;
+            if (n0_now == 0 && wn == 0) {
 #pragma unroll
-            for (int x = 0; x < MI; ++x) {
-                const float s = asum[x] + __shfl_xor(asum[x], 32, 64);
-                const int64_t m = m0 + wm + 32 * x + j;
-                if (h == 0 && m < a.rows) rowsum[(int64_t)blockIdx.y * a.rows + m] = s;
-            }
-        }
-    }
-#pragma unroll
-    for (int x = 0; x < MI; ++x)
-#pragma unroll
-        for (int y = 0; y < NI; ++y) {
-            const int nl = wn + 32 * y + j;
-            const int64_t n = n0 + nl;
-            if (n < b.rows) {
-                const float e = EPI == EPI_SCORES ? s_n[nl] : 0.f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int64_t m = m0 + wm + 32 * x + (r & 3) + 8 * (r >> 2) + 4 * h;
-                    if (m < a.rows) {
-                        float v = acc[x][y][r];
-                        if constexpr (EPI == EPI_SCORES) v = (2.f * v - e) * scale;
-                        if constexpr (EPI == EPI_SCALE) v = v * scale;
-                        out[m * ldo + n] = v;
-                    }
+                for (int x = 0; x < MI; ++x) {
+                    const float s = asum[x] + __shfl_xor(asum[x], 32, 64);
+                    const int64_t m = m0_now + wm + 32 * x + j;
+                    if (h == 0 && m < a.rows) rowsum[(int64_t)z_now * a.rows + m] = s;
                 }
             }
         }
+        const bool inside = m0_now + TM <= a.rows && n0_now + TN <= b.rows;
+#pragma unroll
+        for (int x = 0; x < MI; ++x)
+#pragma unroll
+            for (int y = 0; y < NI; ++y) {
+                const int nl = wn + 32 * y + j;
+                const int64_t n = n0_now + nl, m = m0_now + wm + 32 * x + 4 * h;
+                const float e = EPI == EPI_SCORES ? s_n[nl] : 0.f;
+                float* q = o + m * ldo + n;
+                const bool col = n < b.rows;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int dm = (r & 3) + 8 * (r >> 2);
+                    float v = acc[x][y][r];
+                    if constexpr (EPI == EPI_SCORES) v = (2.f * v - e) * scale;
+                    if constexpr (EPI == EPI_SCALE) v = v * scale;
+                    if (inside || (col && m + dm < a.rows)) q[dm * ldo] = v;
+                }
+            }
+        if (item >= run1) return;
+    }
 }
 
 // de[k, d] = scale * (sum_z part[z][k][d] - (sum_z rowsum[z][k]) * e[k][d]); pieces in order, eight loads on their way at a time
@@ -323,25 +356,32 @@ __global__ __launch_bounds__(256) void code_grad_join_kernel(const float* __rest
 
 bool aligned16(const float* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
 
+template <int TM, int TN, int AM, int BM, int EPI>
+int launch_tiles(const char* what, const Operand& a, const Operand& b, float* out, int64_t ldo, int64_t depth, int splits, int64_t piece,
+                 float scale, const float* sqnorm, float* rowsum, hipStream_t st) {
+    const int64_t mt = (a.rows + TM - 1) / TM, nt = (b.rows + TN - 1) / TN;
+    if (mt > 0x7fffffffLL || nt > 0x7fffffffLL) return lbm::fail(LBM_EUNSUPPORTED, "%s: too many tiles", what);
+    const Tiles t{(int)mt, (int)nt, splits, piece};
+    const int64_t total = mt * nt * splits, fit = TM * TN >= 128 * 128 ? 512 : 1024;      // workgroups that run at a time
+    hipLaunchKernelGGL((code_mm_kernel<TM, TN, AM, BM, EPI>), dim3((unsigned)(total < fit ? total : fit)), dim3(kThreads), 0, st, a, b, out, ldo,
+                       depth, t, scale, sqnorm, rowsum);
+    return lbm::check_launch(what);
+}
+
 template <int AM, int BM, int EPI>
 int launch_mm(const char* what, const Operand& a, const Operand& b, float* out, int64_t ldo, int64_t depth, int splits, int64_t piece,
               float scale, const float* sqnorm, float* rowsum, hipStream_t st) {
-    // 128 x 128 tiles while they fill the 256 CUs; 64 x 64 (a quarter of the work each) below that
-    const int64_t big = ((a.rows + 127) / 128) * ((b.rows + 127) / 128) * splits;
-    const int T = big >= 256 ? 128 : 64;
-    Tiles t;
-    t.mt = (a.rows + T - 1) / T;
-    t.nt = (int)((b.rows + T - 1) / T);
-    t.splits = splits;
-    t.piece = piece;
-    const int64_t blocks = t.mt * t.nt;
-    if (blocks > 0x7fffffffLL) return lbm::fail(LBM_EUNSUPPORTED, "%s: grid too large", what);
-    const dim3 grid((unsigned)blocks, (unsigned)splits);
-    if (T == 128)
-        hipLaunchKernelGGL((code_mm_kernel<128, 128, AM, BM, EPI>), grid, dim3(kThreads), 0, st, a, b, out, ldo, depth, t, scale, sqnorm, rowsum);
-    else
-        hipLaunchKernelGGL((code_mm_kernel<64, 64, AM, BM, EPI>), grid, dim3(kThreads), 0, st, a, b, out, ldo, depth, t, scale, sqnorm, rowsum);
-    return lbm::check_launch(what);
+    // The largest tile whose last round leaves few CUs idle: a round of 128 x 128 tiles on the 256 CUs takes twice one of 64 x 128
+    auto rounds = [&](int tm, int tn) {
+        const int64_t n = ((a.rows + tm - 1) / tm) * ((b.rows + tn - 1) / tn) * splits;
+        return (n + 255) / 256 * (tm * tn);
+    };
+    const int64_t r128 = rounds(128, 128), r64 = rounds(64, 128), r32 = rounds(64, 64);
+    if (r128 <= r64 + r64 / 8 && r128 <= r32 + r32 / 4)
+        return launch_tiles<128, 128, AM, BM, EPI>(what, a, b, out, ldo, depth, splits, piece, scale, sqnorm, rowsum, st);
+    if (r64 <= r32 + r32 / 8)
+        return launch_tiles<64, 128, AM, BM, EPI>(what, a, b, out, ldo, depth, splits, piece, scale, sqnorm, rowsum, st);
+    return launch_tiles<64, 64, AM, BM, EPI>(what, a, b, out, ldo, depth, splits, piece, scale, sqnorm, rowsum, st);
 }
 
 constexpr int64_t kMaxPiece = 32768;   // rows of one fp32 accumulator chain in the codebook's gradient; pieces are joined in 64 bits
