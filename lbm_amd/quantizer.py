@@ -13,6 +13,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import _lib
+from .codes import CodeSampling, code_balance_loss, code_logits, sample_codes
 from .constants import VQ_EMBEDDING_DIM
 
 
@@ -320,8 +321,15 @@ def encoder_forward(x: torch.Tensor, enc: "nn.Sequential | dict", pitched_out: b
 
 # ------------------------------------------------------------------------------------------ modules
 class VectorQuantizerEMA(nn.Module):
-    def __init__(self, num_embeddings, embedding_dim, commitment_cost, decay, epsilon=1e-5):
+    """The reference's quantizer.  ``balance_weight`` > 0 (not a reference argument) adds that many times the usage-balance loss
+    (``code_balance_loss`` of the scores ``code_logits(z, codebook, balance_temperature)`` and the codes picked) to the loss in training mode:
+    its gradient pulls the encoder's outputs towards codes that are used too little.  The codebook itself goes on learning by EMA only."""
+    balance_weight, balance_temperature = 0.0, 1.0       # of modules pickled without them
+
+    def __init__(self, num_embeddings, embedding_dim, commitment_cost, decay, epsilon=1e-5, balance_weight=0.0, balance_temperature=1.0):
         super().__init__()
+        self.balance_weight = balance_weight
+        self.balance_temperature = balance_temperature
         self.embedding_dim = embedding_dim
         self.num_embeddings = num_embeddings
         self.commitment_cost = commitment_cost
@@ -363,6 +371,11 @@ class VectorQuantizerEMA(nn.Module):
         if self.training or grad_path:
             # differentiable gather with the PRE-update codebook (training/model.py:100)
             quantized = F.embedding(idx, w).view(input_shape)
+        balance = None
+        if self.training and self.balance_weight > 0:
+            # on a copy: the EMA kernel below rewrites the codebook before the backward pass reads it
+            scores = code_logits(flat_input, w.detach().clone(), self.balance_temperature)
+            balance = code_balance_loss(scores, idx)[0]
         if self.training:
             # EMA codebook update (training/model.py:103-126): deterministic segmented sums instead of the
             # one-hot matmuls, then the in-place EMA kernel.  With `ema_group` set (one process per GPU), the
@@ -384,6 +397,8 @@ class VectorQuantizerEMA(nn.Module):
             e_latent_loss = F.mse_loss(quantized.detach(), inputs)
             q_latent_loss = F.mse_loss(quantized, inputs.detach())
             loss = q_latent_loss + self.commitment_cost * e_latent_loss
+            if balance is not None:
+                loss = loss + self.balance_weight * balance
             quantized = inputs + (quantized - inputs).detach()
         else:
             q, err = vq_gather_loss(flat_input.detach(), w.detach(), idx)
@@ -395,7 +410,7 @@ class VectorQuantizerEMA(nn.Module):
 
 
 class VQVAE(nn.Module):
-    def __init__(self, input_channels, embedding_dim, num_embeddings, commitment_cost, decay):
+    def __init__(self, input_channels, embedding_dim, num_embeddings, commitment_cost, decay, balance_weight=0.0, balance_temperature=1.0):
         super().__init__()
         self.input_channels = input_channels
         self.embedding_dim = embedding_dim
@@ -404,7 +419,8 @@ class VQVAE(nn.Module):
             nn.Conv1d(64, 128, kernel_size=4, stride=2, padding=1), nn.ReLU(),
             nn.Conv1d(128, 256, kernel_size=3, stride=1, padding=1), nn.ReLU(),
             nn.Conv1d(256, embedding_dim, kernel_size=1, stride=1))
-        self.vq_layer = VectorQuantizerEMA(num_embeddings, embedding_dim, commitment_cost, decay)
+        self.vq_layer = VectorQuantizerEMA(num_embeddings, embedding_dim, commitment_cost, decay, balance_weight=balance_weight,
+                                           balance_temperature=balance_temperature)
         self.decoder = nn.Sequential(
             nn.ConvTranspose1d(embedding_dim, 256, kernel_size=1, stride=1), nn.ReLU(),
             nn.ConvTranspose1d(256, 128, kernel_size=3, stride=1, padding=1), nn.ReLU(),
@@ -460,19 +476,45 @@ class VQVAE(nn.Module):
         idx = vq_argmin(h, cb, ee, channel_major=True, no_xnorm=folded, hist=hist_s, split_tables=tab, screened=True)
         return remap_codes(idx, cmap, kp, hist_s, hist)
 
+    def _sampled_indices(self, h, cb, e_sqnorm, sampling, u, generator, hist):
+        """Codes drawn for h[B, D, S], a run of epochs at a time so that their scores (at most 256 MiB) stay in the last-level cache."""
+        B, _, S = h.shape
+        K = cb.shape[0]
+        if u is None:
+            u = torch.rand((B, S), generator=generator, device=h.device)
+        elif tuple(u.shape) != (B, S):
+            raise ValueError(f"u must be [{B}, {S}], got {tuple(u.shape)}")
+        out = torch.empty((B, S), dtype=torch.int64, device=h.device)
+        step = max(1, (1 << 26) // max(1, S * K))
+        for b in range(0, B, step):
+            scores = code_logits(h[b:b + step], cb, e_sqnorm=e_sqnorm, channel_major=True)
+            out[b:b + step] = sample_codes(scores.view(-1, S, K), u[b:b + step], temperature=sampling.temperature, top_k=sampling.top_k,
+                                           top_p=sampling.top_p, min_p=sampling.min_p, allowed=sampling.allowed, hist=hist)
+        return out
+
     @torch.no_grad()
     @_lib.on_tensor_device
-    def encode(self, x, hist=None, fold_projection: bool = False, screened: bool = False):
+    def encode(self, x, hist=None, fold_projection: bool = False, screened: bool = False, sampling: CodeSampling = None, u=None,
+               generator=None):
         """Input x[B, C, L] -> code indices int64 [B, L//4] (training/model.py:206-214), all on HIP kernels;
         the encoder output is consumed channel-major, so the permute(0,2,1).contiguous() copy disappears.
         ``fold_projection=True``: the last 1x1 convolution is folded into the codebook (see ``fold_projection``): its GEMM and
         the z tensor disappear; indices equal the default's except at documented fp32 near-ties.
         ``screened=True``: the same indices as without it, bit for bit, from the screened search (``lbm_vq_argmin_screened_f32``:
-        2.4x faster at the shipped sizes)."""
+        2.4x faster at the shipped sizes).
+        ``sampling=CodeSampling(...)``: each code is drawn from softmax(-distance / temperature) under its filters (``sample_codes``)
+        instead of the nearest, with the uniform numbers ``u`` [B, L//4], or without them ones from ``generator``."""
+        if sampling is not None and screened:
+            raise ValueError("encode: screened=True settles the nearest code and has no scores to draw from")
+        if sampling is None and (u is not None or generator is not None):
+            raise ValueError("encode: u and generator belong to sampling=CodeSampling(...)")
         if fold_projection:
             h = x
             for i, (st, pd) in zip((0, 2, 4), ((2, 1), (2, 1), (1, 1))):
                 h = conv1d(h, self.encoder[i].weight, self.encoder[i].bias, st, pd, True, pitched_out=True)
+            if sampling is not None:
+                cbf, eef = self._folded_codebook()
+                return self._sampled_indices(h, cbf, eef, sampling, u, generator, hist)
             if screened:
                 idx = self._screened_indices(h, True, hist)
             else:
@@ -480,6 +522,8 @@ class VQVAE(nn.Module):
                 idx = vq_argmin(h, cbf, eef, channel_major=True, no_xnorm=True, hist=hist)
             return idx.view(x.shape[0], -1)
         z = encoder_forward(x, self.encoder, pitched_out=True)
+        if sampling is not None:
+            return self._sampled_indices(z, self.vq_layer.embedding.weight, None, sampling, u, generator, hist)
         if screened:
             idx = self._screened_indices(z.detach(), False, hist)
         else:
@@ -487,16 +531,18 @@ class VQVAE(nn.Module):
         return idx.view(x.shape[0], -1)
 
 
-def encode_data_for_transformer(vq_model, dataloader, device, fold_projection: bool = False, screened: bool = False):
+def encode_data_for_transformer(vq_model, dataloader, device, fold_projection: bool = False, screened: bool = False,
+                                sampling: CodeSampling = None, generator=None):
     """training/model.py:411-427: returns (np.int64 [E, S] indices, np labels).  Batches are encoded
-    back-to-back on the device; indices come back to the host once, after the loop.  ``fold_projection`` and ``screened`` (not
-    reference arguments) are handed to ``VQVAE.encode``."""
+    back-to-back on the device; indices come back to the host once, after the loop.  ``fold_projection``, ``screened``, ``sampling``
+    and ``generator`` (not reference arguments) are handed to ``VQVAE.encode``."""
     vq_model.eval()
     all_indices, all_labels = [], []
     with torch.no_grad():
         for data, labels in dataloader:
             data = data.to(device, non_blocking=True)
-            all_indices.append(vq_model.encode(data, fold_projection=fold_projection, screened=screened))
+            all_indices.append(vq_model.encode(data, fold_projection=fold_projection, screened=screened, sampling=sampling,
+                                               generator=generator))
             all_labels.append(labels.numpy() if isinstance(labels, torch.Tensor) else np.asarray(labels))
     all_indices = torch.cat(all_indices, dim=0).cpu().numpy()
     all_labels = np.concatenate(all_labels, axis=0)

@@ -568,3 +568,100 @@ def test_two_graphs_replayed_in_turn():
             torch.cuda.synchronize()
             for a, b in zip(out, _step(x, e, u, keep)):
                 assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------------------- in the tokenizer
+def _model(shipped, **kw):
+    m = lbm_amd.VQVAE(30, 256, 512, 0.25, 0.99, **kw)
+    m.load_state_dict({k: torch.from_numpy(np.asarray(v)) for k, v in shipped.items()}, strict=False)
+    return m.to(DEV)
+
+
+@pytest.mark.parametrize("fold", [False, True])
+def test_encode_with_sampling(shipped, fold):
+    m = _model(shipped).eval()
+    x = torch.randn((5, 30, 500), generator=gen(1)).to(DEV)
+    nearest = m.encode(x, fold_projection=fold)
+    B, S = nearest.shape
+    # temperature 0 is the nearest code; where the two differ, the distances do by rounding only: |x|^2 + |e|^2 - 2 x.e in fp32 (256 terms)
+    greedy = m.encode(x, fold_projection=fold, sampling=lbm_amd.CodeSampling(temperature=0.0), u=torch.zeros((B, S), device=DEV))
+    z = lbm_amd.encoder_forward(x, m.encoder).permute(0, 2, 1).reshape(-1, 256)
+    z64, e64 = f64(z), f64(m.vq_layer.embedding.weight)
+    d = ((z64[:, None, :] - e64[None]) ** 2).sum(2)
+    rows = np.arange(B * S)
+    gap = np.abs(d[rows, greedy.cpu().numpy().ravel()] - d[rows, nearest.cpu().numpy().ravel()])
+    assert (gap <= 2 * 264 * U * ((z64 ** 2).sum(1) + (e64 ** 2).sum(1).max()) * (4 if fold else 1)).all()
+    # drawn codes are sample_codes of code_logits, whatever the chunking
+    u = torch.rand((B, S), generator=gen(2)).to(DEV)
+    hist = torch.zeros((512,), dtype=torch.int64, device=DEV)
+    set_ = lbm_amd.CodeSampling(temperature=0.5, top_k=20, top_p=0.95, min_p=0.01)
+    got = m.encode(x, hist=hist, fold_projection=fold, sampling=set_, u=u)
+    assert got.shape == (B, S) and got.dtype == torch.int64
+    assert np.array_equal(hist.cpu().numpy(), np.bincount(got.cpu().numpy().ravel(), minlength=512))
+    if not fold:
+        zc = lbm_amd.encoder_forward(x, m.encoder, pitched_out=True)
+        scores = lbm_amd.code_logits(zc, m.vq_layer.embedding.weight.detach(), channel_major=True)
+        want = lbm_amd.sample_codes(scores, u.reshape(-1), temperature=0.5, top_k=20, top_p=0.95, min_p=0.01)
+        assert torch.equal(got.reshape(-1), want)
+        assert np.array_equal(want.cpu().numpy(), sample64(f64(scores), f64(u).ravel(), np.full(B * S, 0.5), np.full(B * S, 20), np.full(B * S, 0.95),
+                                                           np.full(B * S, 0.01)))
+    # codes that may not be drawn are not; numbers from a generator repeat with its seed
+    allowed = torch.zeros((512,), dtype=torch.bool, device=DEV)
+    allowed[[3, 77, 200]] = True
+    only = lbm_amd.CodeSampling(temperature=10.0, allowed=allowed)
+    a = m.encode(x, fold_projection=fold, sampling=only, generator=torch.Generator(device=DEV).manual_seed(5))
+    b = m.encode(x, fold_projection=fold, sampling=only, generator=torch.Generator(device=DEV).manual_seed(5))
+    assert torch.equal(a, b) and set(a.unique().tolist()) <= {3, 77, 200}
+    for kw in (dict(screened=True, sampling=set_), dict(u=u), dict(sampling=set_, u=u[:, :-1])):
+        with pytest.raises(ValueError):
+            m.encode(x, fold_projection=fold, **kw)
+
+
+def test_encode_data_for_transformer_with_sampling(shipped):
+    m = _model(shipped)
+    data = [(torch.randn((2, 30, 100), generator=gen(i)), torch.tensor([i, i])) for i in range(3)]
+    one = lbm_amd.encode_data_for_transformer(m, data, DEV, sampling=lbm_amd.CodeSampling(temperature=2.0),
+                                              generator=torch.Generator(device=DEV).manual_seed(1))
+    two = lbm_amd.encode_data_for_transformer(m, data, DEV, sampling=lbm_amd.CodeSampling(temperature=2.0),
+                                              generator=torch.Generator(device=DEV).manual_seed(1))
+    assert one[0].shape == (6, 25) and one[0].dtype == np.int64 and np.array_equal(one[0], two[0]) and one[1].tolist() == [0, 0, 1, 1, 2, 2]
+    assert not np.array_equal(one[0], lbm_amd.encode_data_for_transformer(m, data, DEV)[0])
+
+
+def test_quantizer_training_step_with_balance():
+    """The balance term's gradient reaches the inputs through the codebook as it was BEFORE the step's EMA update, which itself is the one
+    without the term."""
+    N, D, K, wgt, T = 96, 16, 24, 0.7, 0.5
+    x = torch.randn((4, N // 4, D), generator=gen(1))
+    results = {}
+    for weight in (0.0, wgt):
+        torch.manual_seed(3)
+        q = lbm_amd.VectorQuantizerEMA(K, D, 0.25, 0.9, balance_weight=weight, balance_temperature=T)
+        q.embedding.weight.data.normal_(generator=gen(2))
+        q.ema_w.data.copy_(q.embedding.weight.data)
+        q.ema_cluster_size.data.fill_(1.0)
+        before = q.embedding.weight.detach().clone().double()
+        q = q.to(DEV).train()
+        xd = x.to(DEV).requires_grad_()
+        loss, _, _, idx = q(xd)
+        loss.backward()
+        results[weight] = (loss.detach(), xd.grad, idx, q.embedding.weight.detach().clone(), q.ema_w.clone())
+    l0, g0, i0, w0, m0 = results[0.0]
+    l1, g1, i1, w1, m1 = results[wgt]
+    assert torch.equal(i0, i1) and torch.equal(w0, w1) and torch.equal(m0, m1)
+    assert not torch.equal(w1.cpu().double(), before)
+    xr = x.double().reshape(N, D).requires_grad_()
+    p = torch.softmax((2 * xr @ before.t() - (before * before).sum(1)) / T, 1).mean(0)
+    f = torch.bincount(i1.cpu().reshape(-1), minlength=K).double() / N
+    term = wgt * K * (f * p).sum()
+    (want,) = torch.autograd.grad(term, xr)
+    # scores up to some 100 err by 24 U of that, probabilities and gradients relatively as much: 2e-4; the differences of two fp32 results
+    assert abs(float(l1 - l0) - float(term.detach())) <= 2e-4 * float(term.detach()) + 4 * U * abs(float(l1))
+    err = (g1 - g0).cpu().double().reshape(N, D) - want
+    assert float(err.abs().max()) <= 2e-4 * float(want.abs().max()) + 4 * U * float(g1.abs().max())
+    # not in eval mode
+    q.eval()
+    with torch.no_grad():
+        a = q(x.to(DEV))[0]
+        q.balance_weight = 0.0
+        assert torch.equal(a, q(x.to(DEV))[0])
