@@ -393,7 +393,7 @@ int lbm_perplexity_u64(const unsigned long long* hist, float* out, int32_t K, lb
  *   temperature positive and finite.
  * lbm_code_logits_grad_f32: gradients of a loss with dL/dlogits = g [N, K] (row stride ldg): dx [N, D] = (2 / temperature) g E and
  *   de [K, D] = (2 / temperature) (g^T x - diag(column sums of g) E); norm_grad = 0 leaves the second term out (e_sqnorm was given as a
- *   constant).  Either output may be NULL.  workspace (only for de): lbm_code_logits_grad_workspace_bytes bytes, 16-byte aligned.
+ *   constant).  Either output may be NULL.  workspace: lbm_code_logits_grad_workspace_bytes bytes, 16-byte aligned.
  *   Partial sums are joined in a fixed order: the same input gives the same bits. */
 #define LBM_F32 0
 #define LBM_F16 1

@@ -42,13 +42,11 @@ class _CodeLogits(torch.autograd.Function):
             g = g.contiguous()
         lib = _lib.load()
         dx = torch.empty((N, D), dtype=torch.float32, device=x.device) if need_x else None
-        de = ws = None
-        if need_e:
-            de = torch.empty((K, D), dtype=torch.float32, device=x.device)
-            ws = torch.empty((lib.lbm_code_logits_grad_workspace_bytes(N, D, K),), dtype=torch.uint8, device=x.device)
+        de = torch.empty((K, D), dtype=torch.float32, device=x.device) if need_e else None
+        ws = torch.empty((lib.lbm_code_logits_grad_workspace_bytes(N, D, K),), dtype=torch.uint8, device=x.device)
         _lib.check(lib.lbm_code_logits_grad_f32(_lib.ptr(g), g.stride(0) if N > 1 else K, x.data_ptr(), x.stride(0) if N > 1 else D,
                                                 codebook.data_ptr(), dx.data_ptr() if need_x else None, de.data_ptr() if need_e else None,
-                                                int(ctx.norm_grad), ws.data_ptr() if need_e else None, N, D, K, ctx.temperature,
+                                                int(ctx.norm_grad), ws.data_ptr(), N, D, K, ctx.temperature,
                                                 _lib.stream_ptr()), "lbm_code_logits_grad_f32")
         return dx, de, None, None
 

@@ -153,7 +153,7 @@ struct Tiles {
 
 // out[m, n] over the contraction; EPI_SCORES: out = (2 acc - e_n) * scale, e_n = sqnorm[n] or, where that is NULL, the square sum of B's
 // row n taken from its staged values; EPI_SCALE: out = acc * scale; EPI_PARTIAL: piece z's sums to out[z][m][n] and A's row sums over
-// the piece to rowsum[z][m].
+// the piece to rowsum[z][m] (NULL: not wanted).
 template <int TM, int TN, int AM, int BM, int EPI>
 __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand b, float* __restrict__ out, int64_t ldo, int64_t depth,
                                                               Tiles t, float scale, const float* __restrict__ sqnorm,
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
         float* o = out;
         if constexpr (EPI == EPI_PARTIAL) {
             o += (int64_t)z_now * a.rows * ldo;
-            if (n0_now == 0 && wn == 0) {
+            if (rowsum != nullptr && n0_now == 0 && wn == 0) {
 #pragma unroll
                 for (int x = 0; x < MI; ++x) {
                     const float s = asum[x] + __shfl_xor(asum[x], 32, 64);
@@ -328,13 +328,15 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
     }
 }
 
-// de[k, d] = scale * (sum_z part[z][k][d] - (sum_z rowsum[z][k]) * e[k][d]); pieces in order, eight loads on their way at a time
+// out[m, d] = scale * (sum_z part[z][m][d] - (sum_z rowsum[z][m]) * e[m][d]); NORM = false: without the second term.  Pieces in order, eight
+// loads on their way at a time.
+template <bool NORM>
 __global__ __launch_bounds__(256) void code_grad_join_kernel(const float* __restrict__ part, const float* __restrict__ rowsum,
-                                                             const float* __restrict__ codebook, float* __restrict__ de, int splits,
-                                                             int64_t K, int64_t D, float scale, int with_norm) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = K * D;
+                                                             const float* __restrict__ codebook, float* __restrict__ out, int splits,
+                                                             int64_t M, int64_t D, float scale) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = M * D;
     if (i >= n) return;
-    const int64_t k = i / D;
+    const int64_t m = NORM ? i / D : 0;
     double s = 0.0, c = 0.0;
     for (int z0 = 0; z0 < splits; z0 += 8) {
         float p[8], r[8];
@@ -342,7 +344,7 @@ __global__ __launch_bounds__(256) void code_grad_join_kernel(const float* __rest
         for (int u = 0; u < 8; ++u) {
             const int z = z0 + u < splits ? z0 + u : splits - 1;
             p[u] = part[z * n + i];
-            r[u] = rowsum[z * K + k];
+            r[u] = NORM ? rowsum[z * M + m] : 0.f;
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
@@ -350,8 +352,17 @@ __global__ __launch_bounds__(256) void code_grad_join_kernel(const float* __rest
             c += z0 + u < splits ? (double)r[u] : 0.0;
         }
     }
-    if (with_norm) s -= c * (double)codebook[i];
-    de[i] = (float)(s * (double)scale);
+    if (NORM) s -= c * (double)codebook[i];
+    out[i] = (float)(s * (double)scale);
+}
+
+template <bool NORM>
+int launch_join(const char* what, const float* part, const float* rowsum, const float* codebook, float* out, int splits, int64_t M, int64_t D,
+                float scale, hipStream_t st) {
+    const int64_t blocks = (M * D + 255) / 256;
+    if (blocks > 0x7fffffffLL) return lbm::fail(LBM_EUNSUPPORTED, "%s: gradient too large", what);
+    hipLaunchKernelGGL((code_grad_join_kernel<NORM>), dim3((unsigned)blocks), dim3(256), 0, st, part, rowsum, codebook, out, splits, M, D, scale);
+    return lbm::check_launch(what);
 }
 
 bool aligned16(const float* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
@@ -384,21 +395,28 @@ int launch_mm(const char* what, const Operand& a, const Operand& b, float* out, 
     return launch_tiles<64, 64, AM, BM, EPI>(what, a, b, out, ldo, depth, splits, piece, scale, sqnorm, rowsum, st);
 }
 
-constexpr int64_t kMaxPiece = 32768;   // rows of one fp32 accumulator chain in the codebook's gradient; pieces are joined in 64 bits
-
-// pieces of the N rows: enough tiles for two rounds of the chip, at least 128 rows each
-void plan_split(int64_t N, int32_t D, int32_t K, int* splits, int64_t* piece) {
-    const int64_t tiles = (((int64_t)K + 127) / 128) * (((int64_t)D + 127) / 128);
-    int64_t s = (512 + tiles - 1) / tiles;
-    if (s > (N + 127) / 128) s = (N + 127) / 128;
-    if (s < (N + kMaxPiece - 1) / kMaxPiece) s = (N + kMaxPiece - 1) / kMaxPiece;
-    if (s < 1) s = 1;
-    int64_t p = (N + s - 1) / s;
-    p = (p + kBK - 1) / kBK * kBK;
-    if (p < kBK) p = kBK;
-    *piece = p;
-    *splits = (int)((N + p - 1) / p);
-    if (*splits < 1) *splits = 1;
+// A contraction in pieces whose sums are joined in 64 bits: how many, and the steps of each (a multiple of 32).
+// tiles: of the output; a contraction is cut where they leave CUs idle, into pieces of `least` steps at least, and where it is longer than
+// `most`, the longest fp32 chain.
+struct Split {
+    int n;
+    int64_t piece;
+};
+Split split_steps(int64_t tiles, int64_t depth, int64_t least, int64_t most) {
+    int64_t n = 512 / (tiles > 0 ? tiles : 1);
+    if (n > depth / least) n = depth / least;
+    if (n < (depth + most - 1) / most) n = (depth + most - 1) / most;
+    if (n < 1) n = 1;
+    const int64_t piece = ((depth + n - 1) / n + kBK - 1) / kBK * kBK;
+    return {(int)((depth + piece - 1) / piece), piece};
+}
+// the codebook's gradient sums over the N rows, the rows' over the K codes.  (The latter is cut only where few rows make few tiles: the
+// pieces cost a write and a read of the gradient each.)
+Split split_rows(int64_t N, int32_t D, int32_t K) {
+    return split_steps((((int64_t)K + 127) / 128) * (((int64_t)D + 127) / 128), N, 128, 32768);
+}
+Split split_codes(int64_t N, int32_t D, int32_t K) {
+    return split_steps(((N + 63) / 64) * (((int64_t)D + 127) / 128), K, 256, 1 << 30);
 }
 
 }  // namespace
@@ -436,10 +454,11 @@ extern "C" int lbm_code_logits_f32(const float* x, int64_t ldx, int32_t layout, 
 
 extern "C" size_t lbm_code_logits_grad_workspace_bytes(int64_t N, int32_t D, int32_t K) {
     if (N < 0 || D < 1 || K < 1) return 0;
-    int splits;
-    int64_t piece;
-    plan_split(N, D, K, &splits, &piece);
-    return (size_t)splits * (size_t)K * (size_t)(D + 1) * sizeof(float);
+    if (N == 0) return 16;
+    const Split rows = split_rows(N, D, K), codes = split_codes(N, D, K);
+    const size_t for_e = (size_t)rows.n * (size_t)K * (size_t)(D + 1) * sizeof(float);
+    const size_t for_x = codes.n > 1 ? (size_t)codes.n * (size_t)N * (size_t)D * sizeof(float) : 0;
+    return for_e > for_x ? for_e : for_x;
 }
 
 extern "C" int lbm_code_logits_grad_f32(const float* g, int64_t ldg, const float* x, int64_t ldx, const float* codebook, float* dx_or_null,
@@ -450,37 +469,39 @@ extern "C" int lbm_code_logits_grad_f32(const float* g, int64_t ldg, const float
     LBM_REQUIRE(temperature > 0.0 && temperature < INFINITY, LBM_EINVAL, "%s: temperature must be positive and finite", what);
     LBM_REQUIRE(codebook && (N == 0 || g), LBM_EINVAL, "%s: NULL pointer", what);
     LBM_REQUIRE(N == 0 || ldg >= K, LBM_EINVAL, "%s: ldg (%lld) < K (%d)", what, (long long)ldg, K);
-    LBM_REQUIRE(de_or_null == nullptr || ((N == 0 || x) && workspace), LBM_EINVAL, "%s: the codebook's gradient needs x and a workspace", what);
-    LBM_REQUIRE(de_or_null == nullptr || N == 0 || ldx >= D, LBM_EINVAL, "%s: ldx (%lld) < D (%d)", what, (long long)ldx, D);
-    LBM_REQUIRE(((uintptr_t)workspace & 15) == 0, LBM_EINVAL, "%s: workspace must be 16-byte aligned", what);
+    if (dx_or_null == nullptr && de_or_null == nullptr) return LBM_OK;
+    LBM_REQUIRE(workspace != nullptr && ((uintptr_t)workspace & 15) == 0, LBM_EINVAL, "%s: needs a 16-byte aligned workspace", what);
+    LBM_REQUIRE(de_or_null == nullptr || N == 0 || (x && ldx >= D), LBM_EINVAL, "%s: the codebook's gradient needs x with ldx >= D (%d)", what, D);
     hipStream_t st = lbm::as_stream(stream);
     const float scale = (float)(2.0 / temperature);
+    float* part = static_cast<float*>(workspace);
+    int rc = LBM_OK;
     if (dx_or_null != nullptr && N > 0) {
         const Operand a{g, ldg, 0, 0, N}, b{codebook, D, 0, 0, D};
-        const int rc = aligned16(g, ldg) && aligned16(codebook, D)
-                           ? launch_mm<KCV, MCV, EPI_SCALE>(what, a, b, dx_or_null, D, K, 1, K, scale, nullptr, nullptr, st)
-                           : launch_mm<KC, MC, EPI_SCALE>(what, a, b, dx_or_null, D, K, 1, K, scale, nullptr, nullptr, st);
+        const bool wide_ab = aligned16(g, ldg) && aligned16(codebook, D);
+        const Split sp = split_codes(N, D, K);
+        if (sp.n == 1) {
+            rc = wide_ab ? launch_mm<KCV, MCV, EPI_SCALE>(what, a, b, dx_or_null, D, K, 1, K, scale, nullptr, nullptr, st)
+                         : launch_mm<KC, MC, EPI_SCALE>(what, a, b, dx_or_null, D, K, 1, K, scale, nullptr, nullptr, st);
+        } else {
+            rc = wide_ab ? launch_mm<KCV, MCV, EPI_PARTIAL>(what, a, b, part, D, K, sp.n, sp.piece, 1.f, nullptr, nullptr, st)
+                         : launch_mm<KC, MC, EPI_PARTIAL>(what, a, b, part, D, K, sp.n, sp.piece, 1.f, nullptr, nullptr, st);
+            if (rc == LBM_OK) rc = launch_join<false>(what, part, nullptr, codebook, dx_or_null, sp.n, N, D, scale, st);
+        }
+    }
+    if (rc != LBM_OK || de_or_null == nullptr) return rc;
+    Split sp{0, kBK};
+    float* rowsum = nullptr;
+    if (N > 0) {
+        sp = split_rows(N, D, K);
+        rowsum = part + (int64_t)sp.n * K * D;
+        const Operand a{g, ldg, 0, 0, K}, b{x, ldx, 0, 0, D};
+        // four rows of an operand at a time: their number has to be a multiple of four too
+        rc = aligned16(g, ldg) && aligned16(x, ldx) && ((K | D) & 3) == 0
+                 ? launch_mm<MCV, MCV, EPI_PARTIAL>(what, a, b, part, D, N, sp.n, sp.piece, 1.f, nullptr, rowsum, st)
+                 : launch_mm<MC, MC, EPI_PARTIAL>(what, a, b, part, D, N, sp.n, sp.piece, 1.f, nullptr, rowsum, st);
         if (rc != LBM_OK) return rc;
     }
-    if (de_or_null != nullptr) {
-        int splits = 0;
-        int64_t piece = kBK;
-        float* part = static_cast<float*>(workspace);
-        float* rowsum = part;
-        if (N > 0) {
-            plan_split(N, D, K, &splits, &piece);
-            rowsum = part + (int64_t)splits * K * D;
-            const Operand a{g, ldg, 0, 0, K}, b{x, ldx, 0, 0, D};
-            // four rows of an operand at a time: their number has to be a multiple of four too
-            const int rc = aligned16(g, ldg) && aligned16(x, ldx) && ((K | D) & 3) == 0
-                               ? launch_mm<MCV, MCV, EPI_PARTIAL>(what, a, b, part, D, N, splits, piece, 1.f, nullptr, rowsum, st)
-                               : launch_mm<MC, MC, EPI_PARTIAL>(what, a, b, part, D, N, splits, piece, 1.f, nullptr, rowsum, st);
-            if (rc != LBM_OK) return rc;
-        }
-        const int64_t total = (int64_t)K * D;
-        hipLaunchKernelGGL(code_grad_join_kernel, dim3((unsigned)((total + 255) / 256)), dim3(256), 0, st, part, rowsum, codebook, de_or_null,
-                           splits, K, D, scale, norm_grad);
-        return lbm::check_launch(what);
-    }
-    return LBM_OK;
+    return norm_grad ? launch_join<true>(what, part, rowsum, codebook, de_or_null, sp.n, K, D, scale, st)
+                     : launch_join<false>(what, part, rowsum, codebook, de_or_null, sp.n, K, D, scale, st);
 }

@@ -35,7 +35,7 @@ def _grad(g=P, ldg=16, x=P, ldx=8, cb=P, dx=P, de=P, norm=1, ws=P, N=4, D=8, K=1
 
 
 @pytest.mark.parametrize("kw", [dict(N=-1), dict(D=0), dict(K=0), dict(T=0.0), dict(T=math.nan), dict(g=None), dict(cb=None), dict(ldg=15),
-                                dict(x=None), dict(ws=None), dict(ldx=7), dict(ws=P + 8)])
+                                dict(x=None), dict(ws=None), dict(ldx=7), dict(ws=P + 8), dict(de=None, ws=None)])
 def test_logits_grad_entry_refuses(kw):
     assert _grad(**kw) == EINVAL and "lbm_code_logits_grad_f32" in _err()
 

@@ -36,7 +36,7 @@ def logits_tol(x, e, T, ee=None):
 
 
 @pytest.mark.parametrize("N,D,K", [(1, 1, 1), (1, 256, 512), (2, 3, 5), (63, 8, 65), (64, 32, 64), (129, 33, 127), (375, 256, 413), (1000, 100, 70),
-                                   (4100, 256, 1030), (5, 257, 8192)])
+                                   (4100, 256, 1030), (5, 257, 8192), (40, 64, 7001), (1, 256, 8192)])
 @pytest.mark.parametrize("T", [1.0, 0.07])
 def test_logits_and_gradients(N, D, K, T):
     g = gen(N * 7 + D * 3 + K)
