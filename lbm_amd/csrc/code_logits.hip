@@ -410,13 +410,13 @@ Split split_steps(int64_t tiles, int64_t depth, int64_t least, int64_t most) {
     const int64_t piece = ((depth + n - 1) / n + kBK - 1) / kBK * kBK;
     return {(int)((depth + piece - 1) / piece), piece};
 }
-// the codebook's gradient sums over the N rows, the rows' over the K codes.  (The latter is cut only where few rows make few tiles: the
-// pieces cost a write and a read of the gradient each.)
+// the codebook's gradient sums over the N rows, the rows' over the K codes.  (The latter is cut where few rows make few tiles; the pieces cost
+// a write and a read of the gradient each.)
 Split split_rows(int64_t N, int32_t D, int32_t K) {
     return split_steps((((int64_t)K + 127) / 128) * (((int64_t)D + 127) / 128), N, 128, 32768);
 }
 Split split_codes(int64_t N, int32_t D, int32_t K) {
-    return split_steps(((N + 63) / 64) * (((int64_t)D + 127) / 128), K, 256, 1 << 30);
+    return split_steps(((N + 63) / 64) * (((int64_t)D + 127) / 128), K, 256, 4096);
 }
 
 }  // namespace
