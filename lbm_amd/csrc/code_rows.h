@@ -32,22 +32,19 @@ struct alignas(4 * sizeof(T)) Quad {
     T v[4];
 };
 
-// v[] = the row's scores of thread t, -inf past column K.  vec: four scores in one access (aligned base and row stride, K % 4 == 0).
-template <typename T, int V, int W>
-__device__ __forceinline__ void load_row(const T* __restrict__ row, int K, int t, int vec, float* v) {
+// v[] = the row's scores of thread t, -inf past column K.  VEC: four scores in one access (aligned base and row stride, K % 4 == 0).
+template <typename T, int V, int W, bool VEC>
+__device__ __forceinline__ void load_row(const T* __restrict__ row, int K, int t, float* v) {
 #pragma unroll
     for (int c = 0; c < V / 4; ++c) {
         const int col = (c * 64 * W + t) * 4;
-        if (vec) {
+        if constexpr (VEC) {
             Quad<T> q;
-            if (col < K) {
-                q = *reinterpret_cast<const Quad<T>*>(row + col);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[4 * c + i] = score_to_f32<T>(q.v[i]);
-            } else {
+            for (int i = 0; i < 4; ++i) q.v[i] = score_from_f32<T>(-INFINITY);
+            if (col < K) q = *reinterpret_cast<const Quad<T>*>(row + col);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[4 * c + i] = -INFINITY;
-            }
+            for (int i = 0; i < 4; ++i) v[4 * c + i] = score_to_f32<T>(q.v[i]);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[4 * c + i] = col + i < K ? score_to_f32<T>(row[col + i]) : -INFINITY;

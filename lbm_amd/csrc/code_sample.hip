@@ -365,14 +365,14 @@ __device__ __forceinline__ int settle(Row<V>& R, const Setting& s, float lo, flo
 }
 
 // K <= 64 V: the whole row in registers
-template <typename T, int V>
-__global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ scores, int64_t lds, int vec, const float* __restrict__ u,
+template <typename T, int V, bool VEC>
+__global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ scores, int64_t lds, const float* __restrict__ u,
                                                           Params par, const uint8_t* __restrict__ allowed, int64_t allowed_ld,
                                                           int64_t* __restrict__ out, int64_t N, int K) {
     const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= N) return;                // a whole wave
     Row<V> R;
-    lbm::load_row<T, V, 1>(scores + row * lds, K, R.lane(), vec, R.v);
+    lbm::load_row<T, V, 1, VEC>(scores + row * lds, K, R.lane(), R.v);
     if (allowed != nullptr) {
         const uint8_t* a = allowed + row * allowed_ld;
 #pragma unroll
@@ -413,15 +413,35 @@ constexpr int kReg = 512, kCand = 1536;
 
 // passes over scores of a row, in memory or taken into LDS
 template <typename S>
-struct Passes {
+struct Passes {       // S::request loads four scores that are in range, S::convert makes floats of them, S::four is both with the row's end
     static __device__ __forceinline__ int lane() { return threadIdx.x & 63; }
     __device__ __forceinline__ const S& self() const { return *static_cast<const S*>(this); }
 
-    // f(four scores, slot of the first) in index order across calls
+    // f(four scores, slot of the first) in index order across calls; U chunks' loads are on their way at a time
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
-#pragma unroll 4
-        for (int c = 0; c < self().n; c += 256) {
+        each_<false, 4>(f);
+    }
+    template <typename F>
+    __device__ __forceinline__ void each_raw(F f) const {
+        each_<true, 8>(f);
+    }
+    template <bool RAW, int U, typename F>
+    __device__ __forceinline__ void each_(F f) const {
+        int c = 0;
+        for (; c + U * 256 <= self().n; c += U * 256) {
+            typename S::Four q[U];
+#pragma unroll
+            for (int i = 0; i < U; ++i) q[i] = self().request(c + i * 256 + lane() * 4);
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                float v[4];
+                if constexpr (RAW) self().convert_raw(q[i], c + i * 256 + lane() * 4, v);
+                else self().convert(q[i], c + i * 256 + lane() * 4, v);
+                f(v, c + i * 256 + lane() * 4);
+            }
+        }
+        for (; c < self().n; c += 256) {
             float q[4];
             self().four(c + lane() * 4, q);
             f(q, c + lane() * 4);
@@ -488,38 +508,77 @@ struct Passes {
     }
 };
 
-template <typename T>
-struct Memory : Passes<Memory<T>> {
+// VEC: four scores in one access (aligned row, n % 4 == 0); MASK: codes that may not be drawn.  (Both at compile time: a branch round a load
+// makes the compiler wait for it there, and one access was on its way at a time.)
+template <typename T, bool VEC, bool MASK>
+struct Memory : Passes<Memory<T, VEC, MASK>> {
     const T* row;
     const uint8_t* allowed;
-    int n, vec;
+    int n;
 
     __device__ __forceinline__ float one(int col) const {
         const float f = lbm::score_to_f32<T>(row[col]) + 0.f;
-        return f != f || (allowed != nullptr && allowed[col] == 0) ? -INFINITY : f;
+        return f != f || (MASK && allowed[col] == 0) ? -INFINITY : f;
     }
-    __device__ __forceinline__ void four(int col, float* f) const {       // -inf past the row's end
-        if (vec && col < n) {
-            const lbm::Quad<T> q = *reinterpret_cast<const lbm::Quad<T>*>(row + col);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = lbm::score_to_f32<T>(q.v[i]) + 0.f;
+    using Four = lbm::Quad<T>;
+    __device__ __forceinline__ Four request(int col) const {
+        Four q;
+        if constexpr (VEC) {
+            q = *reinterpret_cast<const Four*>(row + col);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = col + i < n ? lbm::score_to_f32<T>(row[col + i]) + 0.f : -INFINITY;
+            for (int i = 0; i < 4; ++i) q.v[i] = row[col + i];
         }
-        if (allowed != nullptr) {
+        return q;
+    }
+    __device__ __forceinline__ void convert(const Four& q, int col, float* f) const {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (col + i < n && allowed[col + i] == 0) f[i] = -INFINITY;
+        for (int i = 0; i < 4; ++i) {
+            f[i] = lbm::score_to_f32<T>(q.v[i]) + 0.f;
+            f[i] = f[i] != f[i] ? -INFINITY : f[i];
         }
+        mask(col, f);
+    }
+    // where NaN and the sign of 0 do not matter: maxima, comparisons with a score, weights
+    __device__ __forceinline__ void convert_raw(const Four& q, int col, float* f) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = f[i] != f[i] ? -INFINITY : f[i];
+        for (int i = 0; i < 4; ++i) f[i] = lbm::score_to_f32<T>(q.v[i]);
+        mask(col, f);
+    }
+    __device__ __forceinline__ void mask(int col, float* f) const {
+        if constexpr (MASK) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = allowed[col + i] == 0 ? -INFINITY : f[i];
+        }
+    }
+    __device__ __forceinline__ void four(int col, float* f) const {       // -inf past the row's end
+        if constexpr (VEC) {
+            if (col < n) {
+                convert(request(col), col, f);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[i] = -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = col + i < n ? one(col + i) : -INFINITY;
+        }
     }
 };
 
 struct Taken : Passes<Taken> {
     const float* val;     // LDS
     int n;
+    struct Four { float v[4]; };
+    __device__ __forceinline__ Four request(int at) const {
+        const float4 q = *reinterpret_cast<const float4*>(val + at);
+        return {q.x, q.y, q.z, q.w};
+    }
+    __device__ __forceinline__ void convert(const Four& q, int, float* f) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = q.v[i];
+    }
+    __device__ __forceinline__ void convert_raw(const Four& q, int at, float* f) const { convert(q, at, f); }
     __device__ __forceinline__ void four(int at, float* f) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) f[i] = at + i < n ? val[at + i] : -INFINITY;
@@ -541,6 +600,7 @@ __device__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, i
     // what stays: scores above b and the first `keep` of those equal to it
     float b = -INFINITY;
     int keep = 0;
+    equal = 0;
     if (s.by_k) {
         b = R.template border<int>(lo, m, [](float) { return 1; }, [&](int c) { return c >= s.top_k; });
         R.counts(b, &above, &equal);
@@ -578,7 +638,45 @@ __device__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, i
             w[i] = in && w[i] >= lim ? w[i] : 0.0;
         }
     };
-    if (lim > 0.0) {
+    // Sums of 2048 scores at a time, which lead to the group the draw falls into; where the border cuts through equal scores their order
+    // counts and the row is walked from its start.
+    double base = 0.0;
+    int start = 0;
+    if (keep >= equal) {
+        const double least = lim;
+        auto group = [&](int g) {        // the lanes' sums of group g
+            double w = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = g * 2048 + i * 256 + R.lane() * 4;
+                float q[4];
+                R.four(c, q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const double x = weight(q[j]);
+                    w += q[j] >= b && x >= least ? x : 0.0;
+                }
+            }
+            return lbm::wave_total(w);
+        };
+        const int groups = (R.n + 2047) / 2048;
+        here = 0.0;
+        double mine = 0.0;               // lane g % 64 keeps group g's sum of the last 64
+        for (int g = 0; g < groups; ++g) {
+            const double w = group(g);
+            here += w;
+            if ((g & 63) == R.lane()) mine = w;
+        }
+        const double goal = s.u * here;
+        if (groups <= 64) {
+            for (int g = 0; g + 1 < groups; ++g) {
+                const double w = lbm::lane_value(mine, g);
+                if (base + w > goal) break;
+                base += w;
+                start = (g + 1) * 2048;
+            }
+        }
+    } else if (lim > 0.0) {
         double sum = 0.0;
         int seen = 0;
         R.each([&](const float* q, int) {
@@ -589,9 +687,8 @@ __device__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, i
         here = lbm::wave_total(sum);
     }
     const double goal = s.u * here;
-    double base = 0.0;
     int seen = 0, last = -1;
-    for (int c = 0; c < R.n; c += 256) {
+    for (int c = start; c < R.n; c += 256) {
         float q[4];
         double w[4];
         R.four(c + R.lane() * 4, q);
@@ -613,28 +710,27 @@ __device__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, i
 
 constexpr float kLowest = -3.402823466e+38f;
 
-template <typename T>
-__global__ __launch_bounds__(256) void code_sample_long_kernel(const T* __restrict__ scores, int64_t lds, int vec, const float* __restrict__ u,
+template <typename T, bool VEC, bool MASK>
+__global__ __launch_bounds__(256, 3) void code_sample_long_kernel(const T* __restrict__ scores, int64_t lds, const float* __restrict__ u,
                                                                Params par, const uint8_t* __restrict__ allowed, int64_t allowed_ld,
                                                                int64_t* __restrict__ out, int64_t N, int K) {
-    __shared__ float s_val[4][kCand];
-    __shared__ int s_col[4][kCand];
+    __shared__ __align__(16) float s_val[4][kCand];
+    __shared__ unsigned short s_col[4][kCand], s_four[4][kCand];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + wave;
     if (row >= N) return;                // a whole wave
-    Memory<T> S;
+    Memory<T, VEC, MASK> S;
     S.row = scores + row * lds;
-    S.allowed = allowed != nullptr ? allowed + row * allowed_ld : nullptr;
+    S.allowed = MASK ? allowed + row * allowed_ld : nullptr;
     S.n = K;
-    S.vec = vec;
     const Setting s = row_setting(par, u, row, K);
     float* val = s_val[wave];
-    int* col = s_col[wave];
+    unsigned short *col = s_col[wave], *four = s_four[wave];
     constexpr int V = kReg / 64;
     int hit = -2;                        // not answered yet
     float m = -INFINITY, lo = INFINITY;
     const bool greedy = !(s.temp > 0.0), p_alone = s.by_p && !s.by_k;
-    if (!greedy && (s.by_k ? s.top_k <= 1280 : s.by_p || s.min_p > 0.0)) {
+    if (!greedy && K <= 65536 && (s.by_k ? s.top_k <= 1280 : s.by_p || s.min_p > 0.0)) {
         Row<V> R;                        // samples: every (K / 512)-th score
         float t_lo = INFINITY, t_hi = -INFINITY;
 #pragma unroll
@@ -661,34 +757,49 @@ __global__ __launch_bounds__(256) void code_sample_long_kernel(const T* __restri
                     else break;
                 }
             }
-            int n = 0;
+            // first the groups of four that hold a score >= t, by their number; then, of those alone, the scores themselves
+            int fours = 0;
             double sum = 0.0;
             m = -INFINITY;
-            S.each([&](const float* q, int c) {
-                int pre = 0, tot = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    m = fmaxf(m, q[i]);
-                    const unsigned long long b = __ballot(q[i] >= t);
-                    pre = __builtin_amdgcn_mbcnt_hi((unsigned)(b >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)b, pre));
-                    tot += __popcll(b);
-                }
+            S.each_raw([&](const float* q, int c) {
+                const float best = fmaxf(fmaxf(q[0], q[1]), fmaxf(q[2], q[3]));
+                m = fmaxf(m, best);
                 if (p_alone) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) sum += exp2_f64(((double)q[i] - (double)ref) * s.c);
                 }
-                if (tot != 0 && n + tot <= kCand) {
-                    int at = n + pre;
+                const unsigned long long b = __ballot(best >= t);
+                const int at = fours + __builtin_amdgcn_mbcnt_hi((unsigned)(b >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)b, 0));
+                if (best >= t && at < kCand) four[at] = (unsigned short)(c >> 2);
+                fours += __popcll(b);
+            });
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            int n = fours > kCand ? kCand + 1 : 0;
+            for (int f0 = 0; f0 < fours && n <= kCand; f0 += 64) {
+                float q[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                int c = 0;
+                if (f0 + lane < fours) {
+                    c = four[f0 + lane] * 4;
+                    S.four(c, q);
+                }
+                int pre = n, tot = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const unsigned long long b = __ballot(q[i] >= t);
+                    pre = __builtin_amdgcn_mbcnt_hi((unsigned)(b >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)b, pre));
+                    tot += __popcll(b);
+                }
+                if (n + tot <= kCand) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                         if (q[i] >= t) {
-                            val[at] = q[i];
-                            col[at] = c + i;
-                            ++at;
+                            val[pre] = q[i];
+                            col[pre] = (unsigned short)(c + i);
+                            ++pre;
                         }
                 }
                 n += tot;
-            });
+            }
             m = lbm::wave_best(m);
             if (m == -INFINITY) {
                 hit = -1;
@@ -696,7 +807,9 @@ __global__ __launch_bounds__(256) void code_sample_long_kernel(const T* __restri
             }
             if (m == INFINITY) break;
             int next = want;
-            if (n > kCand || (s.by_k && n < s.top_k && t > kLowest)) {
+            // (a list that outgrew the registers is worth another pass where a shorter one does)
+            const int room = tries == 0 && (!s.by_k || s.top_k <= 384) ? kReg : kCand;
+            if (n > room || (s.by_k && n < s.top_k && t > kLowest)) {
                 next = (int)fmin(fmax(1.f, (float)want * (float)aim / (float)(n > 0 ? n : 1)), (float)kReg);
             } else {
                 double total = -1.0;
@@ -740,6 +853,19 @@ __global__ __launch_bounds__(256) void code_sample_long_kernel(const T* __restri
             want = next;
         }
     }
+    if (hit == -2 && greedy) {
+        int at = 0x7fffffff;             // each lane's first best score
+        m = -INFINITY;
+        S.each([&](const float* q, int c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                at = q[i] > m ? c + i : at;
+                m = fmaxf(m, q[i]);
+            }
+        });
+        const float best = lbm::wave_best(m);
+        hit = best == -INFINITY ? -1 : lbm::wave_first(m == best ? at : 0x7fffffff);
+    }
     if (hit == -2) {
         m = -INFINITY;
         lo = INFINITY;
@@ -752,9 +878,7 @@ __global__ __launch_bounds__(256) void code_sample_long_kernel(const T* __restri
         });
         m = lbm::wave_best(m);
         lo = -lbm::wave_best(-lo);
-        if (m == -INFINITY) hit = -1;
-        else if (greedy) hit = S.nth_equal(m, 0);
-        else hit = draw_by_passes(S, s, lo, m, K, -1.0);
+        hit = m == -INFINITY ? -1 : draw_by_passes(S, s, lo, m, K, -1.0);
     }
     if (lane == 0) out[row] = hit;
 }
@@ -763,13 +887,14 @@ template <typename T>
 int run_sample(const void* scores, int64_t lds, const float* u, const Params& par, const uint8_t* allowed, int64_t allowed_ld, int64_t* out,
                int64_t N, int K, hipStream_t st) {
     const T* s = static_cast<const T*>(scores);
-    const int vec = ((uintptr_t)scores % (4 * sizeof(T))) == 0 && (lds & 3) == 0 && (K & 3) == 0 ? 1 : 0;
+    const bool vec = ((uintptr_t)scores % (4 * sizeof(T))) == 0 && (lds & 3) == 0 && (K & 3) == 0;
     const dim3 grid((unsigned)((N + 3) / 4)), block(256);
-#define LBM_SAMPLE(kernel) hipLaunchKernelGGL((kernel), grid, block, 0, st, s, lds, vec, u, par, allowed, allowed_ld, out, N, K)
-    if (K <= 256) LBM_SAMPLE((code_sample_kernel<T, 4>));
-    else if (K <= 512) LBM_SAMPLE((code_sample_kernel<T, 8>));
-    else if (K <= 1024) LBM_SAMPLE((code_sample_kernel<T, 16>));
-    else LBM_SAMPLE((code_sample_long_kernel<T>));
+#define LBM_SAMPLE(kernel) hipLaunchKernelGGL((kernel), grid, block, 0, st, s, lds, u, par, allowed, allowed_ld, out, N, K)
+    if (K <= 256) LBM_SAMPLE((vec ? code_sample_kernel<T, 4, true> : code_sample_kernel<T, 4, false>));
+    else if (K <= 512) LBM_SAMPLE((vec ? code_sample_kernel<T, 8, true> : code_sample_kernel<T, 8, false>));
+    else if (K <= 1024) LBM_SAMPLE((vec ? code_sample_kernel<T, 16, true> : code_sample_kernel<T, 16, false>));
+    else if (allowed == nullptr) LBM_SAMPLE((vec ? code_sample_long_kernel<T, true, false> : code_sample_long_kernel<T, false, false>));
+    else LBM_SAMPLE((vec ? code_sample_long_kernel<T, true, true> : code_sample_long_kernel<T, false, true>));
 #undef LBM_SAMPLE
     return lbm::check_launch("lbm_code_sample");
 }
