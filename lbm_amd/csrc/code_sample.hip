@@ -466,10 +466,11 @@ struct Passes {       // S::request loads four scores that are in range, S::conv
         return lbm::wave_total(s);
     }
     // the highest score x with reached(scores >= x): one of those in [lo, hi], reached(lo).  add(q) is summed over the scores >= the trial.
+    // The first trial is hi itself where `top` (a distribution may have one code).
     template <typename A, typename Add, typename Reached>
-    __device__ __forceinline__ float border(float lo, float hi, Add add, Reached reached) const {
+    __device__ __forceinline__ float border(float lo, float hi, bool top, Add add, Reached reached) const {
         for (int it = 0; it < kSteps && lo < hi; ++it) {
-            const float mid = it == 0 ? hi : trial(it, lo, hi);
+            const float mid = it == 0 && top ? hi : trial(it, lo, hi);
             A sum = A(0);
             float from = -INFINITY, below = -INFINITY;            // from: of the negatives
             each([&](const float* q, int) {
@@ -485,6 +486,25 @@ struct Passes {       // S::request loads four scores that are in range, S::conv
             else hi = lbm::wave_best(below);
         }
         return lo;
+    }
+    // weight above x, number of scores equal to x, the nearest scores above and below
+    __device__ void around(float x, float m, double c, double* above, int* equal, float* up, float* down) const {
+        double s = 0.0;
+        int e = 0;
+        float u = -INFINITY, d = -INFINITY;                       // u: of the negatives
+        each([&](const float* q, int) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s += q[i] > x ? exp2_f64(((double)q[i] - (double)m) * c) : 0.0;
+                e += q[i] == x ? 1 : 0;
+                u = fmaxf(u, q[i] > x ? -q[i] : -INFINITY);
+                d = fmaxf(d, q[i] < x ? q[i] : -INFINITY);
+            }
+        });
+        *above = lbm::wave_total(s);
+        *equal = lbm::wave_total(e);
+        *up = -lbm::wave_best(u);
+        *down = lbm::wave_best(d);
     }
     // slot of the j-th (from 0) score equal to x; -1: there are fewer
     __device__ int nth_equal(float x, int j) const {
@@ -585,9 +605,9 @@ struct Taken : Passes<Taken> {
     }
 };
 
-// the draw by passes; lo, m: lowest and best score; total as for settle (-1 likewise)
+// the draw by passes; lo, m: lowest and best score; total as for settle (-1 likewise); below: top-p's border is known to lie below this score
 template <typename S>
-__device__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, int K, double total) {
+__device__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, int K, double total, float below) {
     int above, equal;
     if (m == INFINITY) {                 // equal weights of 1
         R.counts(m, &above, &equal);
@@ -602,24 +622,54 @@ __device__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, i
     int keep = 0;
     equal = 0;
     if (s.by_k) {
-        b = R.template border<int>(lo, m, [](float) { return 1; }, [&](int c) { return c >= s.top_k; });
+        b = R.template border<int>(lo, m, false, [](float) { return 1; }, [&](int c) { return c >= s.top_k; });
         R.counts(b, &above, &equal);
         keep = s.top_k - above < equal ? s.top_k - above : equal;
     }
-    double here = R.weight_above(b, m, s.c) + (b == -INFINITY ? 0.0 : keep * weight(b));
+    double here = 0.0;
     if (s.by_p) {
+        here = R.weight_above(b, m, s.c) + (b == -INFINITY ? 0.0 : keep * weight(b));
         const double target = s.top_p * (total < 0.0 ? here : total);
         if (here < target) return -1;
         const float l = fmaxf(b == -INFINITY ? lo : b, top_p_floor(m, lo, s.temp, s.top_p, K));
-        const float x = R.template border<double>(l, m, weight, [&](double w) { return w >= target; });
+        const bool top = !(below < m);
+        const float h = top ? m : below;
+        // searched on fp32 sums, settled by 64-bit ones as in keep_top_p
+        const float cf = (float)s.c, goal = (float)target;
+        float x = l < h ? R.template border<float>(l, h, top, [&](float q) { return __builtin_amdgcn_exp2f((q - m) * cf); },
+                                                   [&](float w) { return w >= goal; })
+                        : l;
+        double over = 0.0;
+        bool settled = false;
+        for (int tries = 0; tries < 4 && !settled; ++tries) {
+            float up, down;
+            R.around(x, m, s.c, &over, &equal, &up, &down);
+            settled = true;
+            if (over >= target && x < m) {
+                x = up;
+                settled = false;
+            } else if (equal == 0 || over + equal * weight(x) < target) {
+                if (down > -INFINITY) {
+                    x = down;
+                    settled = false;
+                }
+            }
+        }
+        if (!settled) {
+            x = R.template border<double>(l, m, true, weight, [&](double w) { return w >= target; });
+            float up, down;
+            R.around(x, m, s.c, &over, &equal, &up, &down);
+        }
         if (x > b) {
             b = x;
-            R.counts(b, &above, &equal);
             keep = equal;
+        } else {                         // top-k's border, where `keep` of the equals stay
+            int above_b;
+            R.counts(b, &above_b, &equal);
+            over = R.weight_above(b, m, s.c);
         }
-        const double over = R.weight_above(b, m, s.c), wb = weight(b), n = ceil((target - over) / wb);
+        const double n = ceil((target - over) / weight(b));
         keep = n >= 1.0 ? (n < keep ? (int)n : keep) : 1;
-        here = over + keep * wb;
     }
     const double lim = s.min_p > 0.0 ? fmin(s.min_p, 1.0) : 0.0;
     // weights that stay, four at a time; `seen` counts the equals of b so far
@@ -676,7 +726,7 @@ __device__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, i
                 start = (g + 1) * 2048;
             }
         }
-    } else if (lim > 0.0) {
+    } else {
         double sum = 0.0;
         int seen = 0;
         R.each([&](const float* q, int) {
@@ -728,6 +778,7 @@ __global__ __launch_bounds__(256, 3) void code_sample_long_kernel(const T* __res
     unsigned short *col = s_col[wave], *four = s_four[wave];
     constexpr int V = kReg / 64;
     int hit = -2;                        // not answered yet
+    float below = INFINITY;              // top-p's border is known to lie below this score
     float m = -INFINITY, lo = INFINITY;
     const bool greedy = !(s.temp > 0.0), p_alone = s.by_p && !s.by_k;
     if (!greedy && K <= 65536 && (s.by_k ? s.top_k <= 1280 : s.by_p || s.min_p > 0.0)) {
@@ -838,7 +889,7 @@ __global__ __launch_bounds__(256, 3) void code_sample_long_kernel(const T* __res
                         Q.val = val;
                         Q.n = n;
                         for (int i = lane; i < n; i += 64) lo = fminf(lo, val[i]);
-                        at = draw_by_passes(Q, s, -lbm::wave_best(-lo), m, K, total);
+                        at = draw_by_passes(Q, s, -lbm::wave_best(-lo), m, K, total, INFINITY);
                     }
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 }
@@ -846,6 +897,7 @@ __global__ __launch_bounds__(256, 3) void code_sample_long_kernel(const T* __res
                     hit = col[at];
                     break;
                 }
+                if (p_alone && all) below = t;
                 aim = kCand * 3 / 4;     // the nucleus is larger
                 next = (int)fmax(1.f, (float)aim * kReg / (float)K);
             }
@@ -878,7 +930,7 @@ __global__ __launch_bounds__(256, 3) void code_sample_long_kernel(const T* __res
         });
         m = lbm::wave_best(m);
         lo = -lbm::wave_best(-lo);
-        hit = m == -INFINITY ? -1 : draw_by_passes(S, s, lo, m, K, -1.0);
+        hit = m == -INFINITY ? -1 : draw_by_passes(S, s, lo, m, K, -1.0, below);
     }
     if (lane == 0) out[row] = hit;
 }
