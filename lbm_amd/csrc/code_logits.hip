@@ -7,23 +7,31 @@
 // s is minus the squared distance over the temperature without its row constant |x_n|^2 / T, which softmax, argmax and every ordering
 // of a row ignore and whose size would only cost the differences their low bits.
 //
-// Bound: the fp32 matrix pipe (64 FLOP per cycle and SIMD) -- an output element costs 2 D FLOP for 4 bytes of store, 128 FLOP per byte at
-// D = 256 against the 20 FLOP per byte where the pipe and HBM balance.  That is also why the scores are stored at all: forming them a second
-// time for the gradient costs more than writing and reading them.
+// Products: every fp32 operand is cut into three bf16 pieces, each the nearest bf16 of what is left (the remainders are exact, the three
+// hold 24 bits and more), and a product keeps six terms of the nine, accumulated in fp32 on v_mfma_f32_32x32x16_bf16; the three left out lie
+// below 2^-26 of it.  That is as exact as a chain of fp32 products (7.5e-8 of the scores' size against 64 bits either way) at 16/6 of the fp32
+// matrix rate.  An infinity among the inputs makes NaN of what it enters (inf - inf in its remainder).
 //
-// Tile: 4 waves, each (TM/2) x (TN/2) outputs in 32 x 32 accumulators of v_mfma_f32_32x32x2_f32 (exact fmaf chains).  The contraction
-// runs 32 steps at a time: operands are requested into registers while the previous 32 steps' products run from LDS.  An operand that is
-// contiguous along the contraction sits in LDS as [row][32 + 4] and is read four steps at a time (ds_read_b128); one that is contiguous
-// along its rows (the codebook in dx, both operands in de, a channel-major x) sits as [step][rows + 2] and is read one step at a time, which
-// the 64-cycle MFMA hides.  Lane half h takes steps h*16 .. h*16 + 15 of both.
+// Bound: the matrix pipe and the power it draws; an output element costs 12 D FLOP of bf16 products for 4 bytes of store.  That is also why
+// the scores are stored at all: forming them a second time for the gradient costs more than writing and reading them.
+//
+// Tile: 4 waves, each (TM/2) x (TN/2) outputs in 32 x 32 accumulators.  The contraction runs 32 steps at a time: operands are requested into
+// registers while the products of the previous 32 steps run, cut into pieces and written to LDS as three planes [row][32 + 8] of bf16, which the
+// waves read eight steps at a time (ds_read_b128; the pitch of 80 bytes spreads rows over the banks).
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
 
 using f32x16 = __attribute__((ext_vector_type(16))) float;
+using f32x2 = __attribute__((ext_vector_type(2))) float;
+using b16x2 = __attribute__((ext_vector_type(2))) __bf16;
+using b16x8 = __attribute__((ext_vector_type(8))) __bf16;
 
 constexpr int kThreads = 256;
 constexpr int kBK = 32;
+constexpr int kPitch = 80;        // bytes of a row of one plane
 
 // operand contiguous along the contraction (KC) or along its rows (MC), read 4 bytes or (V) 16 bytes at a time
 enum { KC = 0, MC = 1, KCV = 2, MCV = 3 };
@@ -39,107 +47,129 @@ struct Operand {
     int64_t rows;
 };
 
+// N consecutive steps of one row -> their three pieces
+template <int N>
+__device__ __forceinline__ void cut(const float* v, unsigned (*p)[N / 2]) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+        f32x2 f = {v[2 * i], v[2 * i + 1]};
+#pragma unroll
+        for (int q = 0; q < 3; ++q) {
+            const unsigned w = __builtin_bit_cast(unsigned, __builtin_convertvector(f, b16x2));
+            p[q][i] = w;
+            f.x -= __uint_as_float(w << 16);
+            f.y -= __uint_as_float(w & 0xffff0000u);
+        }
+    }
+}
+
 // One operand's share of a tile: 32 contraction steps of T rows, in registers on the way from memory to LDS.  Rows past the operand's last
 // repeat it (what they give is not stored); steps past the end are zeros and come from load_tail only, so that load has no branch in it.
+//   K:    thread has steps 4 (t % 8) .. + 3 of rows t / 8 + 32 i
+//   MCV:  rows 4 (t / G) .. + 3 of steps U (t % G) .. + U - 1, U = T / 32: the eight (sixteen) threads of four rows write whole LDS rows
+//   MC:   row t % T of steps 4 (t / T) + 4 (256 / T) i .. + 3: the threads of a wave read neighbouring rows
 template <int T, int MODE>
 struct Stage {
     static constexpr bool K = along_k(MODE), WIDE = wide(MODE);
-    static constexpr int kPitch = K ? kBK + 4 : T + 4;
-    static constexpr int kFloats = K ? T * kPitch : kBK * kPitch;
-    static constexpr int kQuads = T * kBK / 4 / kThreads;
-    // K: thread has steps 4 (t % 8) .. + 3 of row t / 8 + 32 i.  else WIDE: rows 4 (t % (T / 4)) .. + 3 of step t / (T / 4) + .. i;
-    // not WIDE: row t % T of steps t / T + (kThreads / T) (4 i + u)
-    static constexpr int kPer = WIDE ? kThreads / (T / 4) : kThreads / T;
-    float v[kQuads][4];
-    const float* base[K ? kQuads : (WIDE ? 1 : 1)];
+    static constexpr int kPlane = T * kPitch, kBytes = 3 * kPlane;
+    static constexpr int Q = T / 32, U = T / 32, G = kBK / U;
+    float v[Q][4];                    // K, MC: [quad][step]; MCV: [step][row]
+    const float* base[K ? Q : 1];
     int64_t ld;
 
-    __device__ __forceinline__ static int kstep(int i, int u) {
-        return WIDE ? threadIdx.x / (T / 4) + kPer * i : threadIdx.x / T + kPer * (4 * i + u);
+    __device__ __forceinline__ static int step(int i, int u) {       // contraction step of v[i][u]
+        if constexpr (K) return (threadIdx.x & 7) * 4 + u;
+        else if constexpr (WIDE) return U * (threadIdx.x % G) + i;
+        else return 4 * (threadIdx.x / T) + 4 * (kThreads / T) * i + u;
+    }
+    __device__ __forceinline__ static int row(int i, int u) {        // tile row of v[i][u]
+        if constexpr (K) return (threadIdx.x >> 3) + 32 * i;
+        else if constexpr (WIDE) return 4 * (threadIdx.x / G) + u;
+        else return threadIdx.x % T;
     }
     __device__ __forceinline__ void init(const Operand& o, int64_t r0, int64_t k0) {
         ld = o.ld;
         if constexpr (K) {
 #pragma unroll
-            for (int i = 0; i < kQuads; ++i) {
-                const int64_t r = r0 + (threadIdx.x >> 3) + 32 * i;
-                base[i] = o.p + (r < o.rows ? r : o.rows - 1) * o.ld + (threadIdx.x & 7) * 4 + k0;
+            for (int i = 0; i < Q; ++i) {
+                const int64_t r = r0 + row(i, 0);
+                base[i] = o.p + (r < o.rows ? r : o.rows - 1) * o.ld + step(0, 0) + k0;
             }
         } else {
-            int64_t r = r0 + (WIDE ? threadIdx.x % (T / 4) * 4 : threadIdx.x % T);
+            int64_t r = r0 + row(0, 0);
             if (WIDE) r = r < o.rows ? r : 0;                      // rows % 4 == 0: four at a time are all in or all out
             else r = r < o.rows ? r : o.rows - 1;
-            base[0] = o.p + (o.S > 0 ? (r / o.S) * o.pitch + r % o.S : r) + (k0 + kstep(0, 0)) * o.ld;
+            base[0] = o.p + (o.S > 0 ? (r / o.S) * o.pitch + r % o.S : r) + (k0 + step(0, 0)) * o.ld;
         }
     }
     // 32 whole steps
     __device__ __forceinline__ void load() {
-        if constexpr (K) {
 #pragma unroll
-            for (int i = 0; i < kQuads; ++i) {
-                if constexpr (WIDE) {
-                    const float4 f = *reinterpret_cast<const float4*>(base[i]);
-                    v[i][0] = f.x; v[i][1] = f.y; v[i][2] = f.z; v[i][3] = f.w;
-                } else {
+        for (int i = 0; i < Q; ++i) {
+            if constexpr (WIDE) {
+                const float4 f = *reinterpret_cast<const float4*>(K ? base[K ? i : 0] : base[0] + (int64_t)i * ld);
+                v[i][0] = f.x; v[i][1] = f.y; v[i][2] = f.z; v[i][3] = f.w;
+            } else {
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) v[i][u] = base[i][u];
-                }
-                base[i] += kBK;
+                for (int u = 0; u < 4; ++u) v[i][u] = K ? base[K ? i : 0][u] : base[0][(int64_t)(4 * (kThreads / T) * i + u) * ld];
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kQuads; ++i) {
-                if constexpr (WIDE) {
-                    const float4 f = *reinterpret_cast<const float4*>(base[0] + (int64_t)(kPer * i) * ld);
-                    v[i][0] = f.x; v[i][1] = f.y; v[i][2] = f.z; v[i][3] = f.w;
-                } else {
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) v[i][u] = base[0][(int64_t)(kPer * (4 * i + u)) * ld];
-                }
-            }
-            base[0] += (int64_t)kBK * ld;
+            if (K) base[K ? i : 0] += kBK;
         }
+        if (!K) base[0] += (int64_t)kBK * ld;
     }
     // the last `left` < 32 steps
     __device__ __forceinline__ void load_tail(int left) {
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i)
+        for (int i = 0; i < Q; ++i)
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 float f = 0.f;
-                if constexpr (K) {
-                    if ((int)(threadIdx.x & 7) * 4 + u < left) f = base[i][u];
-                } else if constexpr (WIDE) {
-                    if (kstep(i, u) < left) f = base[0][(int64_t)(kPer * i) * ld + u];
-                } else {
-                    if (kstep(i, u) < left) f = base[0][(int64_t)(kPer * (4 * i + u)) * ld];
+                if (step(i, u) < left) {
+                    if constexpr (K) f = base[K ? i : 0][u];
+                    else if constexpr (WIDE) f = base[0][(int64_t)i * ld + u];
+                    else f = base[0][(int64_t)(4 * (kThreads / T) * i + u) * ld];
                 }
                 v[i][u] = f;
             }
     }
-    __device__ __forceinline__ void store(float* s) const {
+    // pieces to the three planes at s
+    __device__ __forceinline__ void store(char* s) const {
+        if constexpr (K || !WIDE) {
 #pragma unroll
-        for (int i = 0; i < kQuads; ++i) {
-            const float4 f = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
-            if constexpr (K) {
-                *reinterpret_cast<float4*>(s + ((threadIdx.x >> 3) + 32 * i) * kPitch + (threadIdx.x & 7) * 4) = f;
-            } else if constexpr (WIDE) {
-                *reinterpret_cast<float4*>(s + kstep(i, 0) * kPitch + threadIdx.x % (T / 4) * 4) = f;
-            } else {
+            for (int i = 0; i < Q; ++i) {
+                unsigned p[3][2];
+                cut<4>(v[i], p);
+                char* at = s + row(i, 0) * kPitch + step(i, 0) * 2;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) s[kstep(i, u) * kPitch + threadIdx.x % T] = v[i][u];
+                for (int q = 0; q < 3; ++q) *reinterpret_cast<uint2*>(at + q * kPlane) = make_uint2(p[q][0], p[q][1]);
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float f[U];
+#pragma unroll
+                for (int i = 0; i < U; ++i) f[i] = v[i][r];
+                unsigned p[3][U / 2];
+                cut<U>(f, p);
+                char* at = s + row(0, r) * kPitch + step(0, 0) * 2;
+#pragma unroll
+                for (int q = 0; q < 3; ++q) {
+                    if constexpr (U == 4) *reinterpret_cast<uint2*>(at + q * kPlane) = make_uint2(p[q][0], p[q][1]);
+                    else *reinterpret_cast<unsigned*>(at + q * kPlane) = p[q][0];
+                }
             }
         }
     }
-    // four steps (4q .. 4q+3 of lane half h) of row r
-    static __device__ __forceinline__ void frag(const float* s, int r, int h, int q, float* f) {
-        if constexpr (K) {
-            const float4 t = *reinterpret_cast<const float4*>(s + r * kPitch + h * 16 + 4 * q);
-            f[0] = t.x; f[1] = t.y; f[2] = t.z; f[3] = t.w;
-        } else {
+    // piece q of steps 16 g + 8 h .. + 7 of row r
+    static __device__ __forceinline__ b16x8 frag(const char* s, int r, int g, int h, int q) {
+        return *reinterpret_cast<const b16x8*>(s + q * kPlane + r * kPitch + g * 32 + h * 16);
+    }
+    // sums over the steps in registers, added to sum[4]: K: of row(i); MCV: of row(u); MC: of the one row, in sum[0]
+    __device__ __forceinline__ void add_steps(float* sum) const {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) f[u] = s[(h * 16 + 4 * q + u) * kPitch + r];
-        }
+        for (int i = 0; i < Q; ++i)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum[K ? i : (WIDE ? u : 0)] += v[i][u];
     }
 };
 
@@ -161,9 +191,10 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
     using SA = Stage<TM, AM>;
     using SB = Stage<TN, BM>;
     constexpr int MI = TM / 64, NI = TN / 64;
-    __shared__ __align__(16) float s_a[SA::kFloats];
-    __shared__ __align__(16) float s_b[SB::kFloats];
-    __shared__ float s_n[TN];
+    __shared__ __align__(16) char s_ab[SA::kBytes + SB::kBytes];
+    __shared__ float s_n[EPI == EPI_PARTIAL ? kThreads : TN];      // |e|^2 of the tile's codes; or the threads' row sums
+    char* s_a = s_ab;
+    char* s_b = s_ab + SA::kBytes;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int j = lane & 31, h = lane >> 5;
@@ -207,8 +238,8 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
             for (int y = 0; y < NI; ++y)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
-        float sq[SB::kQuads] = {};
-        float asum[MI] = {};
+        float sq[SB::Q] = {};
+        float asum[4] = {};
 
         auto put = [&] {
             // the waves that stage go before those that multiply: two workgroups share a SIMD, and the other one's products fill the
@@ -219,39 +250,40 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
             sb.store(s_b);
             if constexpr (EPI == EPI_SCORES) {
 #pragma unroll
-                for (int i = 0; i < SB::kQuads; ++i)
+                for (int i = 0; i < SB::Q; ++i)
 #pragma unroll
                     for (int u = 0; u < 4; ++u) sq[i] = fmaf(sb.v[i][u], sb.v[i][u], sq[i]);
             }
+            if constexpr (EPI == EPI_PARTIAL) sa.add_steps(asum);
             __syncthreads();
         };
         auto products = [&] {
-            // fragments of the next four steps are read while the products of these run
-            float fa[2][MI][4], fb[2][NI][4];
-            auto read = [&](int q, int to) {
+            // the pieces of the second 16 steps are read while the products of the first run
+            b16x8 fa[2][MI][3], fb[2][NI][3];
+            auto read = [&](int g) {
 #pragma unroll
-                for (int x = 0; x < MI; ++x) SA::frag(s_a, wm + 32 * x + j, h, q, fa[to][x]);
+                for (int q = 0; q < 3; ++q) {
 #pragma unroll
-                for (int y = 0; y < NI; ++y) SB::frag(s_b, wn + 32 * y + j, h, q, fb[to][y]);
+                    for (int x = 0; x < MI; ++x) fa[g][x][q] = SA::frag(s_a, wm + 32 * x + j, g, h, q);
+#pragma unroll
+                    for (int y = 0; y < NI; ++y) fb[g][y][q] = SB::frag(s_b, wn + 32 * y + j, g, h, q);
+                }
             };
-            read(0, 0);
+            read(0);
             __builtin_amdgcn_s_setprio(0);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int c = q & 1;
-                if (q < 3) read(q + 1, c ^ 1);
+            for (int g = 0; g < 2; ++g) {
+                if (g == 0) read(1);
                 __builtin_amdgcn_sched_barrier(0);
+                // the six products, small ones first
+                constexpr int qa[6] = {2, 1, 0, 1, 0, 0}, qb[6] = {0, 1, 2, 0, 1, 0};
 #pragma unroll
-                for (int u = 0; u < 4; ++u)
+                for (int t6 = 0; t6 < 6; ++t6)
 #pragma unroll
                     for (int x = 0; x < MI; ++x)
 #pragma unroll
                         for (int y = 0; y < NI; ++y)
-                            acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[c][x][u], fb[c][y][u], acc[x][y], 0, 0, 0);
-                if constexpr (EPI == EPI_PARTIAL) {
-#pragma unroll
-                    for (int x = 0; x < MI; ++x) asum[x] += (fa[c][x][0] + fa[c][x][1]) + (fa[c][x][2] + fa[c][x][3]);
-                }
+                            acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[g][x][qa[t6]], fb[g][y][qb[t6]], acc[x][y], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
@@ -283,7 +315,7 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
                 if (threadIdx.x < TN) s_n[threadIdx.x] = n0_now + threadIdx.x < b.rows ? sqnorm[n0_now + threadIdx.x] : 0.f;
             } else {
 #pragma unroll
-                for (int i = 0; i < SB::kQuads; ++i) {
+                for (int i = 0; i < SB::Q; ++i) {
                     float s = sq[i];   // the eight lanes that staged one row of B
                     s += __shfl_xor(s, 1, 64);
                     s += __shfl_xor(s, 2, 64);
@@ -296,12 +328,25 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
         float* o = out;
         if constexpr (EPI == EPI_PARTIAL) {
             o += (int64_t)z_now * a.rows * ldo;
-            if (rowsum != nullptr && n0_now == 0 && wn == 0) {
+            if (rowsum != nullptr && n0_now == 0) {
+                if constexpr (AM == MCV) {
 #pragma unroll
-                for (int x = 0; x < MI; ++x) {
-                    const float s = asum[x] + __shfl_xor(asum[x], 32, 64);
-                    const int64_t m = m0_now + wm + 32 * x + j;
-                    if (h == 0 && m < a.rows) rowsum[(int64_t)z_now * a.rows + m] = s;
+                    for (int u = 0; u < 4; ++u) {
+                        float v = asum[u];             // the threads of four rows are neighbours
+#pragma unroll
+                        for (int o = 1; o < SA::G; o <<= 1) v += __shfl_xor(v, o, 64);
+                        const int64_t m = m0_now + SA::row(0, u);
+                        if (threadIdx.x % SA::G == 0 && m < a.rows) rowsum[(int64_t)z_now * a.rows + m] = v;
+                    }
+                } else if constexpr (AM == MC) {
+                    s_n[threadIdx.x] = asum[0];
+                    __syncthreads();
+                    if (threadIdx.x < TM && m0_now + threadIdx.x < a.rows) {
+                        float v = 0.f;
+#pragma unroll
+                        for (int o = 0; o < kThreads / TM; ++o) v += s_n[threadIdx.x + o * TM];
+                        rowsum[(int64_t)z_now * a.rows + m0_now + threadIdx.x] = v;
+                    }
                 }
             }
         }
