@@ -243,7 +243,7 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
 
         auto put = [&] {
             // the waves that stage go before those that multiply: two workgroups share a SIMD, and the other one's products fill the
-            // gap (40000 x 8192 x 256: 1476 -> 1435 us)
+            // gap (40000 x 8192 x 256: 1089 -> 1054 us)
             __builtin_amdgcn_s_setprio(1);
             __syncthreads();   // the previous steps' fragments are read
             sa.store(s_a);
@@ -427,15 +427,17 @@ int launch_tiles(const char* what, const Operand& a, const Operand& b, float* ou
 template <int AM, int BM, int EPI>
 int launch_mm(const char* what, const Operand& a, const Operand& b, float* out, int64_t ldo, int64_t depth, int splits, int64_t piece,
               float scale, const float* sqnorm, float* rowsum, hipStream_t st) {
-    // The largest tile whose last round leaves few CUs idle: a round of 128 x 128 tiles on the 256 CUs takes twice one of 64 x 128
-    auto rounds = [&](int tm, int tn) {
+    // Cost of a tile size: tiles that the busiest CU gets, their area, and what a product costs in it -- the smaller tiles read and cut more
+    // per product (24000 x 512 x 256, the rows' gradient: 128 x 128 53 us, 64 x 128 60 us, 64 x 64 60 us with a third less work on the
+    // busiest CU; 375 x 512 x 256: 64 x 64 9 us, 128 x 128 19 us).
+    auto cost = [&](int tm, int tn, int each) {
         const int64_t n = ((a.rows + tm - 1) / tm) * ((b.rows + tn - 1) / tn) * splits;
-        return (n + 255) / 256 * (tm * tn);
+        return (n + 255) / 256 * (tm * tn) * (n <= 256 ? each + 3 : each);     // alone on its CU a tile's gaps stay open
     };
-    const int64_t r128 = rounds(128, 128), r64 = rounds(64, 128), r32 = rounds(64, 64);
-    if (r128 <= r64 + r64 / 8 && r128 <= r32 + r32 / 4)
+    const int64_t c128 = cost(128, 128, 10), c64 = cost(64, 128, 14), c32 = cost(64, 64, 15);
+    if (c128 <= c64 && c128 <= c32)
         return launch_tiles<128, 128, AM, BM, EPI>(what, a, b, out, ldo, depth, splits, piece, scale, sqnorm, rowsum, st);
-    if (r64 <= r32 + r32 / 8)
+    if (c64 <= c32)
         return launch_tiles<64, 128, AM, BM, EPI>(what, a, b, out, ldo, depth, splits, piece, scale, sqnorm, rowsum, st);
     return launch_tiles<64, 64, AM, BM, EPI>(what, a, b, out, ldo, depth, splits, piece, scale, sqnorm, rowsum, st);
 }
