@@ -67,7 +67,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
     objs = []
     obj_dir = os.path.join(HERE, "csrc", "_obj")
     os.makedirs(obj_dir, exist_ok=True)
-    flags = ["-O3", "-std=c++17", f"--offload-arch={ARCH}", "-fPIC", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function"]
+    # packed fp32 instructions are left out: some of their forms have given wrong results (the bench runs as fast without: 757 - 763 k
+    # epochs/s against 756 - 759 k)
+    flags = ["-O3", "-std=c++17", f"--offload-arch={ARCH}", "-fPIC", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     # The FFT kernels keep complex values as split re/im registers; the SLP vectorizer pairs them into packed-fp32 ops
     # and pays for it with register moves (fir_fft_kernel: 384 v_mov per item, 16 B of scratch; 3.9 -> 3.2 ms without).
     # Round 3: the same flag for three MFMA kernels whose side arithmetic hipcc had packed (v_pk_add_f32 beside MFMAs costs more than the
@@ -78,8 +81,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
         obj = os.path.join(obj_dir, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
         extra = ["-fno-slp-vectorize"] if os.path.basename(src) in no_slp else []
-        if os.path.basename(src).startswith("code_"):   # no packed fp32 instructions: some of their forms have given wrong results
-            extra += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
         if os.path.basename(src) == "vq.hip":   # 12.23 -> 12.04 ms on the quantizer (A/B x3); neutral on the conv kernels
             extra += ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]
         cmd = [_hipcc(), *flags, *extra, "-Rpass-analysis=kernel-resource-usage", "-c", src, "-o", obj]
