@@ -369,7 +369,8 @@ template <typename T, int V, bool VEC>
 __global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ scores, int64_t lds, const float* __restrict__ u,
                                                           Params par, const uint8_t* __restrict__ allowed, int64_t allowed_ld,
                                                           int64_t* __restrict__ out, int64_t N, int K) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    // one value per wave, and the compiler is told so: branches on a row's settings are the scalar unit's (604 -> 586 us at 384000 x 512, top-k 100)
+    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= N) return;                // a whole wave
     Row<V> R;
     lbm::load_row<T, V, 1, VEC>(scores + row * lds, K, R.lane(), R.v);
