@@ -720,11 +720,15 @@ __device__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, i
         }
         const double goal = s.u * here;
         if (groups <= 64) {
-            for (int g = 0; g + 1 < groups; ++g) {
+            double run = 0.0;
+            for (int g = 0; g < groups; ++g) {
                 const double w = lbm::lane_value(mine, g);
-                if (base + w > goal) break;
-                base += w;
-                start = (g + 1) * 2048;
+                if (w > 0.0) {           // where none passes the goal (u of 1 or more, NaN) the last group that holds a weight
+                    start = g * 2048;
+                    base = run;
+                }
+                run += w;
+                if (run > goal) break;
             }
         }
     } else {

@@ -370,6 +370,16 @@ def test_sample_u_at_the_ends_and_outside():
     u = torch.tensor([0.0, 1.0 - 2.0 ** -24, 1.0, 2.0, 0.5, 0.0, 1.0, 1e-30])
     for kw in (dict(), dict(top_k=3), dict(top_p=0.4, min_p=0.01)):
         check_sample(s, u, **kw)
+    # rows whose weight lies in their first columns only, in the middle, at the end
+    for K in (900, 5000, 150_000):
+        s = torch.full((8, K), float("-inf"))
+        s[:4, 5:300] = torch.randn((4, 295), generator=g)
+        s[4:6, K // 2:K // 2 + 90] = torch.randn((2, 90), generator=g)
+        s[6:, -700:] = torch.randn((2, 700), generator=g)
+        s[::2, 700:] = torch.maximum(s[::2, 700:], torch.tensor(-2000.0))      # there, but without weight in 64 bits
+        for kw in (dict(), dict(top_k=280, top_p=0.999), dict(top_p=0.4, min_p=0.01), dict(min_p=1e-4), dict(temperature=0.0)):
+            check_sample(s, u, **kw)
+    s = torch.randn((8, 100), generator=g)
     # numbers that are none of [0, 1): the last code that stayed for NaN, the first for negative ones
     got = lbm_amd.sample_codes(s[:2].to(DEV), torch.tensor([float("nan"), -1.0], device=DEV)).cpu()
     assert got.tolist() == [99, 0]
