@@ -1,6 +1,5 @@
-// Rows of scores [N, K] (fp32, fp16 or bf16) held in the registers of a team of wavefronts: what the usage-balance and the sampling kernels
-// share.  A team is W waves; its thread t holds V scores of the row, four neighbours at a time: value 4c + i of thread t is column
-// (c * 64 W + t) * 4 + i, so a wave's loads are 1 KiB (fp32) or 512 bytes in one piece and ascending columns are chunk, thread, i.
+// Rows of scores (fp32, fp16 or bf16) in the registers of a wave: conversions, loads and wave-wide sums, maxima and running sums, shared by the
+// usage-balance and the sampling kernels.
 #pragma once
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -32,12 +31,13 @@ struct alignas(4 * sizeof(T)) Quad {
     T v[4];
 };
 
-// v[] = the row's scores of thread t, -inf past column K.  VEC: four scores in one access (aligned base and row stride, K % 4 == 0).
-template <typename T, int V, int W, bool VEC>
+// The row's scores of one wave's lanes, -inf past column K: value 4c + i of lane t is column (64 c + t) * 4 + i, so ascending columns are chunk,
+// lane, i.  VEC: four scores in one access (aligned base and row stride, K % 4 == 0).
+template <typename T, int V, bool VEC>
 __device__ __forceinline__ void load_row(const T* __restrict__ row, int K, int t, float* v) {
 #pragma unroll
     for (int c = 0; c < V / 4; ++c) {
-        const int col = (c * 64 * W + t) * 4;
+        const int col = (c * 64 + t) * 4;
         if constexpr (VEC) {
             Quad<T> q;
 #pragma unroll
@@ -95,27 +95,10 @@ struct OpAdd {
     __device__ __forceinline__ A operator()(A a, A b) const { return a + b; }
 };
 
-
 template <typename A>
 __device__ __forceinline__ A wave_total(A x) { return lane_value(wave_scan<A>(x, A(0), OpAdd()), 63); }
 __device__ __forceinline__ float wave_best(float x) { return lane_value(wave_scan<float>(x, -INFINITY, OpMax()), 63); }
 __device__ __forceinline__ int wave_first(int x) { return lane_value(wave_scan<int>(x, 0x7fffffff, OpMin()), 63); }
-
-// one value per wave of a workgroup of W waves -> all of them, through s ([2][W] in LDS, `round` alternates between the halves: one barrier
-// per exchange, since a half is rewritten only after the next exchange's barrier)
-template <typename A, int W, typename Op>
-__device__ __forceinline__ A team_join(A x, A* s, int& round, Op op) {
-    if constexpr (W > 1) {
-        A* slot = s + round * W;
-        round ^= 1;
-        if ((threadIdx.x & 63) == 0) slot[threadIdx.x >> 6] = x;
-        __syncthreads();
-        x = slot[0];
-#pragma unroll
-        for (int w = 1; w < W; ++w) x = op(x, slot[w]);
-    }
-    return x;
-}
 
 }  // namespace lbm
 

@@ -373,7 +373,7 @@ __global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ 
     const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= N) return;                // a whole wave
     Row<V> R;
-    lbm::load_row<T, V, 1, VEC>(scores + row * lds, K, R.lane(), R.v);
+    lbm::load_row<T, V, VEC>(scores + row * lds, K, R.lane(), R.v);
     if (allowed != nullptr) {
         const uint8_t* a = allowed + row * allowed_ld;
 #pragma unroll
