@@ -8,8 +8,10 @@
 // (4 operations per score), the gradient reads them again and writes as much.  A row lives in registers between its load, its maximum, its
 // sum and its use, the next row's load runs under that, and every thread adds p of its own columns over all rows it sees, so the column
 // sums cost no traffic until the end, where each workgroup leaves one partial row.  Partial sums are joined in a fixed order in 64 bits:
-// results do not change from run to run.  Up to 1024 codes a wave holds a row (no barrier); above that four waves share one and
-// exchange their maxima and sums once per row (eight waves with half the registers each: 217 us for 172 at 40000 x 8192 bf16).
+// results do not change from run to run.  Up to 2048 codes a wave holds a row, or eight, four or two short ones (no barrier); above
+// that four waves share one and exchange their maxima and sums once per row (2048 codes in four waves: 398 us for 264 at 100000 rows of
+// bf16 with the gradient; 8192 in eight waves with half the registers each: 217 us for 172 at 40000 rows; 5 codes, a row to a wave: 653 us
+// for 108 at 1043158 rows of bf16 with the gradient).
 // The gradient takes a relative to its value at the row's best score: where one p is near 1 its a - p.a is a difference of near equals
 // otherwise, and loses what it should return.
 #include "code_rows.h"
@@ -30,10 +32,11 @@ struct Plan {
     size_t off_cnt, off_rows, off_sum2, off_cnt2, total;
 };
 
-int waves_for(int K) { return K <= 1024 ? 1 : 4; }
+// lanes that share a row (256: the workgroup)
+int lanes_for(int K) { return K <= 8 ? 8 : (K <= 64 ? 16 : (K <= 128 ? 32 : (K <= 2048 ? 64 : 256))); }
 
 Plan make_plan(int64_t N, int K) {
-    const int T = waves_for(K) == 1 ? 4 : 1;
+    const int T = 256 / lanes_for(K);     // rows a workgroup works on at a time
     Plan p;
     // eight rows per team at least, so that the partial rows stay small beside the scores -- two where that leaves CUs without work
     p.G = (N + 8 * T - 1) / (8 * T);
@@ -41,7 +44,8 @@ Plan make_plan(int64_t N, int K) {
         p.G = (N + 2 * T - 1) / (2 * T);
         if (p.G > 512) p.G = 512;
     }
-    const int64_t cap = T == 4 ? 2048 : (K <= 4096 ? 1024 : 768);   // as many as run at a time
+    // as many as the registers let run at a time: 8, 7, 4, 3, 4 and 3 per CU (7 at 1536000 x 512 fp32: 603 us, 8 in two rounds 660)
+    const int64_t cap = 256 * (K <= 128 ? 8 : (K <= 512 ? 7 : (K <= 1024 ? 4 : (K <= 2048 ? 3 : (K <= 4096 ? 4 : 3)))));
     if (p.G > cap) p.G = cap;
     if (p.G < 1) p.G = 1;
     const int groups = (K + kJoinCols - 1) / kJoinCols;
@@ -58,18 +62,18 @@ Plan make_plan(int64_t N, int K) {
     return p;
 }
 
-// A row's scores as loaded, 16 bytes at a time: value E c + i of thread t is column (c * 64 W + t) * E + i
-template <typename T, int V, int W, bool VEC>
+// A row's scores as loaded by its L lanes, E of 16 bytes at most at a time: value E c + i of lane t is column (c * L + t) * E + i
+template <typename T, int V, int L, bool VEC>
 struct Held {
-    static constexpr int E = 16 / sizeof(T);
-    struct alignas(16) Pack { T v[E]; };
+    static constexpr int E = V < 16 / (int)sizeof(T) ? V : 16 / (int)sizeof(T);
+    struct alignas(E * sizeof(T)) Pack { T v[E]; };
     Pack q[V / E];
 
-    static __device__ __forceinline__ int column(int i, int t) { return ((i / E) * 64 * W + t) * E + i % E; }
+    static __device__ __forceinline__ int column(int i, int t) { return ((i / E) * L + t) * E + i % E; }
     __device__ __forceinline__ void load(const T* __restrict__ row, int K, int t) {
 #pragma unroll
         for (int c = 0; c < V / E; ++c) {
-            const int col = (c * 64 * W + t) * E;
+            const int col = (c * L + t) * E;
             if (VEC && col < K) {
                 q[c] = *reinterpret_cast<const Pack*>(row + col);
             } else {
@@ -81,38 +85,75 @@ struct Held {
     __device__ __forceinline__ float at(int i) const { return lbm::score_to_f32<T>(q[i / E].v[i % E]); }
 };
 
-// 16 bytes of scores, each rounded once to the nearest
-template <typename T>
-__device__ __forceinline__ uint4 pack16(const float* f) {
-    unsigned w[4];
+// E scores, each rounded once to the nearest, in one access
+template <typename T, int E>
+__device__ __forceinline__ void store_pack(T* out, const float* f) {
+    if constexpr (E * sizeof(T) < 4) {
+        out[0] = lbm::score_from_f32<T>(f[0]);
+    } else {
+        constexpr int W = E * sizeof(T) / 4;
+        unsigned w[W];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if constexpr (sizeof(T) == 4) {
-            w[i] = __float_as_uint(f[i]);
-        } else {
-            const T a = lbm::score_from_f32<T>(f[2 * i]), b = lbm::score_from_f32<T>(f[2 * i + 1]);
-            w[i] = (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16;
+        for (int i = 0; i < W; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                w[i] = __float_as_uint(f[i]);
+            } else {
+                const T a = lbm::score_from_f32<T>(f[2 * i]), b = lbm::score_from_f32<T>(f[2 * i + 1]);
+                w[i] = (unsigned)__builtin_bit_cast(unsigned short, a) | (unsigned)__builtin_bit_cast(unsigned short, b) << 16;
+            }
         }
+        if constexpr (W == 4) *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (W == 2) *reinterpret_cast<uint2*>(out) = make_uint2(w[0], w[1]);
+        else *reinterpret_cast<unsigned*>(out) = w[0];
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// exp(x), x <= 0: the difference, the product and the exponential round once each, (2 |x| + 2) 2^-24 relative
-__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
+constexpr float kLog2e = 1.44269502f;
 
-template <typename T, int V, int W, bool VEC>
-__global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_rows_kernel(const T* __restrict__ scores, int64_t lds, const int64_t* __restrict__ codes,
-                                                           int slots, const uint8_t* __restrict__ keep, float2* __restrict__ stat,
-                                                           float* __restrict__ part, unsigned* __restrict__ part_cnt,
-                                                           unsigned* __restrict__ part_rows, int64_t N, int K) {
-    constexpr int TEAMS = W == 1 ? 4 : 1;
-    using H = Held<T, V, W, VEC>;
-    extern __shared__ unsigned s_cnt[];                  // [K] picks; then, W == 1, the teams' column sums one after the other
+// exp(x), x <= 0: (2 |x| + 2) 2^-24 relative
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// exp(v - m) times a factor that all scores of a row share: 2^(v log2(e) - ml) with ml = m log2(e) rounded, one fused operation and so one
+// rounding of the exponent, where the difference and its product are two (errors of a row's gradients: 3e-7 for 1e-6).  The factor is
+// 2^(m log2(e) - ml); it drops out of e / sum(e).  Scores of 10^6 and more, where ml is no longer near the exponents, take the difference.
+struct RowExp {
+    float m, ml;
+    bool near;
+    __device__ __forceinline__ explicit RowExp(float best) : m(best), ml(best * kLog2e), near(fabsf(best) < 1e6f) {}
+    template <int V>
+    __device__ __forceinline__ void apply(float* v) const {
+        if (near) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = __builtin_amdgcn_exp2f(fmaf(v[i], kLog2e, -ml));
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = exp_neg(v[i] - m);
+        }
+    }
+    // log2 of the factor
+    __device__ __forceinline__ float excess() const { return near ? fmaf(m, kLog2e, -ml) : 0.f; }
+};
+
+// the team; one wave to a row: the same in all its lanes, and the row's addresses are scalar.  (Where four waves share a row that costs
+// registers that the longest rows do not have: 40000 x 8192 fp32 370 us for 267.)
+template <int L>
+__device__ __forceinline__ int team_of() {
+    return L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : threadIdx.x / L;
+}
+
+template <typename T, int V, int L, bool VEC>
+__global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_rows_kernel(const T* __restrict__ scores, int64_t lds,
+                                                                           const int64_t* __restrict__ codes, int slots,
+                                                                           const uint8_t* __restrict__ keep, float2* __restrict__ stat,
+                                                                           float* __restrict__ part, unsigned* __restrict__ part_cnt,
+                                                                           unsigned* __restrict__ part_rows, int64_t N, int K) {
+    constexpr int TEAMS = 256 / L, W = L > 64 ? L / 64 : 1, LW = L > 64 ? 64 : L;
+    using H = Held<T, V, L, VEC>;
+    extern __shared__ unsigned s_cnt[];                  // [K] picks; then the teams' column sums [TEAMS][K]
     __shared__ float2 s_ms[2][W];                        // W > 1: (maximum, sum) of each wave
     __shared__ int s_best[2][W];
-    __shared__ unsigned s_rows[4];
-    const int wave = threadIdx.x >> 6;
-    const int t = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    __shared__ unsigned s_rows[TEAMS];
+    const int team = team_of<L>(), t = threadIdx.x % L, wave = threadIdx.x >> 6;
     const int64_t step = (int64_t)gridDim.x * TEAMS;
     for (int k = threadIdx.x; k < K; k += 256) s_cnt[k] = 0u;
     __syncthreads();
@@ -122,13 +163,28 @@ __global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_rows_kernel(cons
     for (int i = 0; i < V; ++i) acc[i] = 0.f;
     unsigned rows = 0;
     int round = 0;
-    auto kept = [&](int64_t r) { return r < N && (keep == nullptr || keep[r] != 0); };
-    int64_t row = (int64_t)blockIdx.x * TEAMS + (W == 1 ? wave : 0);
-    bool on = kept(row), on_next = kept(row + step);
+    // What the next row needs is loaded while this one is worked on: its scores, its picks, and the keep byte of the row behind it.  Loads
+    // return in order, so nothing that this row waits for is loaded behind them -- but for the picks of the longest rows, whose registers
+    // are all taken.
+    constexpr bool AHEAD = V < 32;
+    auto kept = [&](int64_t r) -> unsigned {
+        unsigned v = 0u;
+        if (r < N) v = keep != nullptr ? keep[r] : 1u;
+        return v;
+    };
+    auto picked = [&](int64_t r) -> int64_t {
+        int64_t v = -1;
+        if (codes != nullptr && t < slots && r < N) v = codes[r * slots + t];
+        return v;
+    };
+    int64_t row = (int64_t)blockIdx.x * TEAMS + team;
+    unsigned on = kept(row), on_next = kept(row + step);
+    int64_t pick_next = AHEAD ? picked(row) : -1;
     H held;
     if (on) held.load(scores + row * lds, K, t);
     for (; row < N; row += step) {
-        const bool now = on;
+        const bool now = on != 0u;
+        int64_t pick = pick_next;
         float e[V];
         if (now) {
 #pragma unroll
@@ -136,43 +192,41 @@ __global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_rows_kernel(cons
         }
         on = on_next;
         if (on) held.load(scores + (row + step) * lds, K, t);
+        if constexpr (AHEAD) pick_next = picked(row + step);
+        else pick = picked(row);
         on_next = kept(row + 2 * step);
         if (!now) {
             if (t == 0) stat[row] = make_float2(0.f, 0.f);
             continue;
         }
-        int64_t pick = -1;
-        if (codes != nullptr && t < slots) pick = codes[row * slots + t];
         float m = -INFINITY;
 #pragma unroll
         for (int i = 0; i < V; ++i) m = fmaxf(m, e[i]);
-        m = lbm::wave_best(m);
+        m = lbm::group_best<LW>(m);
         int best = 0x7fffffff;
         if (codes == nullptr && m > -INFINITY) {         // lowest column that holds the (wave's) maximum
 #pragma unroll
             for (int i = V - 1; i >= 0; --i) best = e[i] == m ? H::column(i, t) : best;
-            best = lbm::wave_first(best);
+            best = lbm::group_first<LW>(best);
         }
-        float s = 0.f, scale;
-        bool nan = false;
+        const RowExp x(m);
+        float s = 0.f, scale = 1.f;
         if (m == -INFINITY) {                            // nothing but -inf, or NaN, which shows
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                nan |= e[i] != e[i];
+                s = e[i] != e[i] ? e[i] : s;
                 e[i] = e[i] != e[i] ? e[i] : 0.f;
             }
-            s = __any(nan) ? NAN : 0.f;
         } else {
+            x.template apply<V>(e);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                e[i] = exp_neg(e[i] - m);
-                s += e[i];
-            }
-            s = lbm::wave_total(s);
+            for (int i = 0; i < V; ++i) s += e[i];
         }
+        s = lbm::group_total<LW>(s);
         if constexpr (W > 1) {                           // the waves' pairs joined: one barrier per row, since the other half of s_ms is
-            if ((threadIdx.x & 63) == 0) {               // written only behind the next row's
-                s_ms[round][wave] = make_float2(m, s);
+            scale = __builtin_amdgcn_exp2f(-x.excess()); // written only behind the next row's
+            if ((threadIdx.x & 63) == 0) {
+                s_ms[round][wave] = make_float2(m, m == -INFINITY ? s : s * scale);
                 s_best[round][wave] = best;
             }
             __syncthreads();
@@ -192,23 +246,22 @@ __global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_rows_kernel(cons
                 best = ms[w].x == m && bw < best ? bw : best;
             }
             round ^= 1;
-            scale = m_wave == m ? 1.f : exp_neg(m_wave - m);
-        } else {
-            scale = 1.f;
+            scale *= m_wave == m ? 1.f : exp_neg(m_wave - m);
         }
         if (m == -INFINITY && s == 0.f) {
             if (t == 0) stat[row] = make_float2(0.f, 0.f);
             continue;
         }
-        const float r = 1.f / s;
+        float r = __builtin_amdgcn_rcpf(s);              // within a unit in the last place
         scale *= r;
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = fmaf(e[i], scale, acc[i]);
         ++rows;
-        if (t == 0) stat[row] = make_float2(m, r);
+        if constexpr (W > 1) r *= __builtin_amdgcn_exp2f(RowExp(m).excess());
+        if (t == 0) stat[row] = make_float2(m, r);       // p = r exp(), with the row's factor
         if (codes != nullptr) {
             if (pick >= 0 && pick < K) atomicAdd(&s_cnt[(int)pick], 1u);
-            for (int q = t + 64 * W; q < slots; q += 64 * W) {
+            for (int q = t + L; q < slots; q += L) {
                 const int64_t k = codes[row * slots + q];
                 if (k >= 0 && k < K) atomicAdd(&s_cnt[(int)k], 1u);
             }
@@ -220,22 +273,27 @@ __global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_rows_kernel(cons
     unsigned* pc = part_cnt + (int64_t)blockIdx.x * K;
     for (int k = threadIdx.x; k < K; k += 256) pc[k] = s_cnt[k];
     float* pp = part + (int64_t)blockIdx.x * K;
-    if constexpr (W == 1) {
+    if (t == 0) s_rows[team] = rows;
+    if constexpr (TEAMS > 1) {
         float* s_sum = reinterpret_cast<float*>(s_cnt);
-        if (t == 0) s_rows[wave] = rows;
-        for (int g = 0; g < TEAMS; ++g) {                // the teams in order
-            __syncthreads();
-            if (wave == g) {
+        __syncthreads();
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const int k = H::column(i, t);
-                    if (k < K) s_sum[k] = g == 0 ? acc[i] : s_sum[k] + acc[i];
-                }
-            }
+        for (int i = 0; i < V; ++i) {
+            const int k = H::column(i, t);
+            if (k < K) s_sum[team * K + k] = acc[i];
         }
         __syncthreads();
-        for (int k = threadIdx.x; k < K; k += 256) pp[k] = s_sum[k];
-        if (threadIdx.x == 0) part_rows[blockIdx.x] = (s_rows[0] + s_rows[1]) + (s_rows[2] + s_rows[3]);
+        for (int k = threadIdx.x; k < K; k += 256) {     // the teams in order
+            float v = 0.f;
+#pragma unroll
+            for (int g = 0; g < TEAMS; ++g) v += s_sum[g * K + k];
+            pp[k] = v;
+        }
+        if (threadIdx.x == 0) {
+            rows = 0;
+            for (int g = 0; g < TEAMS; ++g) rows += s_rows[g];
+            part_rows[blockIdx.x] = rows;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -343,16 +401,16 @@ __global__ __launch_bounds__(kFinish) void balance_finish_kernel(const double* _
     }
 }
 
-template <typename T, int V, int W, bool VEC>
-__global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_grad_kernel(const T* __restrict__ scores, int64_t lds, const float2* __restrict__ stat,
-                                                           const int64_t* __restrict__ counts, const double* __restrict__ totals,
-                                                           const float* __restrict__ g_loss, const float* __restrict__ g_mean,
-                                                           T* __restrict__ ds, int64_t N, int K) {
-    constexpr int TEAMS = W == 1 ? 4 : 1;
-    using H = Held<T, V, W, VEC>;
+template <typename T, int V, int L, bool VEC>
+__global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_grad_kernel(const T* __restrict__ scores, int64_t lds,
+                                                                           const float2* __restrict__ stat, const int64_t* __restrict__ counts,
+                                                                           const double* __restrict__ totals, const float* __restrict__ g_loss,
+                                                                           const float* __restrict__ g_mean, T* __restrict__ ds, int64_t N,
+                                                                           int K) {
+    constexpr int TEAMS = 256 / L, W = L > 64 ? L / 64 : 1, LW = L > 64 ? 64 : L;
+    using H = Held<T, V, L, VEC>;
     __shared__ float4 s_x[2][W];                         // W > 1: each wave's p.(a - ref), its sum of p, its ref, whether it holds the best
-    const int wave = threadIdx.x >> 6;
-    const int t = W == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const int team = team_of<L>(), t = threadIdx.x % L, wave = threadIdx.x >> 6;
     const int64_t step = (int64_t)gridDim.x * TEAMS;
     const double M = totals[0], C = totals[1];
     const double gl = g_loss != nullptr && C > 0.0 ? (double)g_loss[0] * K / C : 0.0;
@@ -364,7 +422,7 @@ __global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_grad_kernel(cons
         a[i] = k < K ? (float)(gl * (double)counts[k] + (g_mean != nullptr ? (double)g_mean[k] : 0.0)) : 0.f;
     }
     int round = 0;
-    int64_t row = (int64_t)blockIdx.x * TEAMS + (W == 1 ? wave : 0);
+    int64_t row = (int64_t)blockIdx.x * TEAMS + team;
     auto row_stat = [&](int64_t q) {
         float2 v = make_float2(0.f, 0.f);
         if (q < N) v = stat[q];
@@ -390,43 +448,41 @@ __global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_grad_kernel(cons
             float ref = -INFINITY, dot = 0.f, mass = 0.f;
 #pragma unroll
             for (int i = 0; i < V; ++i) ref = d[i] == m ? fmaxf(ref, a[i]) : ref;
-            ref = lbm::wave_best(ref);
+            ref = lbm::group_best<LW>(ref);
             const bool best = ref > -INFINITY;
             if (W > 1 && !best) ref = 0.f;
+            RowExp(m).template apply<V>(d);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                d[i] = exp_neg(d[i] - m) * r;
                 dot = fmaf(d[i], a[i] - ref, dot);
                 if constexpr (W > 1) mass += d[i];
             }
-            dot = lbm::wave_total(dot);
+            dot = lbm::group_total<LW>(dot) * r;
             if constexpr (W > 1) {                       // p.(a - ref of the best score), from each wave's own reference
-                mass = lbm::wave_total(mass);
+                mass = lbm::group_total<LW>(mass) * r;
                 if ((threadIdx.x & 63) == 0) s_x[round][wave] = make_float4(dot, mass, ref, best ? 1.f : 0.f);
                 __syncthreads();
-                float4 x[W];
+                float4 xs[W];
                 ref = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
-                    x[w] = s_x[round][w];
-                    ref = x[w].w != 0.f ? fmaxf(ref, x[w].z) : ref;
+                    xs[w] = s_x[round][w];
+                    ref = xs[w].w != 0.f ? fmaxf(ref, xs[w].z) : ref;
                 }
                 dot = 0.f;
 #pragma unroll
-                for (int w = 0; w < W; ++w) dot += fmaf(x[w].z - ref, x[w].y, x[w].x);
+                for (int w = 0; w < W; ++w) dot += fmaf(xs[w].z - ref, xs[w].y, xs[w].x);
                 round ^= 1;
             }
 #pragma unroll
-            for (int i = 0; i < V; ++i) d[i] = d[i] * ((a[i] - ref) - dot) * inv_m;
+            for (int i = 0; i < V; ++i) d[i] *= ((a[i] - ref) - dot) * (r * inv_m);
         }
         T* out = ds + row * (int64_t)K;
 #pragma unroll
         for (int c = 0; c < V / H::E; ++c) {
-            const int col = (c * 64 * W + t) * H::E;
+            const int col = (c * L + t) * H::E;
             if constexpr (VEC) {
-                if (col < K) {
-                    *reinterpret_cast<uint4*>(out + col) = pack16<T>(d + H::E * c);
-                }
+                if (col < K) store_pack<T, H::E>(out + col, d + H::E * c);
             } else {
 #pragma unroll
                 for (int i = 0; i < H::E; ++i)
@@ -436,27 +492,33 @@ __global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_grad_kernel(cons
     }
 }
 
-// 16 bytes at a time: aligned base and rows, and the last 16 bytes of a row end with it
-template <typename T>
+// E scores at a time: aligned base and rows, and the last access of a row ends with it
+template <typename T, int V>
 bool vec_ok(const void* p, int64_t ld, int K) {
-    constexpr int E = 16 / sizeof(T);
-    return ((uintptr_t)p & 15) == 0 && ld % E == 0 && K % E == 0;
+    constexpr int E = Held<T, V, 64, true>::E;
+    return (uintptr_t)p % (E * sizeof(T)) == 0 && ld % E == 0 && K % E == 0;
 }
+
+// CALL(V, L): V scores in each of the L = lanes_for(K) lanes of a row
+#define LBM_BALANCE_SIZES(CALL)       \
+    if (K <= 8) CALL(1, 8);           \
+    else if (K <= 64) CALL(4, 16);    \
+    else if (K <= 128) CALL(4, 32);   \
+    else if (K <= 512) CALL(8, 64);   \
+    else if (K <= 1024) CALL(16, 64); \
+    else if (K <= 2048) CALL(32, 64); \
+    else if (K <= 4096) CALL(16, 256); \
+    else CALL(32, 256);
 
 template <typename T>
 int run_rows(const void* scores, int64_t lds, const int64_t* codes, int slots, const uint8_t* keep, float2* stat, float* part, unsigned* cnt,
              unsigned* rows, int64_t G, int64_t N, int K, hipStream_t st) {
     const T* s = static_cast<const T*>(scores);
-    const bool vec = vec_ok<T>(scores, lds, K);
-    const size_t shm = (size_t)K * 4;
-#define LBM_ROWS(V, W)                                                                                                              \
-    hipLaunchKernelGGL((vec ? balance_rows_kernel<T, V, W, true> : balance_rows_kernel<T, V, W, false>), dim3((unsigned)G), dim3(256), \
-                       shm, st, s, lds, codes, slots, keep, stat, part, cnt, rows, N, K)
-    if (K <= 512) LBM_ROWS(8, 1);
-    else if (K <= 1024) LBM_ROWS(16, 1);
-    else if (K <= 2048) LBM_ROWS(8, 4);
-    else if (K <= 4096) LBM_ROWS(16, 4);
-    else LBM_ROWS(32, 4);
+    const size_t shm = (size_t)K * 4 * (256 / lanes_for(K));
+#define LBM_ROWS(V, L)                                                                                                             \
+    hipLaunchKernelGGL((vec_ok<T, V>(scores, lds, K) ? balance_rows_kernel<T, V, L, true> : balance_rows_kernel<T, V, L, false>), \
+                       dim3((unsigned)G), dim3(256), shm, st, s, lds, codes, slots, keep, stat, part, cnt, rows, N, K)
+    LBM_BALANCE_SIZES(LBM_ROWS)
 #undef LBM_ROWS
     return lbm::check_launch("lbm_code_balance");
 }
@@ -466,15 +528,11 @@ int run_grad(const void* scores, int64_t lds, const float2* stat, const int64_t*
              const float* g_mean, void* ds, int64_t G, int64_t N, int K, hipStream_t st) {
     const T* s = static_cast<const T*>(scores);
     T* o = static_cast<T*>(ds);
-    const bool vec = vec_ok<T>(scores, lds, K) && vec_ok<T>(ds, K, K);
-#define LBM_GRAD(V, W)                                                                                                              \
-    hipLaunchKernelGGL((vec ? balance_grad_kernel<T, V, W, true> : balance_grad_kernel<T, V, W, false>), dim3((unsigned)G), dim3(256), \
-                       0, st, s, lds, stat, counts, totals, g_loss, g_mean, o, N, K)
-    if (K <= 512) LBM_GRAD(8, 1);
-    else if (K <= 1024) LBM_GRAD(16, 1);
-    else if (K <= 2048) LBM_GRAD(8, 4);
-    else if (K <= 4096) LBM_GRAD(16, 4);
-    else LBM_GRAD(32, 4);
+#define LBM_GRAD(V, L)                                                                                                      \
+    hipLaunchKernelGGL((vec_ok<T, V>(scores, lds, K) && vec_ok<T, V>(ds, K, K) ? balance_grad_kernel<T, V, L, true>        \
+                                                                              : balance_grad_kernel<T, V, L, false>),      \
+                       dim3((unsigned)G), dim3(256), 0, st, s, lds, stat, counts, totals, g_loss, g_mean, o, N, K)
+    LBM_BALANCE_SIZES(LBM_GRAD)
 #undef LBM_GRAD
     return lbm::check_launch("lbm_code_balance_grad");
 }
@@ -528,7 +586,7 @@ extern "C" int lbm_code_balance_grad(const void* scores, int32_t dtype, int64_t 
     if (N == 0) return LBM_OK;
     LBM_REQUIRE(scores && row_stat && counts && totals && dscores, LBM_EINVAL, "%s: NULL pointer", what);
     LBM_REQUIRE(N <= 1 || lds >= 0, LBM_EINVAL, "%s: negative row stride", what);
-    const int64_t T = waves_for(K) == 1 ? 4 : 1, cap = T == 4 ? 2048 : (K <= 4096 ? 1024 : 512);
+    const int64_t T = 256 / lanes_for(K), cap = T >= 4 ? 2048 : (K <= 4096 ? 1024 : 512);
     int64_t G = (N + T - 1) / T;
     if (G > cap) G = cap;
     int rc = LBM_OK;

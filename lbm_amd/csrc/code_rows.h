@@ -100,6 +100,29 @@ __device__ __forceinline__ A wave_total(A x) { return lane_value(wave_scan<A>(x,
 __device__ __forceinline__ float wave_best(float x) { return lane_value(wave_scan<float>(x, -INFINITY, OpMax()), 63); }
 __device__ __forceinline__ int wave_first(int x) { return lane_value(wave_scan<int>(x, 0x7fffffff, OpMin()), 63); }
 
+// op over the L neighbouring lanes of a row, the result in each of them.  L < 64: exchanges inside rows of 16 lanes (pairs, quads, halves,
+// the row's mirror image) and one across two rows; other rows' lanes may be off.
+template <int L, typename A, typename Op>
+__device__ __forceinline__ A group_all(A x, A none, Op op) {
+    static_assert(L == 8 || L == 16 || L == 32 || L == 64, "lanes of a row");
+    if constexpr (L == 64) {
+        return lane_value(wave_scan<A>(x, none, op), 63);
+    } else {
+        x = op(x, dpp_move<0xB1, 0xf>(x, x));
+        x = op(x, dpp_move<0x4E, 0xf>(x, x));
+        x = op(x, dpp_move<0x141, 0xf>(x, x));
+        if constexpr (L > 8) x = op(x, dpp_move<0x140, 0xf>(x, x));
+        if constexpr (L > 16) x = op(x, __shfl_xor(x, 16, 64));
+        return x;
+    }
+}
+template <int L>
+__device__ __forceinline__ float group_total(float x) { return group_all<L>(x, 0.f, OpAdd()); }
+template <int L>
+__device__ __forceinline__ float group_best(float x) { return group_all<L>(x, -INFINITY, OpMax()); }
+template <int L>
+__device__ __forceinline__ int group_first(int x) { return group_all<L>(x, 0x7fffffff, OpMin()); }
+
 }  // namespace lbm
 
 // CALL(type) for an LBM_F32 / LBM_F16 / LBM_BF16 argument

@@ -197,6 +197,17 @@ def test_balance_sizes_and_types(kind, N, K):
     check_balance(s, torch.randint(-1, K + 1, (N, 3), generator=g), torch.rand((N,), generator=g) < 0.8)
 
 
+@pytest.mark.parametrize("kind", sorted(TYPES))
+@pytest.mark.parametrize("K", (1, 2, 5, 8, 9, 17, 32, 33, 64, 65, 100, 128, 129))
+def test_balance_rows_that_share_a_wave(kind, K):
+    g = gen(1000 + K)
+    s = (torch.randn((1237, K), generator=g) * 3).to(TYPES[kind])
+    s[5::7, : K // 2] = float("-inf")
+    s[11::13] = float("-inf")                     # rows that end early beside rows that do not
+    check_balance(s, None, torch.rand((1237,), generator=g) < 0.7)
+    check_balance(s[:1200:3], torch.randint(-1, K, (400, 40), generator=g), None)      # more picks than lanes
+
+
 def test_balance_many_rows():
     g = gen(5)
     s = torch.randn((30011, 96), generator=g) * 2
