@@ -62,10 +62,11 @@ Plan make_plan(int64_t N, int K) {
     return p;
 }
 
-// A row's scores as loaded by its L lanes, E of 16 bytes at most at a time: value E c + i of lane t is column (c * L + t) * E + i
+// A row's scores as loaded by its L lanes, E at a time: value E c + i of lane t is column (c * L + t) * E + i.  E is 16 bytes at most, or 1
+// where rows or their addresses are no multiples of that: then one load takes L neighbouring scores
 template <typename T, int V, int L, bool VEC>
 struct Held {
-    static constexpr int E = V < 16 / (int)sizeof(T) ? V : 16 / (int)sizeof(T);
+    static constexpr int E = !VEC ? 1 : (V < 16 / (int)sizeof(T) ? V : 16 / (int)sizeof(T));
     struct alignas(E * sizeof(T)) Pack { T v[E]; };
     Pack q[V / E];
 
@@ -74,11 +75,11 @@ struct Held {
 #pragma unroll
         for (int c = 0; c < V / E; ++c) {
             const int col = (c * L + t) * E;
-            if (VEC && col < K) {
+            if (col < K) {
                 q[c] = *reinterpret_cast<const Pack*>(row + col);
             } else {
 #pragma unroll
-                for (int i = 0; i < E; ++i) q[c].v[i] = !VEC && col + i < K ? row[col + i] : lbm::score_from_f32<T>(-INFINITY);
+                for (int i = 0; i < E; ++i) q[c].v[i] = lbm::score_from_f32<T>(-INFINITY);
             }
         }
     }
@@ -481,13 +482,7 @@ __global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_grad_kernel(cons
 #pragma unroll
         for (int c = 0; c < V / H::E; ++c) {
             const int col = (c * L + t) * H::E;
-            if constexpr (VEC) {
-                if (col < K) store_pack<T, H::E>(out + col, d + H::E * c);
-            } else {
-#pragma unroll
-                for (int i = 0; i < H::E; ++i)
-                    if (col + i < K) out[col + i] = lbm::score_from_f32<T>(d[H::E * c + i]);
-            }
+            if (col < K) store_pack<T, H::E>(out + col, d + H::E * c);
         }
     }
 }
