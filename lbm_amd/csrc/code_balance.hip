@@ -258,7 +258,7 @@ __global__ __launch_bounds__(256, V == 32 ? 3 : 4) void balance_rows_kernel(cons
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] = fmaf(e[i], scale, acc[i]);
         ++rows;
-        if constexpr (W > 1) r *= __builtin_amdgcn_exp2f(RowExp(m).excess());
+        if constexpr (W > 1) r *= __builtin_amdgcn_exp2f(-RowExp(m).excess());
         if (t == 0) stat[row] = make_float2(m, r);       // p = r exp(), with the row's factor
         if (codes != nullptr) {
             if (pick >= 0 && pick < K) atomicAdd(&s_cnt[(int)pick], 1u);

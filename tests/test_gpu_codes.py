@@ -208,6 +208,16 @@ def test_balance_rows_that_share_a_wave(kind, K):
     check_balance(s[:1200:3], torch.randint(-1, K, (400, 40), generator=g), None)      # more picks than lanes
 
 
+@pytest.mark.parametrize("K", (5, 100, 600, 1500, 3001, 8192))
+@pytest.mark.parametrize("offset", (9e5, -9e5, 999_000.0, 3e6, 3e33))
+def test_balance_scores_far_from_zero(offset, K):
+    # p depends on differences alone, which are exact here (scores of one binade; at 3e33 equal but for a code far below)
+    s = (torch.randn((33, K), generator=gen(K)) * 3 + offset).float()
+    s[:, 0] -= abs(offset) / 8
+    check_balance(s, torch.arange(33) % K, None)
+    check_balance(s, None, None)
+
+
 def test_balance_many_rows():
     g = gen(5)
     s = torch.randn((30011, 96), generator=g) * 2
