@@ -32,7 +32,7 @@ struct alignas(4 * sizeof(T)) Quad {
 };
 
 // The row's scores of one wave's lanes, -inf past column K: value 4c + i of lane t is column (64 c + t) * 4 + i, so ascending columns are chunk,
-// lane, i.  VEC: four scores in one access (aligned base and row stride, K % 4 == 0).
+// lane, i.  Four scores in one access; VEC: of aligned rows with K % 4 == 0, else of any, one by one where the row ends.
 template <typename T, int V, bool VEC>
 __device__ __forceinline__ void load_row(const T* __restrict__ row, int K, int t, float* v) {
 #pragma unroll
@@ -47,7 +47,17 @@ __device__ __forceinline__ void load_row(const T* __restrict__ row, int K, int t
             for (int i = 0; i < 4; ++i) v[4 * c + i] = score_to_f32<T>(q.v[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * c + i] = col + i < K ? score_to_f32<T>(row[col + i]) : -INFINITY;
+            for (int i = 0; i < 4; ++i) v[4 * c + i] = -INFINITY;
+            if (col + 4 <= K) {
+                Quad<T> q;
+                __builtin_memcpy(&q, row + col, sizeof(q));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[4 * c + i] = score_to_f32<T>(q.v[i]);
+            } else if (col < K) {
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    if (col + i < K) v[4 * c + i] = score_to_f32<T>(row[col + i]);
+            }
         }
     }
 }

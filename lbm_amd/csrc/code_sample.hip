@@ -529,8 +529,8 @@ struct Passes {       // S::request loads four scores that are in range, S::conv
     }
 };
 
-// VEC: four scores in one access (aligned row, n % 4 == 0); MASK: codes that may not be drawn.  (Both at compile time: a branch round a load
-// makes the compiler wait for it there, and one access was on its way at a time.)
+// VEC: accesses of four scores are aligned and the row ends with one (n % 4 == 0); MASK: codes that may not be drawn.  (Both at compile time: a
+// branch round a load makes the compiler wait for it there, and one access was on its way at a time.)
 template <typename T, bool VEC, bool MASK>
 struct Memory : Passes<Memory<T, VEC, MASK>> {
     const T* row;
@@ -544,12 +544,8 @@ struct Memory : Passes<Memory<T, VEC, MASK>> {
     using Four = lbm::Quad<T>;
     __device__ __forceinline__ Four request(int col) const {
         Four q;
-        if constexpr (VEC) {
-            q = *reinterpret_cast<const Four*>(row + col);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) q.v[i] = row[col + i];
-        }
+        if constexpr (VEC) q = *reinterpret_cast<const Four*>(row + col);
+        else __builtin_memcpy(&q, row + col, sizeof(q));
         return q;
     }
     __device__ __forceinline__ void convert(const Four& q, int col, float* f) const {
@@ -572,17 +568,18 @@ struct Memory : Passes<Memory<T, VEC, MASK>> {
             for (int i = 0; i < 4; ++i) f[i] = allowed[col + i] == 0 ? -INFINITY : f[i];
         }
     }
-    __device__ __forceinline__ void four(int col, float* f) const {       // -inf past the row's end
-        if constexpr (VEC) {
-            if (col < n) {
-                convert(request(col), col, f);
-            } else {
+    // -inf past the row's end, where the last four scores are read and moved up (there are four: rows here have more than 1024)
+    __device__ __forceinline__ void four(int col, float* f) const {
+        const int at = col + 4 <= n ? col : n - 4, by = col - at;
+        float q[4];
+        convert(request(at), at, q);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) f[i] = -INFINITY;
+        for (int i = 0; i < 4; ++i) {
+            f[i] = by == 0 ? q[i] : -INFINITY;
+            if constexpr (!VEC) {
+#pragma unroll
+                for (int k = 1; i + k < 4; ++k) f[i] = by == k ? q[i + k] : f[i];
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = col + i < n ? one(col + i) : -INFINITY;
         }
     }
 };
