@@ -13,7 +13,8 @@
 // 64-bit evaluation's but where a border is met to 1e-15.
 //
 // Borders are found without sorting: a border is a score, and how many scores (what weight) lie at or above a trial score is one pass over the
-// row's registers.  Trial scores halve the interval by value, then, for scores that lie too close together or are equal, by ordered bit
+// row.  Rows in registers cut the range of scores into 64 parts at a time and sum each in LDS (384000 x 512: top-k 100 586 -> 463 us, with
+// top-p 580, against halving); longer rows halve it by trial scores.  Scores that lie too close together or are equal are left to ordered bit
 // patterns.  The search for top-p sums fp32 copies of the weights (a third of the instructions); the score it ends at is then checked with
 // the 64-bit sums and moved where they disagree.
 #include "code_rows.h"
@@ -173,27 +174,72 @@ __device__ __forceinline__ float trial(int it, float lo, float hi) {
     return key_score(kl + (kh - kl + 1u) / 2);
 }
 
+// Where the sum over descending scores of [lo, m], lo < m, reaches `goal`: the range is cut into 64 equal parts, the parts' sums are taken in
+// LDS (h[64], the wave's own) and added up over the lanes, and the part in which the goal is reached is cut again, three times at most or
+// until it holds one score.  A level costs about three trial scores and does the work of six.  *lowest, *highest: the last part's scores;
+// *upto: the sum with all of them.  Parts are monotone in the score whatever rounds, so only sums that round (A = float) can mislead.
+template <typename A, int V, typename Weight>
+__device__ __forceinline__ int narrow(const Row<V>& R, float lo, float m, A goal, A* h, Weight weight, float* lowest, float* highest, A* upto) {
+    const int lane = R.lane();
+    const float scale = 64.f / (0.5f * m - 0.5f * lo);
+    float part[V];                       // < 0: not in it
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[i] = R.v[i] >= lo ? fminf(fmaxf((0.5f * m - 0.5f * R.v[i]) * scale, 0.f), 63.9999f) : -1.f;
+    A base = A(0);
+    int n = 0;
+    for (int level = 0; level < 3; ++level) {
+        h[lane] = A(0);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (part[i] >= 0.f) atomicAdd(&h[(int)part[i]], weight(i));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const A mine = h[lane];
+        const A sum = lbm::wave_scan<A>(mine, A(0), lbm::OpAdd());
+        const unsigned long long full = __ballot(mine > A(0)), over = __ballot(base + sum >= goal) & full;
+        const int at = over != 0 ? __ffsll((long long)over) - 1 : 63 - __clzll((long long)full);
+        *upto = base + lbm::lane_value(sum, at);
+        base = at == 0 ? base : base + lbm::lane_value(sum, at - 1);
+        n = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const bool in = part[i] >= 0.f && (int)part[i] == at;
+            part[i] = in ? fminf((part[i] - (float)at) * 64.f, 63.9999f) : -1.f;
+            n += __popcll(__ballot(in));
+        }
+        if (n == 1) break;
+    }
+    float hi = -INFINITY, low = INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        hi = fmaxf(hi, part[i] >= 0.f ? R.v[i] : -INFINITY);
+        low = fminf(low, part[i] >= 0.f ? R.v[i] : INFINITY);
+    }
+    *highest = lbm::wave_best(hi);
+    *lowest = n == 1 ? *highest : -lbm::wave_best(-low);
+    return n;
+}
+
 // the k best scores stay; lo: a score at or below all of them, m: the best one
 template <int V>
-__device__ __forceinline__ void keep_top_k(Row<V>& R, float lo, float m, int k) {
-    float hi = m;                        // the border is one of the scores in [lo, hi]
+__device__ __forceinline__ void keep_top_k(Row<V>& R, float lo, float m, int k, int* h) {
     int c = 0;
-    for (int it = 0; it < kSteps && lo < hi; ++it) {
-        const float mid = it == 0 ? hi : trial(it, lo, hi);
-        c = R.count_from(mid);
-        if (c >= k) lo = mid;
-        else hi = it < kByValue ? mid : R.next_below(mid);
-        if (c == k || (it == 0 && c >= k)) break;
-        if (it >= kByValue - 1) {        // from here on between scores that are there: equal ones end the search
-            hi = it == kByValue - 1 ? R.next_below(hi) : hi;
-            lo = R.next_from(lo);
+    if (lo < m) {
+        float low, hi;                   // the border is one of the scores in [low, hi]
+        narrow<int>(R, lo, m, k, h, [](int) { return 1; }, &low, &hi, &c);
+        lo = low;
+        if (c != k) {
+            for (int it = kByValue; it < kSteps && lo < hi; ++it) {       // between scores that are there: equal ones end the search
+                const float mid = trial(it, lo, hi);
+                if (R.count_from(mid) >= k) lo = R.next_from(mid);
+                else hi = R.next_below(mid);
+            }
+            c = R.count_from(lo);
         }
+    } else {
+        c = R.count_from(lo);
     }
-    if (c != k) c = R.count_from(lo);
-    if (c > k) {
-        lo = R.next_from(lo);
-        R.keep_first_equal(lo, k - (c - R.count_equal(lo)));
-    }
+    if (c > k) R.keep_first_equal(lo, k - (c - R.count_equal(lo)));
     R.drop_below(lo);
 }
 
@@ -205,27 +251,14 @@ __device__ __forceinline__ float top_p_floor(float m, float lo, double temp, dou
 
 // the codes of the smallest descending prefix that reaches `target` stay; the scores >= lo reach it, lo <= m
 template <int V>
-__device__ __forceinline__ void keep_top_p(Row<V>& R, float lo, float m, double target, double c) {
+__device__ __forceinline__ void keep_top_p(Row<V>& R, float lo, float m, double target, double c, float* h) {
     float wf[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) wf[i] = (float)R.w[i];
-    float l = lo, hi = m, b = m;         // the target is reached at l and not at hi
-    int n_hi;
-    if (R.probe(wf, m, &n_hi) < (float)target) {
-        for (int it = 0; it < kByValue; ++it) {
-            const float mid = trial(it, l, hi);
-            if (mid >= hi) break;
-            int n;
-            if (R.probe(wf, mid, &n) >= (float)target) {
-                l = mid;
-                if (n - n_hi == 1) break;
-            } else {
-                hi = mid;
-                n_hi = n;
-            }
-        }
-        b = R.next_below(hi);
-        l = R.next_from(l);
+    float b = m;
+    if (target > 1.0 && lo < m) {        // the best score alone weighs 1
+        float l, up;
+        narrow<float>(R, lo, m, (float)target, h, [&](int i) { return wf[i]; }, &l, &b, &up);
         for (int it = kByValue; it < kSteps && l < b; ++it) {     // between scores that are there: equal ones end the search
             const float mid = trial(it, l, b);
             int n;
@@ -254,7 +287,7 @@ __device__ __forceinline__ void keep_top_p(Row<V>& R, float lo, float m, double 
         }
     }
     if (!settled) {                      // fp32 sums led too far astray (a border among weights below 1e-7 of the total): search on the 64-bit sums
-        l = R.next_from(lo);
+        float l = R.next_from(lo);
         b = m;
         for (int it = 0; it < kSteps && l < b; ++it) {
             const float mid = trial(it, l, b);
@@ -339,10 +372,10 @@ __device__ __forceinline__ Setting row_setting(const Params& par, const float* u
 }
 
 // everything behind the best score m; lo: a score at or below all others; total: the weight that top-p refers to where the scores here are
-// not all of them (negative: they are).  -1: they do not reach top-p's share of that total.
+// not all of them (negative: they are); h: 64 words of LDS, the wave's own.  -1: they do not reach top-p's share of that total.
 template <int V>
-__device__ __forceinline__ int settle(Row<V>& R, const Setting& s, float lo, float m, int K, double total) {
-    if (s.by_k) keep_top_k<V>(R, lo, m, s.top_k);
+__device__ __forceinline__ int settle(Row<V>& R, const Setting& s, float lo, float m, int K, double total, float* h) {
+    if (s.by_k) keep_top_k<V>(R, lo, m, s.top_k, reinterpret_cast<int*>(h));
     R.weigh(m, s.c);
     if (s.by_p) {
         const double here = R.weight();
@@ -353,7 +386,7 @@ __device__ __forceinline__ int settle(Row<V>& R, const Setting& s, float lo, flo
             const double keep = ceil(target);
             R.keep_first_equal(m, keep < 1.0 ? 1 : (int)keep);
         } else {
-            keep_top_p<V>(R, top_p_floor(m, lo, s.temp, s.top_p, K), m, target, s.c);
+            keep_top_p<V>(R, top_p_floor(m, lo, s.temp, s.top_p, K), m, target, s.c, h);
         }
     }
     if (s.min_p > 0.0) {
@@ -369,16 +402,28 @@ template <typename T, int V, bool VEC>
 __global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ scores, int64_t lds, const float* __restrict__ u,
                                                           Params par, const uint8_t* __restrict__ allowed, int64_t allowed_ld,
                                                           int64_t* __restrict__ out, int64_t N, int K) {
-    // one value per wave, and the compiler is told so: branches on a row's settings are the scalar unit's (604 -> 586 us at 384000 x 512, top-k 100)
+    // one value per wave, and the compiler is told so: branches on a row's settings are the scalar unit's (3 % at 384000 x 512, top-k 100)
     const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ float s_part[4][64];
     if (row >= N) return;                // a whole wave
     Row<V> R;
     lbm::load_row<T, V, VEC>(scores + row * lds, K, R.lane(), R.v);
     if (allowed != nullptr) {
         const uint8_t* a = allowed + row * allowed_ld;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            if (R.slot(i) < K && a[R.slot(i)] == 0) R.v[i] = -INFINITY;
+        for (int c = 0; c < V / 4; ++c) {
+            const int col = R.slot(4 * c);
+            uint8_t q[4] = {0, 0, 0, 0};
+            if (col + 4 <= K) {
+                __builtin_memcpy(q, a + col, 4);
+            } else if (col < K) {
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    if (col + i < K) q[i] = a[col + i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) R.v[4 * c + i] = q[i] == 0 ? -INFINITY : R.v[4 * c + i];
+        }
     }
     const Setting s = row_setting(par, u, row, K);
     float m = -INFINITY, lo = INFINITY;
@@ -399,7 +444,7 @@ __global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ 
         hit = lbm::wave_first(first);
     } else {
         if (s.by_k || s.by_p) lo = -lbm::wave_best(-lo);
-        hit = settle<V>(R, s, lo, m, K, -1.0);
+        hit = settle<V>(R, s, lo, m, K, -1.0, s_part[threadIdx.x >> 6]);
     }
     if (R.lane() == 0) out[row] = hit;
 }
@@ -605,7 +650,7 @@ struct Taken : Passes<Taken> {
 
 // the draw by passes; lo, m: lowest and best score; total as for settle (-1 likewise); below: top-p's border is known to lie below this score
 template <typename S>
-__device__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, int K, double total, float below) {
+__device__ __forceinline__ int draw_by_passes(const S& R, const Setting& s, float lo, float m, int K, double total, float below) {
     int above, equal;
     if (m == INFINITY) {                 // equal weights of 1
         R.counts(m, &above, &equal);
@@ -768,6 +813,7 @@ __global__ __launch_bounds__(256, 3) void code_sample_long_kernel(const T* __res
                                                                int64_t* __restrict__ out, int64_t N, int K) {
     __shared__ __align__(16) float s_val[4][kCand];
     __shared__ unsigned short s_col[4][kCand], s_four[4][kCand];
+    __shared__ float s_part[4][64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + wave;
     if (row >= N) return;                // a whole wave
@@ -885,7 +931,7 @@ __global__ __launch_bounds__(256, 3) void code_sample_long_kernel(const T* __res
                             Q.v[i] = in ? val[Row<V>::slot(i)] : -INFINITY;
                             lo = fminf(lo, in ? Q.v[i] : INFINITY);
                         }
-                        at = settle<V>(Q, s, -lbm::wave_best(-lo), m, K, total);
+                        at = settle<V>(Q, s, -lbm::wave_best(-lo), m, K, total, s_part[wave]);
                     } else {
                         Taken Q;
                         Q.val = val;

@@ -433,6 +433,27 @@ def test_sample_masks_and_extremes():
         assert (check_sample(s, u, allowed=torch.zeros((K,), dtype=torch.bool)) == -1).all()
 
 
+@pytest.mark.parametrize("K", [60, 256, 511, 1000])
+def test_sample_short_rows_of_every_shape(K):
+    # borders that halving and cutting the range of scores do not find soon: clusters, outliers, scores spaced as powers
+    g = gen(40 + K)
+    base = torch.randn((K,), generator=g)
+    s = torch.stack([
+        -torch.exp(torch.linspace(-30, 6, K))[torch.randperm(K, generator=g)],      # dense at the best score
+        torch.exp(torch.linspace(-30, 3, K))[torch.randperm(K, generator=g)],       # dense at the lowest
+        torch.where(torch.arange(K) == 7, torch.tensor(-1e30), base * 1e-3),        # one far below the others
+        torch.where(torch.arange(K) == 7, torch.tensor(40.0), base * 1e-3),         # one far above
+        5.0 + torch.arange(K) % 3 * 2.0 ** -21,                                     # three neighbouring floats
+        torch.where(torch.arange(K) % 2 == 0, torch.tensor(3e38), torch.tensor(-3e38)) * (1 + base.abs() * 1e-2).clamp(max=1.1),
+        base * 1e-42,
+        base.sign() * torch.exp(base * 3),
+    ])
+    u = torch.rand((8,), generator=g)
+    for kw in SETTINGS + [dict(top_k=K // 2), dict(top_k=K - 1), dict(top_p=0.5), dict(top_p=0.999), dict(top_p=0.3, temperature=30.0),
+                          dict(top_k=K // 3, top_p=0.7, temperature=5.0)]:
+        check_sample(s, u, **kw)
+
+
 @pytest.mark.parametrize("K", [1500, 8192])
 def test_sample_long_rows_of_every_shape(K):
     """Rows whose order or spread misleads a look at a few of their scores."""
