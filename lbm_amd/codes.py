@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Union
 
 import torch
 
@@ -200,11 +200,12 @@ def code_balance_loss(scores: torch.Tensor, codes: torch.Tensor = None, keep: to
 # ------------------------------------------------------------------------------------------------------------- sampling
 @dataclass
 class CodeSampling:
-    """Settings of a draw (``sample_codes``), for ``VQVAE.encode(sampling=...)``.  The temperature is that of ``exp(-distance / T)``."""
-    temperature: float = 1.0
-    top_k: int = 0
-    top_p: float = 1.0
-    min_p: float = 0.0
+    """Settings of a draw (``sample_codes``), for ``VQVAE.encode(sampling=...)``.  The temperature is that of ``exp(-distance / T)``.
+    Each is a number or a tensor with one per code position [B, L//4]; ``allowed``: bool [K] or [B, L//4, K]."""
+    temperature: Union[float, torch.Tensor] = 1.0
+    top_k: Union[int, torch.Tensor] = 0
+    top_p: Union[float, torch.Tensor] = 1.0
+    min_p: Union[float, torch.Tensor] = 0.0
     allowed: Optional[torch.Tensor] = None
 
 

@@ -16,6 +16,8 @@ from . import _lib
 from .codes import CodeSampling, code_balance_loss, code_logits, sample_codes
 from .constants import VQ_EMBEDDING_DIM
 
+_SCORES_AT_A_TIME = 1 << 26      # scores that VQVAE.encode(sampling=...) holds at once
+
 
 # ------------------------------------------------------------------------------------------ functional layer
 @_lib.on_tensor_device
@@ -477,7 +479,7 @@ class VQVAE(nn.Module):
         return remap_codes(idx, cmap, kp, hist_s, hist)
 
     def _sampled_indices(self, h, cb, e_sqnorm, sampling, u, generator, hist):
-        """Codes drawn for h[B, D, S], a run of epochs at a time so that their scores (at most 256 MiB) stay in the last-level cache."""
+        """Codes drawn for h[B, D, S], a run of epochs at a time so that their scores (256 MiB, or one epoch's) stay in the last-level cache."""
         B, _, S = h.shape
         K = cb.shape[0]
         if u is None:
@@ -485,11 +487,18 @@ class VQVAE(nn.Module):
         elif tuple(u.shape) != (B, S):
             raise ValueError(f"u must be [{B}, {S}], got {tuple(u.shape)}")
         out = torch.empty((B, S), dtype=torch.int64, device=h.device)
-        step = max(1, (1 << 26) // max(1, S * K))
+        for name in ("temperature", "top_k", "top_p", "min_p", "allowed"):
+            v = getattr(sampling, name)
+            if isinstance(v, torch.Tensor) and v.dim() > 1 and v.shape[0] != B:
+                raise ValueError(f"sampling: {name} must have one entry per code position of {B} epochs, got {tuple(v.shape)}")
+        step = max(1, _SCORES_AT_A_TIME // max(1, S * K))
         for b in range(0, B, step):
+            def part(v):        # settings and masks that come per position
+                return v[b:b + step] if isinstance(v, torch.Tensor) and v.dim() > 1 else v
             scores = code_logits(h[b:b + step], cb, e_sqnorm=e_sqnorm, channel_major=True)
-            out[b:b + step] = sample_codes(scores.view(-1, S, K), u[b:b + step], temperature=sampling.temperature, top_k=sampling.top_k,
-                                           top_p=sampling.top_p, min_p=sampling.min_p, allowed=sampling.allowed, hist=hist)
+            out[b:b + step] = sample_codes(scores.view(-1, S, K), u[b:b + step], temperature=part(sampling.temperature),
+                                           top_k=part(sampling.top_k), top_p=part(sampling.top_p), min_p=part(sampling.min_p),
+                                           allowed=part(sampling.allowed), hist=hist)
         return out
 
     @torch.no_grad()

@@ -669,6 +669,24 @@ def test_encode_with_sampling(shipped, fold):
             m.encode(x, fold_projection=fold, **kw)
 
 
+def test_encode_with_settings_per_position_in_runs_of_epochs(shipped, monkeypatch):
+    import lbm_amd.quantizer as quantizer
+    m = _model(shipped).eval()
+    x = torch.randn((5, 30, 200), generator=gen(11)).to(DEV)
+    B, S = m.encode(x).shape
+    g = gen(12)
+    set_ = lbm_amd.CodeSampling(temperature=(torch.rand((B, S), generator=g) + 0.2).to(DEV), top_k=torch.randint(0, 40, (B, S), generator=g).to(DEV),
+                                top_p=(0.5 + 0.5 * torch.rand((B, S), generator=g)).to(DEV), min_p=(0.05 * torch.rand((B, S), generator=g)).to(DEV),
+                                allowed=(torch.rand((B, S, 512), generator=g) < 0.8).to(DEV))
+    u = torch.rand((B, S), generator=g).to(DEV)
+    whole = m.encode(x, sampling=set_, u=u)
+    monkeypatch.setattr(quantizer, "_SCORES_AT_A_TIME", 2 * S * 512)
+    assert torch.equal(m.encode(x, sampling=set_, u=u), whole)
+    assert set_.allowed.gather(2, whole[..., None]).all()
+    with pytest.raises(ValueError):
+        m.encode(x[:4], sampling=set_, u=u[:4])
+
+
 def test_encode_data_for_transformer_with_sampling(shipped):
     m = _model(shipped)
     data = [(torch.randn((2, 30, 100), generator=gen(i)), torch.tensor([i, i])) for i in range(3)]
