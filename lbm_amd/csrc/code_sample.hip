@@ -159,6 +159,12 @@ struct Row {
         for (int i = 0; i < V; ++i) s += w[i];
         return lbm::wave_total(s);
     }
+    __device__ __forceinline__ int first_of(float x) const {      // lowest slot of a score that is there
+        int first = 0x7fffffff;
+#pragma unroll
+        for (int i = V - 1; i >= 0; --i) first = v[i] == x ? slot(i) : first;
+        return lbm::wave_first(first);
+    }
 };
 
 constexpr int kByValue = 10;             // trial scores that halve by value; then by ordered bit pattern, which 32 end whatever the scores
@@ -249,14 +255,14 @@ __device__ __forceinline__ float top_p_floor(float m, float lo, double temp, dou
     return f > (double)lo && f < (double)m ? (float)f : lo;
 }
 
-// the codes of the smallest descending prefix that reaches `target` stay; the scores >= lo reach it, lo <= m
+// the codes of the smallest descending prefix that reaches `target` > 1 stay; the scores >= lo reach it, lo <= m
 template <int V>
 __device__ __forceinline__ void keep_top_p(Row<V>& R, float lo, float m, double target, double c, float* h) {
     float wf[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) wf[i] = (float)R.w[i];
     float b = m;
-    if (target > 1.0 && lo < m) {        // the best score alone weighs 1
+    if (lo < m) {
         float l, up;
         narrow<float>(R, lo, m, (float)target, h, [&](int i) { return wf[i]; }, &l, &b, &up);
         for (int it = kByValue; it < kSteps && l < b; ++it) {     // between scores that are there: equal ones end the search
@@ -365,6 +371,7 @@ __device__ __forceinline__ Setting row_setting(const Params& par, const float* u
     s.top_p = par.p_row != nullptr ? (double)par.p_row[row] : par.top_p;
     s.min_p = par.min_row != nullptr ? (double)par.min_row[row] : par.min_p;
     s.top_k = par.k_row != nullptr ? par.k_row[row] : par.top_k;
+    if (s.top_k == 1) s.temp = 0.0;      // the best code
     s.u = (double)u[row];
     s.by_k = s.top_k > 0 && s.top_k < K;
     s.by_p = s.top_p < 1.0;
@@ -375,6 +382,22 @@ __device__ __forceinline__ Setting row_setting(const Params& par, const float* u
 // not all of them (negative: they are); h: 64 words of LDS, the wave's own.  -1: they do not reach top-p's share of that total.
 template <int V>
 __device__ __forceinline__ int settle(Row<V>& R, const Setting& s, float lo, float m, int K, double total, float* h) {
+    if (s.by_p && m < INFINITY) {
+        // Where top-p's share of all weight is less than the best code's 1, that code is all that stays (top-k only takes weight away).  On
+        // fp32 weights: w errs by 1.3e-7 |log2 w| w, where |log2 w| w <= 0.54, and their sum by 2^-20 of itself, together less than 10^-4 at
+        // 1024 codes.  Peaked rows, as a trained codebook gives, end here: 384000 x 512, top-p 0.9 374 -> 153 us, with top-k and min-p
+        // 580 -> 152; flat ones pay 3 %.
+        float all = 0.f;
+        if (total < 0.0) {
+            const float c = (float)s.c;
+#pragma unroll
+            for (int i = 0; i < V; ++i) all += __builtin_amdgcn_exp2f((R.v[i] - m) * c);
+            all = lbm::wave_total(all);
+        } else {
+            all = (float)total;
+        }
+        if (s.top_p * all < 0.999) return R.first_of(m);
+    }
     if (s.by_k) keep_top_k<V>(R, lo, m, s.top_k, reinterpret_cast<int*>(h));
     R.weigh(m, s.c);
     if (s.by_p) {
@@ -382,9 +405,10 @@ __device__ __forceinline__ int settle(Row<V>& R, const Setting& s, float lo, flo
         if (total < 0.0) total = here;
         const double target = s.top_p * total;
         if (here < target) return -1;
+        if (target <= 1.0) return R.first_of(m);
         if (m == INFINITY) {             // equal weights of 1
             const double keep = ceil(target);
-            R.keep_first_equal(m, keep < 1.0 ? 1 : (int)keep);
+            R.keep_first_equal(m, (int)keep);
         } else {
             keep_top_p<V>(R, top_p_floor(m, lo, s.temp, s.top_p, K), m, target, s.c, h);
         }
@@ -438,10 +462,7 @@ __global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ 
     if (m == -INFINITY) {
         hit = -1;
     } else if (!(s.temp > 0.0)) {
-        int first = 0x7fffffff;
-#pragma unroll
-        for (int i = V - 1; i >= 0; --i) first = R.v[i] == m ? R.slot(i) : first;
-        hit = lbm::wave_first(first);
+        hit = R.first_of(m);
     } else {
         if (s.by_k || s.by_p) lo = -lbm::wave_best(-lo);
         hit = settle<V>(R, s, lo, m, K, -1.0, s_part[threadIdx.x >> 6]);

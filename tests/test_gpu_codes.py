@@ -454,6 +454,29 @@ def test_sample_short_rows_of_every_shape(K):
         check_sample(s, u, **kw)
 
 
+@pytest.mark.parametrize("K", [2, 64, 512, 1024, 5000])
+def test_sample_nucleus_round_the_best_code(K):
+    # top-p's share of the total lies just below, at and above the best code's weight of 1
+    s = torch.full((60, K), -300.0)
+    g = gen(50 + K)
+    at = torch.randint(0, K, (60,), generator=g)
+    s[torch.arange(60), at] = 0.0
+    second = (at + 1 + torch.randint(0, K - 1, (60,), generator=g)) % K
+    s[torch.arange(60), second] = -3.0 * torch.rand((60,), generator=g)
+    s[40:, : K // 2] = torch.maximum(s[40:, : K // 2], -4.0 - torch.rand((20, K // 2), generator=g))
+    s[::7] += 17.0
+    u = torch.rand((60,), generator=g)
+    u[:20] = 0.999
+    w = np.exp(f64(s) - f64(s).max(1, keepdims=True)).sum(1)
+    for n in range(60):
+        for d in (-1e-2, -1.1e-3, -9e-4, -1e-5, -1e-9, 1e-9, 1e-5, 1e-3):
+            p = min((1.0 + d) / w[n], 1.0)
+            check_sample(s[n:n + 1], u[n:n + 1], top_p=p)
+            check_sample(s[n:n + 1], u[n:n + 1], top_p=p, top_k=2)
+    check_sample(s, u, top_p=torch.from_numpy(1.0 / w).float())
+    check_sample(s, u, top_k=torch.randint(0, 3, (60,), generator=g))
+
+
 @pytest.mark.parametrize("K", [1500, 8192])
 def test_sample_long_rows_of_every_shape(K):
     """Rows whose order or spread misleads a look at a few of their scores."""
