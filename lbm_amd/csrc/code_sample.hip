@@ -524,6 +524,14 @@ struct Passes {       // S::request loads four scores that are in range, S::conv
         *above = lbm::wave_total(a);
         *equal = lbm::wave_total(e);
     }
+    __device__ __forceinline__ double weight_of_all(float m, double c) const {
+        double s = 0.0;
+        each_raw([&](const float* q, int) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s += exp2_f64(((double)q[i] - (double)m) * c);
+        });
+        return lbm::wave_total(s);
+    }
     __device__ double weight_above(float x, float m, double c) const {
         double s = 0.0;
         each([&](const float* q, int) {
@@ -692,7 +700,7 @@ __device__ __forceinline__ int draw_by_passes(const S& R, const Setting& s, floa
     }
     double here = 0.0;
     if (s.by_p) {
-        here = R.weight_above(b, m, s.c) + (b == -INFINITY ? 0.0 : keep * weight(b));
+        here = b == -INFINITY ? R.weight_of_all(m, s.c) : R.weight_above(b, m, s.c) + keep * weight(b);
         const double target = s.top_p * (total < 0.0 ? here : total);
         if (here < target) return -1;
         const float l = fmaxf(b == -INFINITY ? lo : b, top_p_floor(m, lo, s.temp, s.top_p, K));
@@ -936,9 +944,9 @@ __global__ __launch_bounds__(256, 3) void code_sample_long_kernel(const T* __res
                 if (p_alone && total < 0.0) {
                     // all weight: on fp32 weights where that shows that the best code fills top-p's share (as in settle, whose bound grows
                     // with the codes), else by a pass of 64-bit ones.  40000 x 8192 fp16, top-p 0.9: peaked rows 380 -> 257 us against 64
-                    // bits at once; rows spread over tens of codes pay 3 (8192 codes) to 20 % (1500).
+                    // bits at once; rows spread over tens of codes 524 -> 509 at 48828 x 4096, 687 -> 775 at 133333 x 1500.
                     const float all = lbm::wave_total(sum) * __builtin_amdgcn_exp2f((ref - m) * cf);
-                    total = s.top_p * all < 0.999 - 1e-7 * K ? (double)all : S.weight_above(-INFINITY, m, s.c);
+                    total = s.top_p * all < 0.999 - 1e-7 * K ? (double)all : S.weight_of_all(m, s.c);
                 }
                 // min-p alone: everything it leaves must have been taken
                 const bool all = s.by_k || s.by_p || t == kLowest || exp2_f64(((double)t - (double)m) * s.c) < fmin(s.min_p, 1.0);
