@@ -768,6 +768,19 @@ __device__ __forceinline__ int draw_by_passes(const S& R, const Setting& s, floa
         const double least = lim;
         auto group = [&](int g) {        // the lanes' sums of group g
             double w = 0.0;
+            if (b == -INFINITY && least == 0.0 && g * 2048 + 2048 <= R.n) {       // everything: loads at once, no comparisons
+                typename S::Four at_once[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) at_once[i] = R.request(g * 2048 + i * 256 + R.lane() * 4);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float q[4];
+                    R.convert_raw(at_once[i], g * 2048 + i * 256 + R.lane() * 4, q);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w += weight(q[j]);
+                }
+                return lbm::wave_total(w);
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int c = g * 2048 + i * 256 + R.lane() * 4;
