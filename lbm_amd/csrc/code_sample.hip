@@ -421,7 +421,8 @@ __device__ __forceinline__ int settle(Row<V>& R, const Setting& s, float lo, flo
     return draw<V>(R, s.u);
 }
 
-// K <= 64 V: the whole row in registers
+// K <= 64 V: the whole row in registers, a wave to a row.  384000 x 512 fp32: greedy 128 us and top-p of peaked rows 150 (5.2 TB/s), then vector
+// instructions bound it: no filter 257 (64-bit exponentials), top-k 100 454, flat nucleus 350.
 template <typename T, int V, bool VEC>
 __global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ scores, int64_t lds, const float* __restrict__ u,
                                                           Params par, const uint8_t* __restrict__ allowed, int64_t allowed_ld,
@@ -472,10 +473,11 @@ __global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ 
 
 // ---- longer rows: one wave still, which reads the row in chunks of 256 and keeps only what can be drawn.
 //
-// 512 samples of the row give a score t that a few hundred scores reach; one pass takes the best score, the total weight where top-p asks for
-// it, and the scores >= t with their columns into LDS, where they are a short row again: up to 512 in registers (8 a lane), up to kCand by
+// 512 samples of the row give a score t that a few hundred scores reach; one pass takes the best score, the total fp32 weight where top-p
+// asks for it, and the scores >= t with their columns into LDS, where they are a short row again: up to 512 in registers (8 a lane), up to kCand by
 // passes over LDS.  The pass is repeated with a corrected t where too many or too few came, and a row whose nucleus does not fit (or that has
-// no filter at all) is answered by the same passes over memory.  No barrier anywhere: rows do not wait for each other.
+// no filter at all) is answered by the same passes over memory.  No barrier anywhere: rows do not wait for each other.  40000 x 8192 fp16: greedy
+// 125 us (5.2 TB/s), top-k 100 256, top-p 0.9 257, no filter 439, a nucleus of thousands 2.6 ms; a single wave's time for one row is 5 to 20 us.
 constexpr int kReg = 512, kCand = 1536;
 
 // passes over scores of a row, in memory or taken into LDS
