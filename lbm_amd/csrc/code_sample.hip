@@ -477,7 +477,8 @@ __global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ 
 // asks for it, and the scores >= t with their columns into LDS, where they are a short row again: up to 512 in registers (8 a lane), up to kCand by
 // passes over LDS.  The pass is repeated with a corrected t where too many or too few came, and a row whose nucleus does not fit (or that has
 // no filter at all) is answered by the same passes over memory.  No barrier anywhere: rows do not wait for each other.  40000 x 8192 fp16: greedy
-// 125 us (5.2 TB/s), top-k 100 256, top-p 0.9 257, no filter 439, a nucleus of thousands 2.6 ms; a single wave's time for one row is 5 to 20 us.
+// 125 us (5.2 TB/s), top-k 100 256, top-p 0.9 257, no filter 439, a nucleus of thousands 2.6 ms; one row alone 5 to 37 us, 115 such a
+// nucleus.
 constexpr int kReg = 512, kCand = 1536;
 
 // passes over scores of a row, in memory or taken into LDS
