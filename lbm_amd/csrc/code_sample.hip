@@ -961,8 +961,12 @@ __global__ __launch_bounds__(256, 3) void code_sample_long_kernel(const T* __res
                     // all weight: on fp32 weights where that shows that the best code fills top-p's share (as in settle, whose bound grows
                     // with the codes), else by a pass of 64-bit ones.  40000 x 8192 fp16, top-p 0.9: peaked rows 380 -> 257 us against 64
                     // bits at once; rows spread over tens of codes 524 -> 509 at 48828 x 4096, 687 -> 775 at 133333 x 1500.
-                    const float all = lbm::wave_total(sum) * __builtin_amdgcn_exp2f((ref - m) * cf);
-                    total = s.top_p * all < 0.999 - 1e-7 * K ? (double)all : S.weight_of_all(m, s.c);
+                    // The fp32 sum is relative to the best sample.  A best code 2^120 above that (NaN: no finite sample, or a temperature
+                    // whose reciprocal is no float) is left to the 64-bit pass: the factor that brings the sum back to it falls below the
+                    // smallest normal float, where the exponential gives 0, before the sum overflows.
+                    const float up = (m - ref) * cf;
+                    const float all = lbm::wave_total(sum) * __builtin_amdgcn_exp2f(-up);
+                    total = up < 120.f && s.top_p * all < 0.999 - 1e-7 * K ? (double)all : S.weight_of_all(m, s.c);
                 }
                 // min-p alone: everything it leaves must have been taken
                 const bool all = s.by_k || s.by_p || t == kLowest || exp2_f64(((double)t - (double)m) * s.c) < fmin(s.min_p, 1.0);
