@@ -18,6 +18,11 @@ from . import _lib
 
 
 # --------------------------------------------------------------------------------------------------------------- scores
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[N, M] with unit stride along M and rows that do not overlap."""
+    return t.contiguous() if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]) else t
+
+
 class _CodeLogits(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, codebook, e_sqnorm, temperature):
@@ -38,14 +43,13 @@ class _CodeLogits(torch.autograd.Function):
         need_x, need_e = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         N, D = x.shape
         K = codebook.shape[0]
-        if g.stride(1) != 1 or (N > 1 and g.stride(0) < K):
-            g = g.contiguous()
+        g, x, codebook = _rows(g), _rows(x), codebook.contiguous()       # (saved tensors come back in any layout from hooks that offload them)
         lib = _lib.load()
         dx = torch.empty((N, D), dtype=torch.float32, device=x.device) if need_x else None
         de = torch.empty((K, D), dtype=torch.float32, device=x.device) if need_e else None
         ws = torch.empty((lib.lbm_code_logits_grad_workspace_bytes(N, D, K),), dtype=torch.uint8, device=x.device)
-        _lib.check(lib.lbm_code_logits_grad_f32(_lib.ptr(g), g.stride(0) if N > 1 else K, x.data_ptr(), x.stride(0) if N > 1 else D,
-                                                codebook.data_ptr(), dx.data_ptr() if need_x else None, de.data_ptr() if need_e else None,
+        _lib.check(lib.lbm_code_logits_grad_f32(_lib.ptr(g), g.stride(0) if N > 1 else K, _lib.ptr(x), x.stride(0) if N > 1 else D,
+                                                _lib.ptr(codebook), dx.data_ptr() if need_x else None, de.data_ptr() if need_e else None,
                                                 int(ctx.norm_grad), ws.data_ptr(), N, D, K, ctx.temperature,
                                                 _lib.stream_ptr()), "lbm_code_logits_grad_f32")
         return dx, de, None, None
@@ -100,9 +104,7 @@ def code_logits(x: torch.Tensor, codebook: torch.Tensor, temperature: float = 1.
                                                            _lib.ptr(cb), _lib.ptr(ee), _lib.ptr(out), K, B * S, D, K, temperature,
                                                            _lib.stream_ptr()), "lbm_code_logits_f32")
             return out
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < D):
-        x = x.contiguous()
-    return _CodeLogits.apply(x, cb, ee, temperature)
+    return _CodeLogits.apply(_rows(x), cb, ee, temperature)
 
 
 # -------------------------------------------------------------------------------------------------------------- balance
@@ -142,7 +144,6 @@ class _CodeBalance(torch.autograd.Function):
                                         None if keep is None else keep.data_ptr(), loss.data_ptr(), counts.data_ptr(), mean.data_ptr(),
                                         at + 16, at, ws.data_ptr(), N, K, _lib.stream_ptr()), "lbm_code_balance")
         ctx.save_for_backward(scores, saved, counts)
-        ctx.ld = ld
         ctx.mark_non_differentiable(counts)
         ctx.set_materialize_grads(False)
         return loss, counts, mean
@@ -151,12 +152,14 @@ class _CodeBalance(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, _g_counts, g_mean):
         scores, saved, counts = ctx.saved_tensors
+        # hooks that offload saved tensors bring them back in any layout
+        (scores, ld), saved, counts = _score_rows(scores, "code_balance_loss"), saved.contiguous(), counts.contiguous()
         N, K = scores.shape
         ds = torch.empty((N, K), dtype=scores.dtype, device=scores.device)
         if g_mean is not None:
             g_mean = g_mean.contiguous()
         at = saved.data_ptr()
-        _lib.check(_lib.load().lbm_code_balance_grad(_lib.ptr(scores), _lib.SCORE_TYPES[scores.dtype], ctx.ld, at + 16, counts.data_ptr(), at,
+        _lib.check(_lib.load().lbm_code_balance_grad(_lib.ptr(scores), _lib.SCORE_TYPES[scores.dtype], ld, at + 16, counts.data_ptr(), at,
                                                      None if g_loss is None else g_loss.data_ptr(),
                                                      None if g_mean is None else g_mean.data_ptr(), ds.data_ptr(), N, K, _lib.stream_ptr()),
                    "lbm_code_balance_grad")

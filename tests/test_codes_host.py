@@ -135,3 +135,50 @@ def test_python_surface_refuses_cpu_tensors():
             call()
     with pytest.raises(NotImplementedError, match="8192"):
         lbm_amd.code_balance_loss(torch.zeros((1, 8193)))
+
+
+class _Recorder:
+    """Stands for the library: every call succeeds and is written down, nothing is touched."""
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.calls.append((name, args))
+            return 64 if name.endswith("_bytes") else 0
+        return call
+
+
+@pytest.mark.parametrize("op", ["balance", "logits"])
+@pytest.mark.parametrize("wide", [False, True])
+def test_backward_addresses_saved_tensors_as_they_come_back(monkeypatch, op, wide):
+    """Saved tensors may come back in another layout than they went (offloading to host memory makes them dense, a hook may also spread
+    them): the backward pass goes by the strides they have then."""
+    rec = _Recorder()
+    monkeypatch.setattr(_lib, "load", lambda: rec)
+    monkeypatch.setattr(_lib, "ptr", lambda t: None if t is None else t.data_ptr())
+    monkeypatch.setattr(_lib, "stream_ptr", lambda: 0)
+    monkeypatch.setattr(_lib, "dev_f32", lambda t, device=None: t.float().contiguous())
+    N, K, D = 6, 16, 16
+    back = []
+
+    def unpack(t):
+        if t.dtype == torch.float32 and t.dim() == 2:
+            t = torch.zeros((t.shape[0], 4 * t.shape[1]))[:, ::4] if wide else t.clone(memory_format=torch.contiguous_format)
+        back.append(t)
+        return t
+    x = torch.zeros((N, 100))[:, 3:3 + K].requires_grad_()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        if op == "balance":
+            out = lbm_amd.code_balance_loss(x)[0]
+        else:
+            out = lbm_amd.code_logits(x, torch.zeros((K, D)).requires_grad_()).sum()
+    out.backward()
+    name, args = rec.calls[-1]
+    stride, pointers = (args[2], args[:1]) if op == "balance" else (args[3], (args[2], args[4]))
+    assert name == ("lbm_code_balance_grad" if op == "balance" else "lbm_code_logits_grad_f32")
+    assert stride == K
+    if not wide:
+        assert set(pointers) <= {t.data_ptr() for t in back}
+    else:
+        assert not set(pointers) & {t.data_ptr() for t in back}      # dense copies of rows whose scores are not neighbours

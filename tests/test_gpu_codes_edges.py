@@ -1,5 +1,7 @@
 """The code-score operators on the GPU where scores, operands and sizes go to their ends: best codes far above a row's other scores, operands
 near the largest float, more rows or gradient entries than one launch holds.  Plain 64-bit evaluations and tolerances as in test_gpu_codes."""
+import contextlib
+
 import numpy as np
 import pytest
 import torch
@@ -41,3 +43,24 @@ def test_sample_nucleus_of_best_codes_far_above_the_rest(K, T, kind):
                 # more, on each of the two evaluations: 16 2^-53 of the total in all.  u moved by that much to either side brackets it.
                 lo, hi = (sample64(f64(st), f64(ut) + d, np.full(n, T), np.zeros(n, int), np.full(n, p), np.zeros(n)) for d in (-2.0 ** -49, 2.0 ** -49))
                 assert ((got == lo) | (got == hi)).all(), (best, u, p, got, lo, hi)
+
+
+# ------------------------------------------------------------------------------------------------------------- gradients
+@pytest.mark.parametrize("kind", sorted(TYPES))
+def test_gradients_with_saved_tensors_offloaded(kind):
+    """Saved tensors that went to host memory come back dense: gradients are those without, bit for bit, whatever the scores' row stride was."""
+    g = gen(31)
+    wide = torch.randn((90, 700), generator=g).to(TYPES[kind]).to(DEV)
+    codes = torch.randint(0, 130, (90,), generator=g).to(DEV)
+    e = torch.randn((70, 130), generator=g).to(DEV).requires_grad_()
+    gm, gs = torch.randn((130,), generator=g).to(DEV), torch.randn((90, 70), generator=g).to(DEV)
+    for at in (0, 3):
+        results = []
+        for offload in (False, True):
+            s = wide[:, at:at + 130].detach().requires_grad_()
+            with torch.autograd.graph.save_on_cpu() if offload else contextlib.nullcontext():
+                loss, _, mean = lbm_amd.code_balance_loss(s, codes)
+                out = lbm_amd.code_logits(s.float(), e, 0.5)
+            results.append(torch.autograd.grad((loss, mean), s, (torch.ones((), device=DEV), gm)) + torch.autograd.grad(out, (s, e), gs))
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
