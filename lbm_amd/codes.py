@@ -72,6 +72,7 @@ def code_logits(x: torch.Tensor, codebook: torch.Tensor, temperature: float = 1.
     those of the distances.  ``x``: [N, D] rows (any row stride), or with ``channel_major`` the encoder output z[B, D, S] (N = B*S rows, row
     n = (n // S, n % S), no permute copy).  Differentiable in ``x`` and ``codebook``; with ``channel_major`` and a gradient to take, the
     rows are copied first.  ``e_sqnorm`` ([K], as ``fold_projection`` returns it) takes the place of |e_k|^2 as a constant.
+    Values of 3.396e38 and more in magnitude, infinities among them, give NaN wherever they enter.
 
     The backward pass reads ``x`` and ``codebook`` as they are then: hand it a copy of a codebook that an EMA step rewrites in between
     (``vq_ema_apply`` writes through raw pointers, which autograd's version check does not see)."""

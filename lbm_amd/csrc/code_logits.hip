@@ -10,7 +10,8 @@
 // Products: every fp32 operand is cut into three bf16 pieces, each the nearest bf16 of what is left (the remainders are exact, the three
 // hold 24 bits and more), and a product keeps six terms of the nine, accumulated in fp32 on v_mfma_f32_32x32x16_bf16; the three left out lie
 // below 2^-26 of it.  That is as exact as a chain of fp32 products (7.5e-8 of the scores' size against 64 bits either way) at 16/6 of the fp32
-// matrix rate.  An infinity among the inputs makes NaN of what it enters (inf - inf in its remainder).
+// matrix rate.  An operand whose nearest bf16 is an infinity (0x1.ffp127 = 3.396e38 and more) makes NaN of what it enters: inf - inf among
+// its pieces.  (Clamping the first piece would let finite ones through; two instructions per pair of values: 40000 x 8192 x 256 1067 -> 1094 us.)
 //
 // Bound: the matrix pipe and the power it draws; an output element costs 12 D FLOP of bf16 products for 4 bytes of store.  That is also why
 // the scores are stored at all: forming them a second time for the gradient costs more than writing and reading them.

@@ -64,3 +64,39 @@ def test_gradients_with_saved_tensors_offloaded(kind):
             results.append(torch.autograd.grad((loss, mean), s, (torch.ones((), device=DEV), gm)) + torch.autograd.grad(out, (s, e), gs))
         for a, b in zip(*results):
             assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------------------------------------------- scores
+@pytest.mark.parametrize("D,K,N", [(1, 3, 5), (64, 96, 70), (65, 97, 130), (256, 512, 1000)])
+def test_logits_of_operands_near_the_largest_float(D, K, N):
+    """Operands up to the last float that rounds to a finite bf16 number give what the formula gives; the next one, the largest float and an
+    infinity give NaN in their own row or column and nowhere else."""
+    last = float(np.uint32(0x7f7f7fff).view(np.float32))
+    g = gen(D)
+    x, e = torch.randn((N, D), generator=g) * 1e-3, torch.randn((K, D), generator=g) * 1e-3
+    x[::3, D // 2], x[1::3, 0] = last, -last
+    w = torch.randn((N, K), generator=g) * 1e-3
+    w[N // 2, K // 2] = -last
+    xd, ed = x.to(DEV).requires_grad_(), e.to(DEV).requires_grad_()
+    s = lbm_amd.code_logits(xd, ed, 0.5)
+    x64, e64, w64 = f64(x), f64(e), f64(w)
+    assert (np.abs(f64(s) - logits64(x64, e64, 0.5)) <= logits_tol(x64, e64, 0.5)).all()
+    (dx,) = torch.autograd.grad(s, xd, w.to(DEV))
+    assert (np.abs(f64(dx) - 4 * w64 @ e64) <= U * (K + 8) * 4 * (np.abs(w64) @ np.abs(e64)) + 1e-37).all()
+    for value in (float(np.uint32(0x7f7f8000).view(np.float32)), -torch.finfo(torch.float32).max, float("inf")):
+        for channel_major in (False, True):
+            a, b = x.clone(), e.clone()
+            a[N - 2, D - 1], b[K - 2, 0] = value, value
+            a = (a.t()[None] if channel_major else a).contiguous()
+            t = lbm_amd.code_logits(a.to(DEV), b.to(DEV), 0.5, channel_major=channel_major).cpu()
+            other = torch.ones((N, K), dtype=torch.bool)
+            other[N - 2] = other[:, K - 2] = False
+            assert torch.isnan(t[~other]).all()
+            assert (np.abs(f64(t) - logits64(x64, e64, 0.5))[other] <= logits_tol(x64, e64, 0.5)[other]).all()
+        v = torch.randn((N, K), generator=g)
+        v[N - 2, K - 1] = value
+        y = x.clamp(-1, 1)
+        yd = y.to(DEV).requires_grad_()
+        dx, de = (t.cpu() for t in torch.autograd.grad(lbm_amd.code_logits(yd, ed, 0.5), (yd, ed), v.to(DEV)))
+        assert torch.isnan(dx[N - 2]).all() and torch.isfinite(dx[torch.arange(N) != N - 2]).all()
+        assert torch.isnan(de[K - 1]).all() and torch.isfinite(de[:K - 1]).all()
