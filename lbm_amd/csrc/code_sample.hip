@@ -1035,20 +1035,35 @@ __global__ __launch_bounds__(256, 3) void code_sample_long_kernel(const T* __res
     if (lane == 0) out[row] = hit;
 }
 
+constexpr int64_t kLaunchRows = 1 << 25;       // a launch holds fewer than 2^32 threads; a wave works on a row
+
 template <typename T>
-int run_sample(const void* scores, int64_t lds, const float* u, const Params& par, const uint8_t* allowed, int64_t allowed_ld, int64_t* out,
-               int64_t N, int K, hipStream_t st) {
+int run_sample(const void* scores, int64_t lds, const float* u, Params par, const uint8_t* allowed, int64_t allowed_ld, int64_t* out, int64_t N,
+               int K, hipStream_t st) {
     const T* s = static_cast<const T*>(scores);
     const bool vec = ((uintptr_t)scores % (4 * sizeof(T))) == 0 && (lds & 3) == 0 && (K & 3) == 0;
-    const dim3 grid((unsigned)((N + 3) / 4)), block(256);
-#define LBM_SAMPLE(kernel) hipLaunchKernelGGL((kernel), grid, block, 0, st, s, lds, u, par, allowed, allowed_ld, out, N, K)
-    if (K <= 256) LBM_SAMPLE((vec ? code_sample_kernel<T, 4, true> : code_sample_kernel<T, 4, false>));
-    else if (K <= 512) LBM_SAMPLE((vec ? code_sample_kernel<T, 8, true> : code_sample_kernel<T, 8, false>));
-    else if (K <= 1024) LBM_SAMPLE((vec ? code_sample_kernel<T, 16, true> : code_sample_kernel<T, 16, false>));
-    else if (allowed == nullptr) LBM_SAMPLE((vec ? code_sample_long_kernel<T, true, false> : code_sample_long_kernel<T, false, false>));
-    else LBM_SAMPLE((vec ? code_sample_long_kernel<T, true, true> : code_sample_long_kernel<T, false, true>));
+    for (;;) {
+        const int64_t n = N < kLaunchRows ? N : kLaunchRows;
+        const dim3 grid((unsigned)((n + 3) / 4)), block(256);
+#define LBM_SAMPLE(kernel) hipLaunchKernelGGL((kernel), grid, block, 0, st, s, lds, u, par, allowed, allowed_ld, out, n, K)
+        if (K <= 256) LBM_SAMPLE((vec ? code_sample_kernel<T, 4, true> : code_sample_kernel<T, 4, false>));
+        else if (K <= 512) LBM_SAMPLE((vec ? code_sample_kernel<T, 8, true> : code_sample_kernel<T, 8, false>));
+        else if (K <= 1024) LBM_SAMPLE((vec ? code_sample_kernel<T, 16, true> : code_sample_kernel<T, 16, false>));
+        else if (allowed == nullptr) LBM_SAMPLE((vec ? code_sample_long_kernel<T, true, false> : code_sample_long_kernel<T, false, false>));
+        else LBM_SAMPLE((vec ? code_sample_long_kernel<T, true, true> : code_sample_long_kernel<T, false, true>));
 #undef LBM_SAMPLE
-    return lbm::check_launch("lbm_code_sample");
+        const int rc = lbm::check_launch("lbm_code_sample");
+        if (rc != LBM_OK || n == N) return rc;
+        s += n * lds;
+        u += n;
+        out += n;
+        if (allowed != nullptr) allowed += n * allowed_ld;
+        if (par.T_row != nullptr) par.T_row += n;
+        if (par.k_row != nullptr) par.k_row += n;
+        if (par.p_row != nullptr) par.p_row += n;
+        if (par.min_row != nullptr) par.min_row += n;
+        N -= n;
+    }
 }
 
 constexpr int kMaxK = 1 << 24;

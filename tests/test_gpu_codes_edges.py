@@ -100,3 +100,22 @@ def test_logits_of_operands_near_the_largest_float(D, K, N):
         dx, de = (t.cpu() for t in torch.autograd.grad(lbm_amd.code_logits(yd, ed, 0.5), (yd, ed), v.to(DEV)))
         assert torch.isnan(dx[N - 2]).all() and torch.isfinite(dx[torch.arange(N) != N - 2]).all()
         assert torch.isnan(de[K - 1]).all() and torch.isfinite(de[:K - 1]).all()
+
+
+# ---------------------------------------------------------------------------------------------------------- large extents
+def test_sample_more_rows_than_one_launch_holds():
+    """Row counts whose waves are more than 2^32 threads: every row is answered, with its own settings, mask and number."""
+    if torch.cuda.get_device_properties(0).total_memory < 20e9:
+        pytest.skip("needs 8 GB of device memory")
+    N = (1 << 26) + 1001
+    g = torch.Generator(device=DEV).manual_seed(1)
+    s = torch.randn((N, 3), generator=g, device=DEV, dtype=torch.bfloat16)
+    u = torch.rand((N,), generator=g, device=DEV)
+    allowed = torch.rand((N, 3), generator=g, device=DEV) < 0.7
+    k = torch.randint(0, 3, (N,), generator=g, device=DEV, dtype=torch.int32)
+    hist = torch.zeros((3,), dtype=torch.int64, device=DEV)
+    got = lbm_amd.sample_codes(s, u, top_k=k, allowed=allowed, hist=hist)
+    for a in (0, 1 << 25, N // 2, (1 << 26) - 5, N - 1001):
+        b = slice(a, a + 1001)
+        assert torch.equal(got[b], lbm_amd.sample_codes(s[b], u[b], top_k=k[b], allowed=allowed[b]))
+    assert torch.equal(hist, torch.stack([(got == i).sum() for i in range(3)]))
