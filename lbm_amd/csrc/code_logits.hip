@@ -379,8 +379,8 @@ __global__ __launch_bounds__(kThreads, 2) void code_mm_kernel(Operand a, Operand
 template <bool NORM>
 __global__ __launch_bounds__(256) void code_grad_join_kernel(const float* __restrict__ part, const float* __restrict__ rowsum,
                                                              const float* __restrict__ codebook, float* __restrict__ out, int splits,
-                                                             int64_t M, int64_t D, float scale) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = M * D;
+                                                             int64_t M, int64_t D, float scale, int64_t first) {
+    const int64_t i = first + (int64_t)blockIdx.x * 256 + threadIdx.x, n = M * D;
     if (i >= n) return;
     const int64_t m = NORM ? i / D : 0;
     double s = 0.0, c = 0.0;
@@ -405,10 +405,15 @@ __global__ __launch_bounds__(256) void code_grad_join_kernel(const float* __rest
 template <bool NORM>
 int launch_join(const char* what, const float* part, const float* rowsum, const float* codebook, float* out, int splits, int64_t M, int64_t D,
                 float scale, hipStream_t st) {
-    const int64_t blocks = (M * D + 255) / 256;
-    if (blocks > 0x7fffffffLL) return lbm::fail(LBM_EUNSUPPORTED, "%s: gradient too large", what);
-    hipLaunchKernelGGL((code_grad_join_kernel<NORM>), dim3((unsigned)blocks), dim3(256), 0, st, part, rowsum, codebook, out, splits, M, D, scale);
-    return lbm::check_launch(what);
+    constexpr int64_t kEntries = 1LL << 31;               // a launch holds fewer than 2^32 threads
+    for (int64_t first = 0; first < M * D; first += kEntries) {
+        const int64_t n = M * D - first < kEntries ? M * D - first : kEntries;
+        hipLaunchKernelGGL((code_grad_join_kernel<NORM>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, part, rowsum, codebook, out,
+                           splits, M, D, scale, first);
+        const int rc = lbm::check_launch(what);
+        if (rc != LBM_OK) return rc;
+    }
+    return LBM_OK;
 }
 
 bool aligned16(const float* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }

@@ -119,3 +119,34 @@ def test_sample_more_rows_than_one_launch_holds():
         b = slice(a, a + 1001)
         assert torch.equal(got[b], lbm_amd.sample_codes(s[b], u[b], top_k=k[b], allowed=allowed[b]))
     assert torch.equal(hist, torch.stack([(got == i).sum() for i in range(3)]))
+
+
+def test_logits_gradients_of_more_entries_than_one_launch_holds():
+    """Gradients of more than 2^32 entries that are joined from pieces."""
+    if torch.cuda.get_device_properties(0).total_memory < 120e9:
+        pytest.skip("needs 70 GB of device memory")
+    D, n, m = 8192, (1 << 19) + 1000, 3
+    g = torch.Generator(device=DEV).manual_seed(1)
+    big = torch.empty((n, D), device=DEV).normal_(generator=g)
+    w = torch.randn((m, n), generator=g, device=DEV)
+    small = torch.randn((m, D), generator=g, device=DEV)
+
+    def close(got, rows, want, mag, steps):
+        assert ((got[rows].double() - want).abs() <= U * (steps + 16) * mag + 1e-37).all()
+    rows = torch.tensor([0, 1, 77, (1 << 19) - 1, 1 << 19, n - 2, n - 1], device=DEV)
+    # the codebook's gradient
+    e = big.requires_grad_()
+    (de,) = torch.autograd.grad(lbm_amd.code_logits(small, e, 1.0), e, w)
+    wr = w[:, rows].double().t().contiguous()
+    er, c = big.detach()[rows].double(), wr.sum(1)[:, None]
+    close(de, rows, 2 * (torch.mm(wr, small.double()) - c * er), 2 * (torch.mm(wr.abs(), small.double().abs()) + wr.abs().sum(1)[:, None] * er.abs()), m)
+
+    # the rows' gradient: the codes in more than one piece
+    del de, e
+    x, cb = big.detach().requires_grad_(), torch.randn((4100, D), generator=g, device=DEV)
+    w = torch.zeros((n, 4100), device=DEV)
+    w[rows] = torch.randn((7, 4100), generator=g, device=DEV)
+    (dx,) = torch.autograd.grad(lbm_amd.code_logits(x, cb, 1.0), x, w)
+    wr = w[rows].double()
+    close(dx, rows, 2 * torch.mm(wr, cb.double()), 2 * torch.mm(wr.abs(), cb.double().abs()), 4100)
+    assert not dx[2:70].any() and not dx[-90:-3].any()
