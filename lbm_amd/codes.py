@@ -241,7 +241,8 @@ def sample_codes(scores: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_
     ``top_p`` < 1 then keeps, in descending order, every code before which less than that share of the kept weight lies; ``min_p`` then keeps
     codes of at least that share of the best code's weight; the answer is the first index whose running sum exceeds u times the total.
     ``temperature`` 0 answers the best code, lowest index first.  Each setting is a number, or a tensor [...] with one per row (on the
-    device, unchecked: temperatures that are not positive mean 0, top_k <= 0 and top_p >= 1 mean all codes).
+    device, unchecked: temperatures that are not positive mean 0, top_k <= 0 and top_p >= 1 mean all codes).  ``u`` and settings per row
+    are taken as float32.
 
     ``scores``: float32, float16 or bfloat16.  ``allowed``: bool [K] or [..., K], codes that may be drawn.  Scores of +inf share all
     the weight, NaN counts as -inf; a row with nothing to draw from answers -1.  ``hist`` ([K] int64, K <= 32768) is ADDED to when given."""
@@ -251,6 +252,8 @@ def sample_codes(scores: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_
     dev = s.device
     if not isinstance(u, torch.Tensor) or not u.is_floating_point() or tuple(u.shape) != lead:
         raise ValueError(f"sample_codes: u must be a floating-point tensor of shape {lead}")
+    if u.dtype is torch.float64:
+        u = torch.where(u < 1.0, u.clamp(max=1.0 - 2.0 ** -24), u)        # numbers below 1 stay there when they are rounded to fp32
     u = u.to(device=dev, dtype=torch.float32).contiguous()
     t_row, t = _setting(temperature, "temperature", lead, dev, torch.float32, 0.0, math.inf)
     k_row, k = _setting(top_k, "top_k", lead, dev, torch.int32, 0, math.inf)

@@ -45,6 +45,19 @@ def test_sample_nucleus_of_best_codes_far_above_the_rest(K, T, kind):
                 assert ((got == lo) | (got == hi)).all(), (best, u, p, got, lo, hi)
 
 
+def test_sample_numbers_in_64_bits_stay_below_one():
+    """Numbers of [0, 1) that round to 1 in fp32 are the last fp32 number below it: the code that a share of 1 - 2^-24 falls on, not a code
+    without weight to speak of behind it."""
+    for K in (2, 700, 5000):
+        s = torch.full((4, K), float("-inf"))
+        s[:, 0], s[:, K - 1] = 0.0, -100.0
+        u = torch.tensor([1 - 1e-9, 1 - 2.0 ** -53, 0.25, 1.0], dtype=torch.float64)
+        for kw in (dict(), dict(top_k=2), dict(top_p=0.999999999999)):
+            got = lbm_amd.sample_codes(s.to(DEV), u.to(DEV), **kw).tolist()
+            assert got[:3] == [0, 0, 0]
+        assert lbm_amd.sample_codes(s.to(DEV), u.to(DEV)).tolist()[3] == K - 1       # 1 itself: the last code that stayed
+
+
 # ------------------------------------------------------------------------------------------------------------- gradients
 @pytest.mark.parametrize("kind", sorted(TYPES))
 def test_gradients_with_saved_tensors_offloaded(kind):
