@@ -390,7 +390,7 @@ int lbm_perplexity_u64(const unsigned long long* hist, float* out, int32_t K, lb
  * lbm_code_logits_f32: logits[n*ldl + k] = (2 x_n . e_k - |e_k|^2) / temperature -- minus the squared distance over the temperature
  *   without the row constant |x_n|^2 / temperature.  x, ldx, layout (LBM_VQ_ROWS or LBM_VQ_CHANNEL_MAJOR), S as for lbm_vq_argmin_f32;
  *   any D >= 1, K >= 1, any 4-byte alignment; e_sqnorm_or_null [K]: taken instead of |e_k|^2 (folded codebooks).
- *   temperature positive and finite.
+ *   temperature positive and finite, 2 / temperature below the largest float.
  *   Operands (x, codebook, and g below) of 3.396e38 and more in magnitude, infinities among them, give NaN wherever they enter.
  * lbm_code_logits_grad_f32: gradients of a loss with dL/dlogits = g [N, K] (row stride ldg): dx [N, D] = (2 / temperature) g E and
  *   de [K, D] = (2 / temperature) (g^T x - diag(column sums of g) E); norm_grad = 0 leaves the second term out (e_sqnorm was given as a

@@ -77,8 +77,8 @@ def code_logits(x: torch.Tensor, codebook: torch.Tensor, temperature: float = 1.
     The backward pass reads ``x`` and ``codebook`` as they are then: hand it a copy of a codebook that an EMA step rewrites in between
     (``vq_ema_apply`` writes through raw pointers, which autograd's version check does not see)."""
     temperature = float(temperature)
-    if not (temperature > 0.0 and math.isfinite(temperature)):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not (temperature > 0.0 and math.isfinite(temperature) and 2.0 / temperature <= torch.finfo(torch.float32).max):
+        raise ValueError(f"temperature must be positive and finite, and 2 / temperature in float32 too, got {temperature}")
     x, cb = _f32_param(x, "x"), _f32_param(codebook, "codebook").contiguous()
     if cb.dim() != 2 or cb.numel() == 0:
         raise ValueError("codebook must be a non-empty [K, D] tensor")

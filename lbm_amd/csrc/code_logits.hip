@@ -416,6 +416,9 @@ int launch_join(const char* what, const float* part, const float* rowsum, const 
     return LBM_OK;
 }
 
+// 2 / T is a finite float, and 1 / T
+bool usable(double temperature) { return temperature > 0.0 && temperature < INFINITY && 2.0 / temperature <= 0x1.fffffep127; }
+
 bool aligned16(const float* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && (ld & 3) == 0; }
 
 template <int TM, int TN, int AM, int BM, int EPI>
@@ -479,7 +482,7 @@ extern "C" int lbm_code_logits_f32(const float* x, int64_t ldx, int32_t layout, 
                                    double temperature, lbm_stream_t stream) {
     const char* what = "lbm_code_logits_f32";
     LBM_REQUIRE(N >= 0 && D >= 1 && K >= 1, LBM_EINVAL, "%s: bad sizes (N=%lld D=%d K=%d)", what, (long long)N, D, K);
-    LBM_REQUIRE(temperature > 0.0 && temperature < INFINITY, LBM_EINVAL, "%s: temperature must be positive and finite", what);
+    LBM_REQUIRE(usable(temperature), LBM_EINVAL, "%s: temperature must be positive and finite, and 2 / temperature too", what);
     LBM_REQUIRE(layout == LBM_VQ_ROWS || layout == LBM_VQ_CHANNEL_MAJOR, LBM_EINVAL, "%s: unknown layout %d", what, layout);
     if (N == 0) return LBM_OK;
     LBM_REQUIRE(x && codebook && logits, LBM_EINVAL, "%s: NULL pointer", what);
@@ -519,7 +522,7 @@ extern "C" int lbm_code_logits_grad_f32(const float* g, int64_t ldg, const float
                                         double temperature, lbm_stream_t stream) {
     const char* what = "lbm_code_logits_grad_f32";
     LBM_REQUIRE(N >= 0 && D >= 1 && K >= 1, LBM_EINVAL, "%s: bad sizes (N=%lld D=%d K=%d)", what, (long long)N, D, K);
-    LBM_REQUIRE(temperature > 0.0 && temperature < INFINITY, LBM_EINVAL, "%s: temperature must be positive and finite", what);
+    LBM_REQUIRE(usable(temperature), LBM_EINVAL, "%s: temperature must be positive and finite, and 2 / temperature too", what);
     LBM_REQUIRE(codebook && (N == 0 || g), LBM_EINVAL, "%s: NULL pointer", what);
     LBM_REQUIRE(N == 0 || ldg >= K, LBM_EINVAL, "%s: ldg (%lld) < K (%d)", what, (long long)ldg, K);
     if (dx_or_null == nullptr && de_or_null == nullptr) return LBM_OK;

@@ -182,3 +182,15 @@ def test_backward_addresses_saved_tensors_as_they_come_back(monkeypatch, op, wid
         assert set(pointers) <= {t.data_ptr() for t in back}
     else:
         assert not set(pointers) & {t.data_ptr() for t in back}      # dense copies of rows whose scores are not neighbours
+
+
+@pytest.mark.parametrize("T", [1e-300, 5e-324, 1e-39, 2.0 / torch.finfo(torch.float32).max * (1 - 1e-12)])
+def test_temperatures_whose_reciprocal_is_no_float_are_refused(T):
+    assert _logits(T=T) == EINVAL and "2 / temperature" in _err()
+    assert _grad(T=T) == EINVAL and "2 / temperature" in _err()
+    with pytest.raises(ValueError, match="2 / temperature"):
+        lbm_amd.code_logits(S, S, temperature=T)
+
+
+def test_smallest_temperatures_are_taken():
+    assert _logits(T=6e-39, N=0) == 0 and _grad(T=6e-39, dx=None, de=None, x=None, ws=None) == 0
