@@ -580,6 +580,7 @@ extern "C" int lbm_code_balance_grad(const void* scores, int32_t dtype, int64_t 
     LBM_REQUIRE(dtype == LBM_F32 || dtype == LBM_F16 || dtype == LBM_BF16, LBM_EINVAL, "%s: unknown score type %d", what, dtype);
     if (N == 0) return LBM_OK;
     LBM_REQUIRE(scores && row_stat && counts && totals && dscores, LBM_EINVAL, "%s: NULL pointer", what);
+    LBM_REQUIRE(((uintptr_t)row_stat & 7) == 0, LBM_EINVAL, "%s: row_stat must be 8-byte aligned", what);
     LBM_REQUIRE(N <= 1 || lds >= 0, LBM_EINVAL, "%s: negative row stride", what);
     const int64_t T = 256 / lanes_for(K), cap = T >= 4 ? 2048 : (K <= 4096 ? 1024 : 512);
     int64_t G = (N + T - 1) / T;

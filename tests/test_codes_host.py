@@ -194,3 +194,7 @@ def test_temperatures_whose_reciprocal_is_no_float_are_refused(T):
 
 def test_smallest_temperatures_are_taken():
     assert _logits(T=6e-39, N=0) == 0 and _grad(T=6e-39, dx=None, de=None, x=None, ws=None) == 0
+
+
+def test_balance_grad_entry_refuses_unaligned_row_statistics():
+    assert _balance_grad(stat=P + 4) == EINVAL and "lbm_code_balance_grad: row_stat" in _err()
