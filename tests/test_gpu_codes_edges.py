@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import lbm_amd
-from tests.test_gpu_codes import DEV, TYPES, U, f64, gen, logits64, logits_tol, sample64
+from tests.test_gpu_codes import DEV, TYPES, U, _inputs, _step, f64, gen, logits64, logits_tol, sample64
 
 pytestmark = pytest.mark.gpu
 
@@ -163,3 +163,42 @@ def test_logits_gradients_of_more_entries_than_one_launch_holds():
     wr = w[rows].double()
     close(dx, rows, 2 * torch.mm(wr, cb.double()), 2 * torch.mm(wr.abs(), cb.double().abs()), 4100)
     assert not dx[2:70].any() and not dx[-90:-3].any()
+
+
+# ------------------------------------------------------------------------------------------------------ together, in training
+def test_chain_gradients_of_scores_of_ordinary_size():
+    """Scores -> drawn codes -> loss and entropy of the mean -> gradients, every entry within a bound from the operations: scores of a few units,
+    so that every code has a share of every row."""
+    T, N, D, K = 0.2, 700, 96, 130                      # those of _step and _inputs
+    x, e, u, keep = _inputs(5)
+    x, e = (x * 0.15).requires_grad_(), (e * 0.15).requires_grad_()
+    codes, loss, counts, mean, dx, de = _step(x, e, u, keep)
+    x64, e64, on = f64(x), f64(e), keep.cpu().numpy()
+    s = logits64(x64, e64, T)
+    p = np.exp(s - s.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    assert np.median(p.max(1)) < 0.5
+    M = on.sum()
+    f = np.bincount(codes.cpu().numpy()[on], minlength=K)
+    assert np.array_equal(counts.cpu().numpy(), f)
+    f = f / f.sum()
+    P = p[on].mean(0)
+    a = K * f + np.log(P + 1e-10) + P / (P + 1e-10)
+    ds = np.where(on[:, None], p * (a - (p * a).sum(1, keepdims=True)) / M, 0)
+    # relative error of a row's p: its scores' errors twice (its own and the sum's), then the exponential, the sum of 130 and the reciprocal;
+    # of P: the worst row's and the sum over the rows; of a: that of P in the logarithm (absolutely) and in P / P, and the roundings of its parts
+    r = 2 * logits_tol(x64, e64, T).max(1) + 64 * U
+    rP = r[on].max() + (N + 16) * U
+    ta = 3 * rP + 8 * U * (K * f + np.abs(np.log(P + 1e-10)) + 1)
+    assert (np.abs(f64(mean) - P) <= rP * P).all()
+    assert abs(float(loss) - K * (f * P).sum()) <= (rP + 4 * U) * K * (f * P).sum()
+    dev = np.abs(a - (p * a).sum(1, keepdims=True))
+    inner = (p * (r[:, None] * dev + ta)).sum(1, keepdims=True)      # of p.a (p's errors sum to nothing but rounding: a is taken from its mean)
+    tds = np.where(on[:, None], p * (r[:, None] * dev + ta + inner + 64 * U * np.abs(a).max()) / M, 0)
+    gx, ge = 2 / T * ds @ e64, 2 / T * (ds.T @ x64 - ds.sum(0)[:, None] * e64)
+    tx = 2 / T * (tds @ np.abs(e64) + U * (K + 8) * np.abs(ds) @ np.abs(e64))
+    mag = np.abs(ds).T @ np.abs(x64) + np.abs(ds).sum(0)[:, None] * np.abs(e64)
+    te = 2 / T * (tds.T @ np.abs(x64) + tds.sum(0)[:, None] * np.abs(e64) + U * (N + 16) * mag)
+    assert (np.abs(f64(dx) - gx) <= tx).all() and (np.abs(f64(de) - ge) <= te).all()
+    # what the bounds can tell apart: a twentieth of an ordinary entry
+    assert np.median(tx[on] / np.abs(gx[on]).clip(1e-30)) < 0.05 and np.median(te / np.abs(ge).clip(1e-30)) < 0.05
