@@ -325,7 +325,8 @@ def encoder_forward(x: torch.Tensor, enc: "nn.Sequential | dict", pitched_out: b
 class VectorQuantizerEMA(nn.Module):
     """The reference's quantizer.  ``balance_weight`` > 0 (not a reference argument) adds that many times the usage-balance loss
     (``code_balance_loss`` of the scores ``code_logits(z, codebook, balance_temperature)`` and the codes picked) to the loss in training mode:
-    its gradient pulls the encoder's outputs towards codes that are used too little.  The codebook itself goes on learning by EMA only."""
+    its gradient pulls the encoder's outputs towards codes that are used too little.  The codebook itself goes on learning by EMA only.
+    With ``ema_group`` set the EMA step sums all ranks' counts, the balance term takes this rank's rows and counts alone."""
     balance_weight, balance_temperature = 0.0, 1.0       # of modules pickled without them
 
     def __init__(self, num_embeddings, embedding_dim, commitment_cost, decay, epsilon=1e-5, balance_weight=0.0, balance_temperature=1.0):

@@ -202,3 +202,23 @@ def test_chain_gradients_of_scores_of_ordinary_size():
     assert (np.abs(f64(dx) - gx) <= tx).all() and (np.abs(f64(de) - ge) <= te).all()
     # what the bounds can tell apart: a twentieth of an ordinary entry
     assert np.median(tx[on] / np.abs(gx[on]).clip(1e-30)) < 0.05 and np.median(te / np.abs(ge).clip(1e-30)) < 0.05
+
+
+def test_balance_term_takes_this_ranks_rows_where_the_ema_step_is_summed_over_ranks(monkeypatch):
+    x = torch.randn((96, 16), generator=gen(1)).to(DEV)
+    results = []
+    for group in (None, "all"):
+        if group is not None:
+            monkeypatch.setattr(torch.distributed, "all_reduce", lambda t, group=None: t.mul_(3))     # two more ranks with the same rows
+        q = lbm_amd.VectorQuantizerEMA(24, 16, 0.25, 0.9, balance_weight=0.7, balance_temperature=0.5)
+        q.embedding.weight.data.normal_(generator=gen(2))
+        q.ema_w.data.copy_(q.embedding.weight.data)
+        q.ema_cluster_size.data.fill_(1.0)
+        q.ema_group = group
+        q = q.to(DEV).train()
+        xd = x.clone().requires_grad_()
+        loss, _, _, _ = q(xd)
+        loss.backward()
+        results.append((loss.detach(), xd.grad, q.embedding.weight.detach().clone()))
+    (l0, g0, w0), (l1, g1, w1) = results
+    assert torch.equal(l0, l1) and torch.equal(g0, g1) and not torch.equal(w0, w1)
