@@ -68,21 +68,16 @@ def build(force: bool = False, verbose: bool = False) -> str:
     obj_dir = os.path.join(HERE, "csrc", "_obj")
     os.makedirs(obj_dir, exist_ok=True)
     # packed fp32 instructions are left out: some of their forms have given wrong results (the bench runs as fast without: 757 - 763 k
-    # epochs/s against 756 - 759 k)
+    # epochs/s against 756 - 759 k).  The SLP vectorizer then pairs nothing: -fno-slp-vectorize, which kept the FFT and some MFMA kernels
+    # from pairs that cost more register moves than they saved, changes no instruction any more.
     flags = ["-O3", "-std=c++17", f"--offload-arch={ARCH}", "-fPIC", "-munsafe-fp-atomics", "-Wall", "-Wno-unused-function",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-    # The FFT kernels keep complex values as split re/im registers; the SLP vectorizer pairs them into packed-fp32 ops
-    # and pays for it with register moves (fir_fft_kernel: 384 v_mov per item, 16 B of scratch; 3.9 -> 3.2 ms without).
-    # Round 3: the same flag for three MFMA kernels whose side arithmetic hipcc had packed (v_pk_add_f32 beside MFMAs costs more than the
-    # two scalar adds, MI355X_MICROARCH.md): screening 4.756 -> 4.718 ms, affine_post 1.540 -> 1.523, the F(3,2) conv layers -0.4 % (A/B x2).
-    no_slp = {"fir_fft.hip", "welch.hip", "resample.hip", "vq_screen.hip", "conv_k4s2_wino_ws.hip", "affine_post.hip"}
     procs = []
     for src in sources():
         obj = os.path.join(obj_dir, os.path.basename(src)[:-4] + ".o")
         objs.append(obj)
-        extra = ["-fno-slp-vectorize"] if os.path.basename(src) in no_slp else []
-        if os.path.basename(src) == "vq.hip":   # 12.23 -> 12.04 ms on the quantizer (A/B x3); neutral on the conv kernels
-            extra += ["-mllvm", "-amdgpu-sched-strategy=max-ilp"]
+        # 12.23 -> 12.04 ms on the quantizer (A/B x3); neutral on the conv kernels
+        extra = ["-mllvm", "-amdgpu-sched-strategy=max-ilp"] if os.path.basename(src) == "vq.hip" else []
         cmd = [_hipcc(), *flags, *extra, "-Rpass-analysis=kernel-resource-usage", "-c", src, "-o", obj]
         if verbose:
             print(" ".join(cmd))
