@@ -9,9 +9,10 @@
 // sum and its use, the next row's load runs under that, and every thread adds p of its own columns over all rows it sees, so the column
 // sums cost no traffic until the end, where each workgroup leaves one partial row.  Partial sums are joined in a fixed order in 64 bits:
 // results do not change from run to run.  Up to 2048 codes a wave holds a row, or eight, four or two short ones (no barrier); above
-// that four waves share one and exchange their maxima and sums once per row (2048 codes in four waves: 398 us for 264 at 100000 rows of
-// bf16 with the gradient; 8192 in eight waves with half the registers each: 217 us for 172 at 40000 rows; 5 codes, a row to a wave: 653 us
-// for 108 at 1043158 rows of bf16 with the gradient).
+// that four waves share one and exchange their maxima and sums once per row (100000 rows with the gradient in four waves: 2048 codes 408 us
+// for 270 in bf16 and 551 for 514 in fp32, 1100 codes 375 for 301 in fp32; 2047 codes 413 for 367 in bf16, but 545 for 775 in fp32, where a
+// wave's registers spill; 8192 codes in eight waves with half the registers each: 217 us for 172 at 40000 rows; 5 codes, a row to a wave: 653
+// us for 108 at 1043158 rows of bf16 with the gradient).
 // The gradient takes a relative to its value at the row's best score: where one p is near 1 its a - p.a is a difference of near equals
 // otherwise, and loses what it should return.
 #include "code_rows.h"

@@ -13,8 +13,8 @@
 // 64-bit evaluation's but where a border is met to 1e-15.
 //
 // Borders are found without sorting: a border is a score, and how many scores (what weight) lie at or above a trial score is one pass over the
-// row.  Rows in registers cut the range of scores into 64 parts at a time and sum each in LDS (384000 x 512: top-k 100 586 -> 463 us, with
-// top-p 580, against halving); longer rows halve it by trial scores.  Scores that lie too close together or are equal are left to ordered bit
+// row.  Rows in registers cut the range of scores into 64 parts at a time and sum each in LDS (384000 x 512, top-k 100: 586 -> 463 us
+// against halving); longer rows halve it by trial scores.  Scores that lie too close together or are equal are left to ordered bit
 // patterns.  The search for top-p sums fp32 copies of the weights (a third of the instructions); the score it ends at is then checked with
 // the 64-bit sums and moved where they disagree.
 #include "code_rows.h"
@@ -385,8 +385,7 @@ __device__ __forceinline__ int settle(Row<V>& R, const Setting& s, float lo, flo
     if (s.by_p && m < INFINITY) {
         // Where top-p's share of all weight is less than the best code's 1, that code is all that stays (top-k only takes weight away).  On
         // fp32 weights: w errs by 1.3e-7 |log2 w| w, where |log2 w| w <= 0.54, and their sum by 2^-20 of itself, together less than 10^-4 at
-        // 1024 codes.  Peaked rows, as a trained codebook gives, end here: 384000 x 512, top-p 0.9 374 -> 153 us, with top-k and min-p
-        // 580 -> 152; flat ones pay 3 %.
+        // 1024 codes.  Peaked rows end here: 384000 x 512, top-p 0.9 374 -> 153 us, with top-k and min-p 580 -> 152; flat ones pay 3 %.
         float all = 0.f;
         if (total < 0.0) {
             const float c = (float)s.c;
@@ -421,8 +420,9 @@ __device__ __forceinline__ int settle(Row<V>& R, const Setting& s, float lo, flo
     return draw<V>(R, s.u);
 }
 
-// K <= 64 V: the whole row in registers, a wave to a row.  384000 x 512 fp32: greedy 128 us and top-p of peaked rows 150 (5.2 TB/s), then vector
-// instructions bound it: no filter 257 (64-bit exponentials), top-k 100 454, flat nucleus 350.
+// K <= 64 V: the whole row in registers, a wave to a row.  384000 x 512 fp32: greedy 122 - 134 us and top-p of peaked rows 150 - 180 (HBM), then
+// vector instructions and LDS atomics bound it: no filter 260 - 310 (64-bit exponentials), top-k 100 435 - 465, top-p 0.9 with a nucleus of 35 codes
+// 610, of hundreds 1040.
 template <typename T, int V, bool VEC>
 __global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ scores, int64_t lds, const float* __restrict__ u,
                                                           Params par, const uint8_t* __restrict__ allowed, int64_t allowed_ld,
@@ -477,8 +477,8 @@ __global__ __launch_bounds__(256) void code_sample_kernel(const T* __restrict__ 
 // asks for it, and the scores >= t with their columns into LDS, where they are a short row again: up to 512 in registers (8 a lane), up to kCand by
 // passes over LDS.  The pass is repeated with a corrected t where too many or too few came, and a row whose nucleus does not fit (or that has
 // no filter at all) is answered by the same passes over memory.  No barrier anywhere: rows do not wait for each other.  40000 x 8192 fp16: greedy
-// 125 us (5.2 TB/s), top-k 100 256, top-p 0.9 257, no filter 439, a nucleus of thousands 2.6 ms; one row alone 5 to 37 us, 115 such a
-// nucleus.
+// 117 - 133 us (HBM), top-k 100 250, top-p 0.9 of peaked rows 247 - 277, no filter 384 - 432, a nucleus of 400 codes 935, of thousands 3.3 ms; top-k
+// under a mask 520.  One row alone: 4 to 15 us, 42 where the nucleus has 480 codes, 107 - 119 thousands.
 constexpr int kReg = 512, kCand = 1536;
 
 // passes over scores of a row, in memory or taken into LDS

@@ -530,7 +530,7 @@ __global__ __launch_bounds__(64 * TS) __attribute__((amdgpu_waves_per_eu((TS == 
         }
         // ---- folded pruned DFT: this wave's k-steps of every tile.  Steps with 0 < n < Q on every lane ("fast": all but
         // t = 0 and t = QS - 1) run as ONE straight line of kTeamSteps steps from immediate LDS offsets -- no branches, no
-        // clamps, window and basis from registers, packed f32 arithmetic: the VALU port, not the MFMA pipe, was what the
+        // clamps, window and basis from registers, arithmetic on pairs: the VALU port, not the MFMA pipe, was what the
         // fold kernel saturated.  Steps of that line the wave does not own carry zero weights.  The two end steps take the
         // general form under a uniform branch.
         f32x4 accs[NTILES][4];   // [tile][re_e, im_e, re_o, im_o]

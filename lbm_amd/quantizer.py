@@ -480,7 +480,8 @@ class VQVAE(nn.Module):
         return remap_codes(idx, cmap, kp, hist_s, hist)
 
     def _sampled_indices(self, h, cb, e_sqnorm, sampling, u, generator, hist):
-        """Codes drawn for h[B, D, S], a run of epochs at a time so that their scores (256 MiB, or one epoch's) stay in the last-level cache."""
+        """Codes drawn for h[B, D, S], a run of epochs at a time, whose scores take 256 MiB or one epoch's (``encode`` of 1024 epochs of 375
+        codes out of 512: 2.9 ms; 3.9 with 16 MiB, 3.0 with 1 GiB)."""
         B, _, S = h.shape
         K = cb.shape[0]
         if u is None:
