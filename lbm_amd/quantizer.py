@@ -227,6 +227,10 @@ def _pitched_rows(x: torch.Tensor) -> torch.Tensor:
     """x[B, C, L] as the kernels address it: unit stride in L, one pitch between consecutive (b, c) rows.
     Contiguous tensors and the [..., :L] views of pitched buffers pass through; anything else is copied."""
     B, Cc, L = x.shape
+    if Cc == 1 and B > 1 and x.stride(1) != x.stride(0):       # the stride of a dimension of one is any number: the pitch is the epochs' distance
+        if x.stride(2) != 1 or x.stride(0) < L:
+            x = x.contiguous()
+        x = x.as_strided((B, 1, L), (x.stride(0), x.stride(0), 1))
     if x.stride(2) == 1 and (B == 1 or x.stride(0) == Cc * x.stride(1)) and (B * Cc == 1 or x.stride(1) >= L):
         return x
     return x.contiguous()

@@ -198,3 +198,19 @@ def test_smallest_temperatures_are_taken():
 
 def test_balance_grad_entry_refuses_unaligned_row_statistics():
     assert _balance_grad(stat=P + 4) == EINVAL and "lbm_code_balance_grad: row_stat" in _err()
+
+
+def test_pitch_of_a_single_channel_is_the_distance_of_the_epochs():
+    """[B, 1, L] views whose middle stride, of a dimension of one, is any number: the pitch the kernels are given stays inside the tensor."""
+    from lbm_amd.quantizer import _pitched_rows
+    base = torch.arange(1000.0)
+    for B, L in ((5, 7), (2, 1), (1, 6), (5, 8)):
+        for s0 in (L, L + 1, 8, 1, 0):
+            for s1 in (0, 1, L, B * L, 900):
+                x = torch.as_strided(base, (B, 1, L), (s0, s1, 1))
+                y = _pitched_rows(x)
+                assert torch.equal(x, y)
+                if B > 1:      # what conv1d, vq_argmin and code_logits hand over as the pitch
+                    assert y.stride(1) == y.stride(0) >= L and (L == 1 or y.stride(2) == 1)
+    y = _pitched_rows(base[:35].view(1, 5, 7).transpose(0, 1))
+    assert y.stride(1) == 7 and y.data_ptr() == base.data_ptr()

@@ -222,3 +222,17 @@ def test_balance_term_takes_this_ranks_rows_where_the_ema_step_is_summed_over_ra
         results.append((loss.detach(), xd.grad, q.embedding.weight.detach().clone()))
     (l0, g0, w0), (l1, g1, w1) = results
     assert torch.equal(l0, l1) and torch.equal(g0, g1) and not torch.equal(w0, w1)
+
+
+@pytest.mark.parametrize("B,S,K", [(5, 5, 3), (7, 130, 70), (300, 1, 33), (1, 9, 4)])
+def test_logits_channel_major_of_one_channel(B, S, K):
+    """One channel: the stride of that dimension is any number, here that of the whole tensor, of one element, of a wider row."""
+    g = gen(B)
+    z, e = torch.randn((B, 1, S), generator=g), torch.randn((K, 1), generator=g)
+    d = z.to(DEV)
+    wide = torch.zeros((B, 3, S + 5), device=DEV)
+    wide[:, 1:2, 2:2 + S] = d
+    want, tol = logits64(f64(z).reshape(-1, 1), f64(e), 0.5), logits_tol(f64(z).reshape(-1, 1), f64(e), 0.5)
+    for x in (d, d.view(1, B, S).transpose(0, 1), d.view(B, S, 1).permute(0, 2, 1), wide[:, 1:2, 2:2 + S], wide[:, 1:2, 2:2 + S].transpose(0, 1).contiguous().transpose(0, 1)):
+        assert torch.equal(x, d)
+        assert (np.abs(f64(lbm_amd.code_logits(x, e.to(DEV), 0.5, channel_major=True)) - want) <= tol).all()
