@@ -111,7 +111,7 @@ extern "C" int lbm_affine_ch_f32(const float* x, float* y, int64_t E, int32_t Ci
     const int vec = vec4 ? 4 : 1;
     const int tchunks = (T + kThreads * vec - 1) / (kThreads * vec);
     const int64_t bx = E * tchunks;
-    LBM_REQUIRE(bx <= 0x7fffffffLL, LBM_EUNSUPPORTED, "lbm_affine_ch_f32: grid too large");
+    LBM_REQUIRE(lbm::grid_fits(bx, kThreads), LBM_EUNSUPPORTED, "lbm_affine_ch_f32: grid too large");
     const dim3 grid((unsigned)bx, (unsigned)((Cout + kCoBlk - 1) / kCoBlk));
     const size_t lds = (size_t)(Cin * kCoBlk + kCoBlk) * sizeof(float);
     if (vec4)

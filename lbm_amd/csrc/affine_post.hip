@@ -268,7 +268,7 @@ extern "C" int lbm_affine_post_f32(const float* x, const float* A, const float* 
     if (E == 0) return LBM_OK;
     const int do_std = (standardize_mode == LBM_STD_EPOCH_CHANNEL && y_std != nullptr) ? 1 : 0;
     LBM_REQUIRE(x && A, LBM_EINVAL, "lbm_affine_post_f32: NULL pointer");
-    LBM_REQUIRE(E <= 0x7fffffffLL, LBM_EUNSUPPORTED, "lbm_affine_post_f32: grid too large");
+    LBM_REQUIRE(lbm::grid_fits(E, 64 * ((T + 127) / 128)), LBM_EUNSUPPORTED, "lbm_affine_post_f32: grid too large");
     LBM_REQUIRE(!(y_base == nullptr && !do_std && keep == nullptr && row_scale == nullptr), LBM_EINVAL, "lbm_affine_post_f32: no output requested");
     hipStream_t st = lbm::as_stream(stream);
     if (keep != nullptr) {

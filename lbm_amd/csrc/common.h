@@ -22,6 +22,9 @@ inline int check_launch(const char* what) {
     return LBM_OK;
 }
 
+// A launch of 2^32 threads and more along one dimension runs the rest beyond 2^32 only, and reports no error.
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= 0xffffffffLL / threads; }
+
 constexpr int kWave = 64;
 
 __device__ __forceinline__ float wave_sum(float v) {

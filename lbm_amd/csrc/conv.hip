@@ -602,7 +602,7 @@ int launch_tile(const float* x, const float* w, const float* bias, float* y, int
     const int ptiles = (Lout + Cfg::BN - 1) / Cfg::BN;
     const int mtiles = (Cout + BM - 1) / BM;
     const int64_t blocks = B * ptiles * mtiles;
-    if (blocks > 0x7fffffffLL) return lbm::fail(LBM_EUNSUPPORTED, "lbm_conv1d_f32: grid too large");
+    if (!lbm::grid_fits(blocks, kThreads)) return lbm::fail(LBM_EUNSUPPORTED, "lbm_conv1d_f32: grid too large");
     const size_t lds = Cfg::LDS_FLOATS * sizeof(float);
     const bool vec = (ldx % 4 == 0) && (ldy % 4 == 0) && ldx >= 4 && ((((uintptr_t)x) | ((uintptr_t)y)) & 15) == 0;
     auto k = vec ? conv_tile_kernel<KS, STRIDE, BM, 4, PM> : conv_tile_kernel<KS, STRIDE, BM, 1, PM>;
@@ -620,7 +620,7 @@ int launch_wino3(const float* x, const float* w, const float* bias, float* y, in
     const int ptiles = (Lout + BN - 1) / BN;
     const int mtiles = (Cout + WinoCfg::BM - 1) / WinoCfg::BM;
     const int64_t blocks = B * ptiles * mtiles;
-    if (blocks > 0x7fffffffLL) return lbm::fail(LBM_EUNSUPPORTED, "lbm_conv1d_f32: grid too large");
+    if (!lbm::grid_fits(blocks, kThreads)) return lbm::fail(LBM_EUNSUPPORTED, "lbm_conv1d_f32: grid too large");
     const size_t lds = WinoCfg::LDS_FLOATS * sizeof(float);
     const bool vec = (ldx % 4 == 0) && (ldy % 4 == 0) && ldx >= 4 && ((((uintptr_t)x) | ((uintptr_t)y)) & 15) == 0;
     auto k = utab ? (vec ? conv_wino3_kernel<4, true> : conv_wino3_kernel<1, true>) : (vec ? conv_wino3_kernel<4, false> : conv_wino3_kernel<1, false>);
@@ -669,7 +669,7 @@ extern "C" int lbm_conv1d_pitched_f32(const float* x, int64_t ldx, const float* 
     const int64_t Ntot = B * Lout;
     const int64_t gx = (Ntot + BN - 1) / BN;
     const int gy = (Cout + GBM - 1) / GBM;
-    LBM_REQUIRE(gx <= 0x7fffffffLL && gy <= 65535, LBM_EUNSUPPORTED, "lbm_conv1d_f32: grid too large");
+    LBM_REQUIRE(lbm::grid_fits(gx, kThreads) && gy <= 65535, LBM_EUNSUPPORTED, "lbm_conv1d_f32: grid too large");
     hipLaunchKernelGGL(conv1d_generic_kernel, dim3((unsigned)gx, (unsigned)gy), dim3(kThreads), 0, st, x, w, bias, y, Ntot, Cin,
                        Lin, ldx, Cout, Lout, ldy, ksize, stride, pad, relu);
     return lbm::check_launch("lbm_conv1d_f32");

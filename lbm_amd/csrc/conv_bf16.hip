@@ -273,7 +273,7 @@ extern "C" int lbm_conv1d_bf16x6_f32(const float* x, int64_t ldx, const void* ta
     const int64_t N = B * Lout64;
     const int64_t blocks = (N + kRows - 1) / kRows;
     LBM_REQUIRE(N < 0x7fffff00LL, LBM_EUNSUPPORTED, "lbm_conv1d_bf16x6_f32: B * Lout must be below 2^31");
-    LBM_REQUIRE(blocks <= 0x7fffffffLL, LBM_EUNSUPPORTED, "lbm_conv1d_bf16x6_f32: grid too large");
+    LBM_REQUIRE(lbm::grid_fits(blocks, kThreads), LBM_EUNSUPPORTED, "lbm_conv1d_bf16x6_f32: grid too large");
     ConvGeom g;
     g.Cin = Cin; g.CinP = p.CinP; g.Lin = Lin; g.Lout = (int)Lout64; g.Cout = Cout; g.ksize = ksize; g.stride = stride; g.pad = pad;
     g.relu = relu; g.ldx = (int)ldx; g.ldy = (int)ldy;

@@ -31,7 +31,7 @@ extern "C" int lbm_epochs_gather_f32(const float* raw, int64_t ldr, const int64_
     LBM_REQUIRE(raw && starts && out, LBM_EINVAL, "lbm_epochs_gather_f32: NULL pointer");
     const int64_t rows = E * C;
     const int64_t blocks = (rows + 3) / 4;
-    LBM_REQUIRE(blocks <= 0x7fffffffLL, LBM_EUNSUPPORTED, "lbm_epochs_gather_f32: grid too large");
+    LBM_REQUIRE(lbm::grid_fits(blocks, 256), LBM_EUNSUPPORTED, "lbm_epochs_gather_f32: grid too large");
     hipLaunchKernelGGL(epochs_gather_kernel, dim3((unsigned)blocks), dim3(256), 0, lbm::as_stream(stream), raw, ldr, starts, out,
                        rows, C, Tw, Trec);
     return lbm::check_launch("lbm_epochs_gather_f32");

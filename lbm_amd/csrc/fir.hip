@@ -106,7 +106,7 @@ extern "C" int lbm_fir_f32(const float* x, float* y, int64_t rows, int32_t T, co
     LBM_REQUIRE(lds <= 160 * 1024, LBM_EUNSUPPORTED, "lbm_fir_f32: ntaps=%d needs %zu B of LDS (max 163840)", ntaps, lds);
     const int tiles_per_row = (T + kTile - 1) / kTile;
     const int64_t blocks = rows * tiles_per_row;
-    LBM_REQUIRE(blocks <= 0x7fffffffLL, LBM_EUNSUPPORTED, "lbm_fir_f32: too many tiles (%lld)", (long long)blocks);
+    LBM_REQUIRE(lbm::grid_fits(blocks, kThreads), LBM_EUNSUPPORTED, "lbm_fir_f32: too many tiles (%lld)", (long long)blocks);
     if (lds > 64 * 1024) {
         hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fir_kernel),
                                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

@@ -210,7 +210,7 @@ extern "C" int lbm_ica_stats_f32(const float* z, int64_t ldz, int64_t T, int32_t
     LBM_REQUIRE(n <= 64, LBM_EUNSUPPORTED, "lbm_ica_stats_f32: n=%d components (at most 64)", n);
     LBM_REQUIRE(fun >= LBM_ICA_FUN_LOGCOSH && fun <= LBM_ICA_FUN_IDENTITY, LBM_EINVAL, "lbm_ica_stats_f32: unknown fun %d", fun);
     const Plan p = make_plan(T, n);
-    LBM_REQUIRE(p.nwg <= 0x7fffffffLL, LBM_EUNSUPPORTED, "lbm_ica_stats_f32: grid too large");
+    LBM_REQUIRE(lbm::grid_fits(p.nwg, 64 * kWaves), LBM_EUNSUPPORTED, "lbm_ica_stats_f32: grid too large");
     hipStream_t st = lbm::as_stream(stream);
     float* part = static_cast<float*>(workspace);
     const size_t lds = (size_t)kWaves * p.stride * sizeof(float);

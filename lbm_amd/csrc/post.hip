@@ -191,7 +191,7 @@ int launch_post(const float* x, float* y_base, float* y_std, uint8_t* keep, int6
     constexpr int BLOCK = TPR < 256 ? 256 : TPR;
     constexpr int RPB = BLOCK / TPR;
     const int64_t blocks = (rows + RPB - 1) / RPB;
-    if (blocks > 0x7fffffffLL) return lbm::fail(LBM_EUNSUPPORTED, "lbm_epoch_post_f32: grid too large");
+    if (!lbm::grid_fits(blocks, BLOCK)) return lbm::fail(LBM_EUNSUPPORTED, "lbm_epoch_post_f32: grid too large");
     const bool vec = (T % 4 == 0) && (((uintptr_t)x | (uintptr_t)y_base | (uintptr_t)y_std) & 15) == 0;
     if (vec)
         hipLaunchKernelGGL((post_kernel<TPR, kNV, 4>), dim3((unsigned)blocks), dim3(BLOCK), 0, st, x, y_base, y_std, keep,
@@ -232,7 +232,7 @@ int launch_channel_moments(const char* who, const float* x, const uint8_t* keep,
     const int64_t rows = E * C;
     if (rows > 0) {
         const int64_t blocks = (rows + 3) / 4;
-        if (blocks > 0x7fffffffLL) return lbm::fail(LBM_EUNSUPPORTED, "%s: grid too large", who);
+        if (!lbm::grid_fits(blocks, 256)) return lbm::fail(LBM_EUNSUPPORTED, "%s: grid too large", who);
         hipLaunchKernelGGL(row_moments_kernel, dim3((unsigned)blocks), dim3(256), 0, st, x, keep, row_ws, rows, C, T);
     }
     hipLaunchKernelGGL(channel_moments_kernel, dim3(C), dim3(256), 0, st, row_ws, keep, moments, E, C, T);
@@ -302,7 +302,7 @@ extern "C" int lbm_channel_scale_f32(const float* x, float* y, const float* mean
     LBM_REQUIRE(x && y && mean && scale, LBM_EINVAL, "lbm_channel_scale_f32: NULL pointer");
     const int64_t rows = E * C;
     const int64_t blocks = (rows + 3) / 4;
-    LBM_REQUIRE(blocks <= 0x7fffffffLL, LBM_EUNSUPPORTED, "lbm_channel_scale_f32: grid too large");
+    LBM_REQUIRE(lbm::grid_fits(blocks, 256), LBM_EUNSUPPORTED, "lbm_channel_scale_f32: grid too large");
     hipLaunchKernelGGL(channel_scale_kernel, dim3((unsigned)blocks), dim3(256), 0, lbm::as_stream(stream), x, y, mean, scale,
                        rows, C, T);
     return lbm::check_launch("lbm_channel_scale_f32");

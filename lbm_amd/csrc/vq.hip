@@ -404,7 +404,7 @@ int launch_vq(const float* x, int64_t ldx, int layout, int no_xnorm, int64_t S, 
               float* mind, int64_t N, int D, int K, hipStream_t st) {
     const size_t lds = ((size_t)kTileCodes * (DP + 4) + kTileCodes) * sizeof(float);
     const int64_t blocks = (N + kRowsPerBlock - 1) / kRowsPerBlock;
-    if (blocks > 0x7fffffffLL) return lbm::fail(LBM_EUNSUPPORTED, "lbm_vq_argmin_f32: grid too large");
+    if (!lbm::grid_fits(blocks, kThreads)) return lbm::fail(LBM_EUNSUPPORTED, "lbm_vq_argmin_f32: grid too large");
     const int vec_ok = (((uintptr_t)x & 15) == 0 && (ldx & 3) == 0) ? 1 : 0;
     hipError_t e;
     if (layout == LBM_VQ_ROWS) {
@@ -427,7 +427,7 @@ int launch_vq_dma(const float* x, int64_t ldx, int layout, int no_xnorm, int64_t
                   int64_t* idx_out, float* mind, int64_t N, int K, hipStream_t st) {
     const size_t lds = (size_t)2 * kDmaBufFloats * sizeof(float);
     const int64_t blocks = (N + kDmaRows - 1) / kDmaRows;
-    if (blocks > 0x7fffffffLL) return lbm::fail(LBM_EUNSUPPORTED, "lbm_vq_argmin_f32: grid too large");
+    if (!lbm::grid_fits(blocks, kDmaThreads)) return lbm::fail(LBM_EUNSUPPORTED, "lbm_vq_argmin_f32: grid too large");
     const int vec_ok = (((uintptr_t)x & 15) == 0 && (ldx & 3) == 0) ? 1 : 0;
     auto k = layout == LBM_VQ_ROWS ? vq_argmin_dma_kernel<LBM_VQ_ROWS> : vq_argmin_dma_kernel<LBM_VQ_CHANNEL_MAJOR>;
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -491,7 +491,7 @@ extern "C" int lbm_rownorm2_f32(const float* m, float* out, int64_t rows, int32_
     if (rows == 0) return LBM_OK;
     LBM_REQUIRE(m && out, LBM_EINVAL, "lbm_rownorm2_f32: NULL pointer");
     const int64_t blocks = (rows + 3) / 4;
-    LBM_REQUIRE(blocks <= 0x7fffffffLL, LBM_EUNSUPPORTED, "lbm_rownorm2_f32: grid too large");
+    LBM_REQUIRE(lbm::grid_fits(blocks, 256), LBM_EUNSUPPORTED, "lbm_rownorm2_f32: grid too large");
     hipLaunchKernelGGL(rownorm2_kernel, dim3((unsigned)blocks), dim3(256), 0, lbm::as_stream(stream), m, out, rows, D);
     return lbm::check_launch("lbm_rownorm2_f32");
 }

@@ -356,7 +356,7 @@ extern "C" int lbm_vq_argmin_bf16x6_f32(const float* x, int64_t ldx, int32_t lay
     const VqTabPlan p = vq_tab_plan(K, D);
     LBM_REQUIRE(p.piece_bytes / 16 < 0x7fffffffULL, LBM_EUNSUPPORTED, "lbm_vq_argmin_bf16x6_f32: table too large");
     const int64_t blocks = (N + kRows - 1) / kRows;
-    LBM_REQUIRE(blocks <= 0x7fffffffLL, LBM_EUNSUPPORTED, "lbm_vq_argmin_bf16x6_f32: grid too large");
+    LBM_REQUIRE(lbm::grid_fits(blocks, kThreads), LBM_EUNSUPPORTED, "lbm_vq_argmin_bf16x6_f32: grid too large");
     hipStream_t st = lbm::as_stream(stream);
     auto k = layout == LBM_VQ_ROWS ? vq_bf16x6_kernel<LBM_VQ_ROWS> : vq_bf16x6_kernel<LBM_VQ_CHANNEL_MAJOR>;
     hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, kLdsBytes);

@@ -616,6 +616,7 @@ extern "C" int lbm_vq_argmin_screened_f32(const float* x, int64_t ldx, int32_t l
     }
     const VqTabPlan p = vq_tab_plan(K, D);
     const int64_t blocks = (N + kSRows - 1) / kSRows;
+    LBM_REQUIRE(D == 256 || lbm::grid_fits(blocks, kSThreads), LBM_EUNSUPPORTED, "lbm_vq_argmin_screened_f32: grid too large");
     hipStream_t st = lbm::as_stream(stream);
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     int* row_count = reinterpret_cast<int*>(ws);

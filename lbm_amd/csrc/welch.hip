@@ -906,6 +906,7 @@ int welch_impl(const float* x, const float* row_scale, float* psd, float* seg_or
         hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(welch_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return lbm::fail(LBM_ELAUNCH, "lbm_welch_f32: hipFuncSetAttribute: %s", hipGetErrorString(e));
     }
+    LBM_REQUIRE(lbm::grid_fits(rows, kThreads), LBM_EUNSUPPORTED, "lbm_welch_f32: too many rows");
     hipLaunchKernelGGL(welch_kernel, dim3((unsigned)rows), dim3(kThreads), lds, lbm::as_stream(stream), x, row_scale, psd, seg_or_null, T,
                        (double)fs, nfft, nperseg, hop, nseg, tables, bin_lo, F, average_mode);
     return lbm::check_launch("lbm_welch_f32");
@@ -953,7 +954,7 @@ extern "C" int lbm_bandpower_f32(const float* psd, const float* freqs, float* ou
     const int64_t groups = per_channel ? E * C : E;
     const int n_elem = per_channel ? F : C * F;
     const int64_t blocks = (groups + 3) / 4;
-    LBM_REQUIRE(blocks <= 0x7fffffffLL, LBM_EUNSUPPORTED, "lbm_bandpower_f32: grid too large");
+    LBM_REQUIRE(lbm::grid_fits(blocks, 256), LBM_EUNSUPPORTED, "lbm_bandpower_f32: grid too large");
     hipLaunchKernelGGL(bandpower_kernel, dim3((unsigned)blocks), dim3(256), 0, lbm::as_stream(stream), psd, freqs, out, groups,
                        n_elem, F, already_db);
     return lbm::check_launch("lbm_bandpower_f32");
