@@ -272,8 +272,8 @@ extern "C" int lbm_affine_post_f32(const float* x, const float* A, const float* 
     LBM_REQUIRE(!(y_base == nullptr && !do_std && keep == nullptr && row_scale == nullptr), LBM_EINVAL, "lbm_affine_post_f32: no output requested");
     hipStream_t st = lbm::as_stream(stream);
     if (keep != nullptr) {
-        hipError_t err = hipMemsetAsync(keep, 1, (size_t)E, st);
-        if (err != hipSuccess) return lbm::fail(LBM_ELAUNCH, "lbm_affine_post_f32: memset keep: %s", hipGetErrorString(err));
+        const int rc = lbm::fill_bytes("lbm_affine_post_f32(keep)", keep, 1, E, st);
+        if (rc != LBM_OK) return rc;
     }
     // tiles per wave: the smallest NT that covers T with <= 8 waves (more, shorter waves spread the MFMA work over the SIMDs)
 #define LBM_AP_LAUNCH(KCH, NT) \

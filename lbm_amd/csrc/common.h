@@ -27,6 +27,16 @@ inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks <= 0xffff
 
 constexpr int kWave = 64;
 
+// n bytes set to v by a kernel: memset nodes of a captured graph have given wrong results on replays after the first
+static __global__ __launch_bounds__(256) void fill_bytes_kernel(uint8_t* p, uint8_t v, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = v;
+}
+inline int fill_bytes(const char* what, uint8_t* p, uint8_t v, int64_t n, hipStream_t st) {
+    const int64_t blocks = (n + 255) / 256;
+    hipLaunchKernelGGL(fill_bytes_kernel, dim3((unsigned)(blocks < 2048 ? blocks : 2048)), dim3(256), 0, st, p, v, n);
+    return check_launch(what);
+}
+
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

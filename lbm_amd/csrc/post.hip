@@ -214,8 +214,8 @@ extern "C" int lbm_epoch_post_f32(const float* x, float* y_base, float* y_std, u
     if (E == 0) return LBM_OK;
     hipStream_t st = lbm::as_stream(stream);
     if (keep != nullptr) {
-        hipError_t e = hipMemsetAsync(keep, 1, (size_t)E, st);
-        if (e != hipSuccess) return lbm::fail(LBM_ELAUNCH, "lbm_epoch_post_f32: memset keep: %s", hipGetErrorString(e));
+        const int rc = lbm::fill_bytes("lbm_epoch_post_f32(keep)", keep, 1, E, st);
+        if (rc != LBM_OK) return rc;
     }
     if (T == 0) return LBM_OK;
     LBM_REQUIRE(x != nullptr, LBM_EINVAL, "lbm_epoch_post_f32: NULL x");

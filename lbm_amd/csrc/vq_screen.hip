@@ -51,8 +51,10 @@ constexpr int kSSlotB = 2 * kSTile * 4;
 constexpr int kSLds = kSConst + 3 * kSSlotB;
 
 // cee[k] = ee[k] - beta |ee[k]| (the allowance for the fp32 roundings that form a score), +inf beyond K (padding codes never win)
-__global__ __launch_bounds__(256) void vq_screen_consts_kernel(const float* __restrict__ e_sqnorm, float* __restrict__ cee, int K, int Kp) {
+__global__ __launch_bounds__(256) void vq_screen_consts_kernel(const float* __restrict__ e_sqnorm, float* __restrict__ cee, int K, int Kp,
+                                                               int* __restrict__ row_count) {
     const int k = blockIdx.x * 256 + threadIdx.x;
+    if (k == 0) *row_count = 0;          // (no memset: its nodes in a captured graph have given wrong results on replays after the first)
     if (k >= Kp) return;
     const float e2 = k < K ? e_sqnorm[k] : INFINITY;
     cee[k] = k < K ? e2 - kBeta * fabsf(e2) : INFINITY;
@@ -622,9 +624,8 @@ extern "C" int lbm_vq_argmin_screened_f32(const float* x, int64_t ldx, int32_t l
     int* row_count = reinterpret_cast<int*>(ws);
     float* cee = reinterpret_cast<float*>(ws + 256);
     int64_t* row_list = reinterpret_cast<int64_t*>(ws + 256 + (size_t)p.Kp * sizeof(float));
-    hipError_t e = hipMemsetAsync(row_count, 0, 256, st);
-    if (e != hipSuccess) return lbm::fail(LBM_ELAUNCH, "lbm_vq_argmin_screened_f32: hipMemsetAsync: %s", hipGetErrorString(e));
-    hipLaunchKernelGGL(vq_screen_consts_kernel, dim3((unsigned)((p.Kp + 255) / 256)), dim3(256), 0, st, e_sqnorm, cee, K, p.Kp);
+    hipLaunchKernelGGL(vq_screen_consts_kernel, dim3((unsigned)((p.Kp + 255) / 256)), dim3(256), 0, st, e_sqnorm, cee, K, p.Kp,
+                       row_count);
     const unsigned char* tb = static_cast<const unsigned char*>(tables);
     const float* en_tab = reinterpret_cast<const float*>(tb + p.piece_bytes);
     const int vec_ok = (((uintptr_t)x & 15) == 0 && (ldx & 3) == 0) ? 1 : 0;

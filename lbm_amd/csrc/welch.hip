@@ -936,10 +936,10 @@ extern "C" int lbm_welch_keep_f32(const float* x, float* psd, uint8_t* keep, int
     LBM_REQUIRE(E >= 0 && C >= 1, LBM_EINVAL, "lbm_welch_keep_f32: bad sizes");
     if (E == 0) return LBM_OK;
     LBM_REQUIRE(keep != nullptr, LBM_EINVAL, "lbm_welch_keep_f32: NULL keep");
-    hipError_t e = hipMemsetAsync(keep, 1, (size_t)E, lbm::as_stream(stream));
-    if (e != hipSuccess) return lbm::fail(LBM_ELAUNCH, "lbm_welch_keep_f32: memset keep: %s", hipGetErrorString(e));
+    int rc = lbm::fill_bytes("lbm_welch_keep_f32(keep)", keep, 1, E, lbm::as_stream(stream));
+    if (rc != LBM_OK) return rc;
     bool fused = false;
-    const int rc = welch_impl(x, nullptr, psd, nullptr, E * C, T, fs, nfft, nperseg, noverlap, tables, bin_lo, bin_hi, LBM_AVG_MEAN, stream,
+    rc = welch_impl(x, nullptr, psd, nullptr, E * C, T, fs, nfft, nperseg, noverlap, tables, bin_lo, bin_hi, LBM_AVG_MEAN, stream,
                               keep, C, ptp_thresh, &fused);
     if (rc != LBM_OK || fused) return rc;
     // the launch above was not the team kernel: the reject test as its own pass (the post kernel in its mask-only form)
