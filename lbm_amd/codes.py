@@ -16,21 +16,26 @@ import torch
 
 from . import _lib
 
+_F32_MAX = torch.finfo(torch.float32).max
+
 
 # --------------------------------------------------------------------------------------------------------------- scores
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """[N, M] with unit stride along M and rows that do not overlap."""
-    return t.contiguous() if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < t.shape[1]) else t
+def _rows(t: torch.Tensor):
+    """[N, M] as (tensor with unit stride along M, row stride of M at least)."""
+    (n, m), (ld, unit) = t.shape, t.stride()
+    if unit != 1 or (n > 1 and ld < m):
+        t, ld = t.contiguous(), m
+    return t, (ld if n > 1 else m)
 
 
 class _CodeLogits(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, codebook, e_sqnorm, temperature):
+    def forward(ctx, x, ldx, codebook, e_sqnorm, temperature):
         N, D = x.shape
         K = codebook.shape[0]
         out = torch.empty((N, K), dtype=torch.float32, device=x.device)
-        _lib.check(_lib.load().lbm_code_logits_f32(_lib.ptr(x), x.stride(0) if N > 1 else D, _lib.VQ_ROWS, 0, _lib.ptr(codebook),
-                                                   _lib.ptr(e_sqnorm), out.data_ptr(), K, N, D, K, temperature, _lib.stream_ptr()),
+        _lib.check(_lib.load().lbm_code_logits_f32(_lib.ptr(x), ldx, _lib.VQ_ROWS, 0, _lib.ptr(codebook), _lib.ptr(e_sqnorm),
+                                                   out.data_ptr(), K, N, D, K, temperature, _lib.stream_ptr()),
                    "lbm_code_logits_f32")
         ctx.save_for_backward(x, codebook)
         ctx.temperature, ctx.norm_grad = temperature, e_sqnorm is None
@@ -40,19 +45,21 @@ class _CodeLogits(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         x, codebook = ctx.saved_tensors
-        need_x, need_e = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        need_x, _, need_e = ctx.needs_input_grad[:3]
         N, D = x.shape
         K = codebook.shape[0]
-        g, x, codebook = _rows(g), _rows(x), codebook.contiguous()       # (saved tensors come back in any layout from hooks that offload them)
+        # saved tensors come back in any layout from hooks that offload them
+        (g, ldg), (x, ldx), codebook = _rows(g), _rows(x), codebook.contiguous()
+        if not g.get_device() == x.get_device() == codebook.get_device():
+            raise _lib.LbmError("code_logits: saved tensors came back on another device")
         lib = _lib.load()
         dx = torch.empty((N, D), dtype=torch.float32, device=x.device) if need_x else None
         de = torch.empty((K, D), dtype=torch.float32, device=x.device) if need_e else None
         ws = torch.empty((lib.lbm_code_logits_grad_workspace_bytes(N, D, K),), dtype=torch.uint8, device=x.device)
-        _lib.check(lib.lbm_code_logits_grad_f32(_lib.ptr(g), g.stride(0) if N > 1 else K, _lib.ptr(x), x.stride(0) if N > 1 else D,
-                                                _lib.ptr(codebook), dx.data_ptr() if need_x else None, de.data_ptr() if need_e else None,
-                                                int(ctx.norm_grad), ws.data_ptr(), N, D, K, ctx.temperature,
-                                                _lib.stream_ptr()), "lbm_code_logits_grad_f32")
-        return dx, de, None, None
+        _lib.check(lib.lbm_code_logits_grad_f32(_lib.ptr(g), ldg, x.data_ptr(), ldx, codebook.data_ptr(), dx.data_ptr() if need_x else None,
+                                                de.data_ptr() if need_e else None, int(ctx.norm_grad), ws.data_ptr(), N, D, K,
+                                                ctx.temperature, _lib.stream_ptr()), "lbm_code_logits_grad_f32")
+        return dx, None, de, None, None
 
 
 def _f32_param(t, what):
@@ -77,7 +84,7 @@ def code_logits(x: torch.Tensor, codebook: torch.Tensor, temperature: float = 1.
     The backward pass reads ``x`` and ``codebook`` as they are then: hand it a copy of a codebook that an EMA step rewrites in between
     (``vq_ema_apply`` writes through raw pointers, which autograd's version check does not see)."""
     temperature = float(temperature)
-    if not (temperature > 0.0 and math.isfinite(temperature) and 2.0 / temperature <= torch.finfo(torch.float32).max):
+    if not (temperature > 0.0 and math.isfinite(temperature) and 2.0 / temperature <= _F32_MAX):
         raise ValueError(f"temperature must be positive and finite, and 2 / temperature in float32 too, got {temperature}")
     x, cb = _f32_param(x, "x"), _f32_param(codebook, "codebook").contiguous()
     if cb.dim() != 2 or cb.numel() == 0:
@@ -105,7 +112,7 @@ def code_logits(x: torch.Tensor, codebook: torch.Tensor, temperature: float = 1.
                                                            _lib.ptr(cb), _lib.ptr(ee), _lib.ptr(out), K, B * S, D, K, temperature,
                                                            _lib.stream_ptr()), "lbm_code_logits_f32")
             return out
-    return _CodeLogits.apply(_rows(x), cb, ee, temperature)
+    return _CodeLogits.apply(*_rows(x), cb, ee, temperature)
 
 
 # -------------------------------------------------------------------------------------------------------------- balance
@@ -153,9 +160,10 @@ class _CodeBalance(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g_loss, _g_counts, g_mean):
         scores, saved, counts = ctx.saved_tensors
-        # hooks that offload saved tensors bring them back in any layout
-        (scores, ld), saved, counts = _score_rows(scores, "code_balance_loss"), saved.contiguous(), counts.contiguous()
-        N, K = scores.shape
+        (N, K), (ld, unit) = scores.shape, scores.stride()
+        if K > 1 and unit != 1:              # saved tensors come back in any layout from hooks that offload them
+            scores, ld = scores.contiguous(), K
+        saved, counts = saved.contiguous(), counts.contiguous()
         ds = torch.empty((N, K), dtype=scores.dtype, device=scores.device)
         if g_mean is not None:
             g_mean = g_mean.contiguous()
@@ -179,7 +187,8 @@ def code_balance_loss(scores: torch.Tensor, codes: torch.Tensor = None, keep: to
     ``scores``: [..., K] float32, float16 or bfloat16 (K <= 8192).  ``codes``: integer [...] or [..., slots], the picks of each row (several for
     routers that pick several; negative ones, as ``sample_codes`` answers for empty rows, and ones >= K are not counted); without them the
     best score counts, lowest index first.  ``keep``: bool [...], rows to count (the pipeline's artifact mask, padding); the others' scores are
-    not read and their gradient is 0.  A row of nothing but -inf does not count either.  Where no row counts everything is 0."""
+    not read and their gradient is 0.  A row of nothing but -inf does not count either.  Where no row counts everything is 0.
+    Probabilities below the smallest normal float, 2^-126, are 0."""
     s, ld = _score_rows(scores, "code_balance_loss")
     lead = tuple(scores.shape[:-1])
     N = s.shape[0]
